@@ -178,6 +178,109 @@ int kvx_store(const void *key, const void *value, int64_t key_stride, int64_t va
               int num_heads, int head_bytes, const kvx_store_dest *dests, int n_dests, int32_t *status, int flags,
               void *stream);
 
+/* ---- norm, rotation and store in one pass ---- */
+
+/* Element types of rows, caches and queries. */
+#define KVX_BF16 0
+#define KVX_FP16 1
+
+/* A step's rows of one kind, [token][head][dim], by strides in bytes; a head's elements are contiguous. num_heads 0:
+ * there are none of this kind. */
+typedef struct kvx_rotate_rows {
+    const void *rows;
+    int64_t token_stride;
+    int64_t head_stride;
+    int32_t num_heads;
+    int32_t dim;          /* elements of a head's row */
+    int32_t norm_dim;     /* its leading elements that are normed (0: none) ... */
+    int32_t rotary_first; /* and the first rotated one (of kvx_rotate_args.rotary_dim) */
+    const void *weight;   /* norm_dim elements of the rows' type; NULL without a norm */
+} kvx_rotate_rows;
+
+typedef struct kvx_rotate_args {
+    kvx_rotate_rows query;    /* rotated into query_out */
+    kvx_rotate_rows key;      /* keys (or latents), rotated into the destinations' k_cache */
+    kvx_rotate_rows value;    /* values, stored as they are; none for latents */
+    void *query_out;          /* may be the queries' own rows */
+    int64_t out_token_stride; /* bytes */
+    int64_t out_head_stride;
+    const float *table;       /* device [num_positions][rotary_dim]: the cos of each of a position's rotary_dim / 2
+                                 angles, then their sin */
+    const void *positions;    /* device array of num_tokens positions */
+    int32_t num_positions;    /* a row whose position lies outside the table takes its nearest row and is flagged
+                                 (device error 8), unless its slot is -1 */
+    int32_t rotary_dim;       /* rotated elements per row (even; 0: none) */
+    int32_t interleaved;      /* pairs are (2p, 2p + 1); else (p, p + rotary_dim / 2) */
+    int32_t position_bytes;   /* 4 (int32) or 8 (int64) */
+    int32_t num_tokens;
+    int32_t dtype;            /* KVX_BF16 or KVX_FP16: rows, weights, query_out and caches */
+    float eps;
+    int32_t pad_;
+} kvx_rotate_args;
+
+/* One pass over a step's queries, keys and values: each head's norm, x * rsqrt(mean(x^2) + eps) * weight, the rotation
+ * of its pairs by its token's position, (a, b) -> (a cos - b sin, b cos + a sin), and the store of keys and values
+ * into every destination, as kvx_store places rows (its flags and status word too; bit 8 for a position outside the
+ * table). Computed in 32 bits and rounded once. What the reference's attention layers do ahead of store_kvcache
+ * (attention/triton_cache.py:58-91), in three passes. */
+int kvx_rotate_store(const kvx_rotate_args *args, const kvx_store_dest *dests, int n_dests, int32_t *status, int flags,
+                     void *stream);
+
+/* ---- attention over the paged cache ---- */
+
+typedef struct kvx_attention_args {
+    const void *query;          /* [num_tokens][q_heads][head_dim] by strides in bytes */
+    int64_t q_token_stride;
+    int64_t q_head_stride;
+    void *out;                  /* the same shape, by its own strides */
+    int64_t out_token_stride;
+    int64_t out_head_stride;
+    uint64_t k_cache;           /* device address of block 0's keys; strides in bytes over (block, token, head), */
+    uint64_t v_cache;           /* shared by keys and values: NHD and HND caches both work */
+    int64_t block_stride;
+    int64_t token_stride;
+    int64_t head_stride;
+    const int32_t *block_tables;/* device [batch][table_stride]: each sequence's block ids, max_blocks of them */
+    int64_t table_stride;       /* entries between sequences */
+    const int32_t *kv_lens;     /* device [batch]: each sequence's cached tokens, its query tokens included */
+    const int32_t *q_starts;    /* device [batch + 1]: where each sequence's query tokens begin; NULL: one each */
+    const float *slopes;        /* device [q_heads]: the bias slope * (key position - query position); NULL: none */
+    const int32_t *prefix_lens; /* device [batch]: every row sees the keys below it; NULL: none */
+    const int32_t *shared_table;/* device block ids of a prefix that every sequence has in front; NULL: none */
+    void *workspace;            /* kvx_attention_workspace_bytes() of device memory, its first
+                                   KVX_ATTENTION_ZEROED bytes zero before its first use; one launch at a time uses it */
+    int32_t *status;            /* status word or NULL: bit 2 for a block id past the cache or a length past its table,
+                                   bit 16 for a bounded wait that ran out */
+    int32_t shared_len;         /* tokens of the shared prefix */
+    int32_t shared_blocks;      /* entries of shared_table */
+    int32_t block_size;
+    int32_t num_blocks;
+    int32_t max_blocks;
+    int32_t batch;
+    int32_t num_tokens;
+    int32_t q_heads;
+    int32_t kv_heads;
+    int32_t head_dim;           /* 64 or 128 */
+    int32_t dtype;              /* KVX_BF16 or KVX_FP16 */
+    int32_t max_q_len;          /* the most query tokens of a sequence and the most cached ones, for the choice of */
+    int32_t max_kv_len;         /* launch shape: a wrong bound costs time, not correctness */
+    int32_t window;             /* a row sees its own position and the window - 1 before it; 0: all */
+    float scale;                /* scores are scale * q.k ... */
+    float softcap;              /* ... capped to softcap * tanh(score / softcap); 0: as they are */
+} kvx_attention_args;
+
+#define KVX_ATTENTION_ZEROED 65536
+
+uint64_t kvx_attention_workspace_bytes(void);
+
+/* Softmax attention of each sequence's query tokens over its keys and values in the paged cache. Query token i of n,
+ * in a sequence of kv_len, stands at position kv_len - n + i and sees position j when j <= its own, when the window
+ * holds it, or when j is below the sequence's prefix; a shared prefix lies in front of every sequence's own tokens,
+ * and every row sees all of it. A row that sees nothing gets zeros. Tokens at or past kv_len are never read as numbers;
+ * a block id outside the cache reads as zeros and is flagged. No counterpart in the reference's transfer path: it is
+ * what its attention layers read the cache with. */
+int kvx_attention(const kvx_attention_args *args, int flags, void *stream);
+
 /* ---- transfers with completion (post, poll, release) ---- */
 
 /* kvx_copy after `wait_event` (a cudaEvent_t as void*, may be 0) has passed on `stream`, then records a completion
@@ -266,9 +369,10 @@ int kvx_job_bytes(const kvx_cache *caches, int n_caches, const kvx_job *jobs, in
 
 /* Reads and clears, in one atomic step on the device, the diagnostic error word of the current device: 0, or the OR
  * of the errors kernels recorded since the last read -- 1 a copy's bounded TMA wait ran out (its bytes did not all
- * land), 2 a store slot or block id past its cache (skipped), 4 kvx_wait_selftest gave up as designed. Runs on a
- * stream of the library's own and waits on no other. Transfers are judged by their own status words, not by this
- * word: reading it (or not) changes no transfer's result. */
+ * land), 2 a store slot or block id past its cache (skipped), 4 kvx_wait_selftest gave up as designed, 8 a position
+ * outside its rotary table, 16 a bounded wait of an attention launch ran out. Runs on a stream of the library's own
+ * and waits on no other. Transfers are judged by their own status words, not by this word: reading it (or not) changes
+ * no transfer's result. */
 int kvx_device_error(int *out_code);
 
 /* Runs, on `stream`, the bounded wait that guards every TMA copy against a transfer that never arrives: one

@@ -26,6 +26,12 @@ KVX_ERR_TIMEOUT = -5
 STATUS_COPY_WAIT = 1  # a copy's bounded wait ran out: not every byte landed
 STATUS_PAST_CACHE = 2  # a store row whose slot or block lies past its cache was skipped
 STATUS_SELFTEST = 4  # kvx_wait_selftest gave up, as designed
+STATUS_POSITION = 8  # a row whose position lies outside its rotary table took the nearest row
+STATUS_ATTENTION_WAIT = 16  # a bounded wait of an attention launch ran out: its output is not to be used
+
+BF16 = 0  # element types of kvx_rotate_store and kvx_attention
+FP16 = 1
+ATTENTION_ZEROED = 65536  # leading bytes of an attention workspace that are zero before its first use
 
 STORE_SERIAL = 1  # kvx_store flag: a plain launch, no overlap with the kernel before it
 STORE_PEERS_ONLY = 4  # kvx_store flag: only the peer destinations are written (destination 0 places their rows)
@@ -122,6 +128,81 @@ class StoreDest(ctypes.Structure):
     ]
 
 
+class RotateRows(ctypes.Structure):
+    _fields_ = [
+        ("rows", ctypes.c_void_p),
+        ("token_stride", ctypes.c_int64),
+        ("head_stride", ctypes.c_int64),
+        ("num_heads", ctypes.c_int32),
+        ("dim", ctypes.c_int32),
+        ("norm_dim", ctypes.c_int32),
+        ("rotary_first", ctypes.c_int32),
+        ("weight", ctypes.c_void_p),
+    ]
+
+
+class RotateArgs(ctypes.Structure):
+    _fields_ = [
+        ("query", RotateRows),
+        ("key", RotateRows),
+        ("value", RotateRows),
+        ("query_out", ctypes.c_void_p),
+        ("out_token_stride", ctypes.c_int64),
+        ("out_head_stride", ctypes.c_int64),
+        ("table", ctypes.c_void_p),
+        ("positions", ctypes.c_void_p),
+        ("num_positions", ctypes.c_int32),
+        ("rotary_dim", ctypes.c_int32),
+        ("interleaved", ctypes.c_int32),
+        ("position_bytes", ctypes.c_int32),
+        ("num_tokens", ctypes.c_int32),
+        ("dtype", ctypes.c_int32),
+        ("eps", ctypes.c_float),
+        ("pad_", ctypes.c_int32),
+    ]
+
+
+class AttentionArgs(ctypes.Structure):
+    _fields_ = [
+        ("query", ctypes.c_void_p),
+        ("q_token_stride", ctypes.c_int64),
+        ("q_head_stride", ctypes.c_int64),
+        ("out", ctypes.c_void_p),
+        ("out_token_stride", ctypes.c_int64),
+        ("out_head_stride", ctypes.c_int64),
+        ("k_cache", ctypes.c_uint64),
+        ("v_cache", ctypes.c_uint64),
+        ("block_stride", ctypes.c_int64),
+        ("token_stride", ctypes.c_int64),
+        ("head_stride", ctypes.c_int64),
+        ("block_tables", ctypes.c_void_p),
+        ("table_stride", ctypes.c_int64),
+        ("kv_lens", ctypes.c_void_p),
+        ("q_starts", ctypes.c_void_p),
+        ("slopes", ctypes.c_void_p),
+        ("prefix_lens", ctypes.c_void_p),
+        ("shared_table", ctypes.c_void_p),
+        ("workspace", ctypes.c_void_p),
+        ("status", ctypes.c_void_p),
+        ("shared_len", ctypes.c_int32),
+        ("shared_blocks", ctypes.c_int32),
+        ("block_size", ctypes.c_int32),
+        ("num_blocks", ctypes.c_int32),
+        ("max_blocks", ctypes.c_int32),
+        ("batch", ctypes.c_int32),
+        ("num_tokens", ctypes.c_int32),
+        ("q_heads", ctypes.c_int32),
+        ("kv_heads", ctypes.c_int32),
+        ("head_dim", ctypes.c_int32),
+        ("dtype", ctypes.c_int32),
+        ("max_q_len", ctypes.c_int32),
+        ("max_kv_len", ctypes.c_int32),
+        ("window", ctypes.c_int32),
+        ("scale", ctypes.c_float),
+        ("softcap", ctypes.c_float),
+    ]
+
+
 # Every symbol include/kvx.h declares, with its argtypes and restype.
 _P = ctypes.c_void_p
 SIGNATURES: dict[str, tuple[list, object]] = {
@@ -140,6 +221,10 @@ SIGNATURES: dict[str, tuple[list, object]] = {
                      ctypes.c_int, ctypes.c_int, ctypes.c_int, ctypes.c_int, _P], ctypes.c_int),
     "kvx_store": ([_P, _P, ctypes.c_int64, ctypes.c_int64, ctypes.c_int, ctypes.c_int, ctypes.c_int,
                    ctypes.POINTER(StoreDest), ctypes.c_int, _P, ctypes.c_int, _P], ctypes.c_int),
+    "kvx_rotate_store": ([ctypes.POINTER(RotateArgs), ctypes.POINTER(StoreDest), ctypes.c_int, _P, ctypes.c_int, _P],
+                         ctypes.c_int),
+    "kvx_attention_workspace_bytes": ([], ctypes.c_uint64),
+    "kvx_attention": ([ctypes.POINTER(AttentionArgs), ctypes.c_int, _P], ctypes.c_int),
     "kvx_transfer": ([ctypes.POINTER(Cache), ctypes.c_int, ctypes.POINTER(Job), ctypes.c_int, ctypes.c_int, _P, _P,
                       ctypes.POINTER(ctypes.c_void_p)], ctypes.c_int),
     "kvx_transfer_after": ([ctypes.POINTER(Cache), ctypes.c_int, ctypes.POINTER(Job), ctypes.c_int, ctypes.c_int, _P,

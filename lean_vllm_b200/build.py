@@ -6,17 +6,20 @@ import os
 import shutil
 import subprocess
 import sys
+import tempfile
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(HERE)
-SOURCES = [os.path.join(HERE, "csrc", "kvx.cu")]
-HEADERS = [os.path.join(ROOT, "include", "kvx.h")]
+CSRC = os.path.join(HERE, "csrc")
+SOURCES = [os.path.join(CSRC, name) for name in ("kvx.cu", "rotary.cu", "attention.cu")]
+HEADERS = [os.path.join(ROOT, "include", "kvx.h"),
+           *(os.path.join(CSRC, name) for name in sorted(os.listdir(CSRC)) if name.endswith(".cuh"))]
 OUTPUT = os.path.join(HERE, "libkvx.so")
 
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",
     "-O3", "-lineinfo", "-std=c++17",
-    "-Xcompiler", "-fPIC", "-shared",
+    "-Xcompiler", "-fPIC",
     "-Xptxas", "-warn-spills",
 ]
 
@@ -38,11 +41,19 @@ def stale() -> bool:
 def build(force: bool = False, verbose: bool = False) -> str:
     if not force and not stale():
         return OUTPUT
-    cmd = [nvcc(), *NVCC_FLAGS, "-I", os.path.join(ROOT, "include"), "-o", OUTPUT + ".tmp", *SOURCES]
-    if verbose:
-        cmd.insert(1, "-Xptxas=-v")
-        print(" ".join(cmd))
-    subprocess.run(cmd, check=True)
+    # One object per source, compiled side by side, then linked; objects are rebuilt together with the library.
+    with tempfile.TemporaryDirectory(prefix="kvx_build_") as work:
+        objects = [os.path.join(work, os.path.basename(source) + ".o") for source in SOURCES]
+        compiles = [[nvcc(), *(["-Xptxas=-v"] if verbose else []), *NVCC_FLAGS, "-I", os.path.join(ROOT, "include"),
+                     "-c", "-o", obj, source] for source, obj in zip(SOURCES, objects)]
+        if verbose:
+            print("\n".join(" ".join(cmd) for cmd in compiles))
+        running = [subprocess.Popen(cmd) for cmd in compiles]
+        codes = [p.wait() for p in running]
+        for code, cmd in zip(codes, compiles):
+            if code:
+                raise subprocess.CalledProcessError(code, cmd)
+        subprocess.run([nvcc(), *NVCC_FLAGS, "-shared", "-o", OUTPUT + ".tmp", *objects], check=True)
     os.replace(OUTPUT + ".tmp", OUTPUT)
     return OUTPUT
 

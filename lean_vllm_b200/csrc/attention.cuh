@@ -1,0 +1,100 @@
+// What the attention kernels share: a launch's parameters, the mask, and the joining of partial results.
+#pragma once
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include "kvx_internal.cuh"
+
+namespace kvx {
+
+constexpr float kLog2e = 1.4426950408889634f;
+
+struct AttnParams {
+    uint64_t query, out, k_cache, v_cache;
+    int64_t q_token_stride, q_head_stride, out_token_stride, out_head_stride;  // bytes
+    int64_t block_stride, token_stride, head_stride;                           // bytes
+    const int32_t *block_tables, *kv_lens, *q_starts, *prefix_lens;
+    const float *slopes;
+    int64_t table_stride;
+    int32_t block_size, block_shift, num_blocks, max_blocks;  // block_shift: log2 of a power-of-two size, else -1
+    int32_t batch, num_tokens, q_heads, kv_heads, group;      // group: query heads a KV head
+    int32_t window;
+    float scale, softcap;
+    // Tokens that every sequence has in front of its own (rows see all of them), in blocks of their own; none when
+    // their part arrives as partial results.
+    const int32_t *shared_table;
+    int32_t shared_len;
+    int32_t *counters;
+    float *partial_o;    // [slot][row of the tile][dim]
+    float2 *partial_ml;  // [slot][row of the tile]: running maximum (log2 domain) and sum
+    // Partial results over a shared prefix, by split, query token and head; none when prefix_splits is 0.
+    const float *prefix_o;
+    const float2 *prefix_ml;
+    int32_t prefix_splits;
+    int32_t *status, *error_word;
+};
+
+// A sequence's query rows and cached tokens (a shared prefix's first), with its lengths brought into range.
+struct Sequence {
+    int32_t q0, q_len, kv_len, prefix;
+};
+
+__device__ __forceinline__ Sequence sequence_of(const AttnParams &p, int s) {
+    Sequence q;
+    q.q0 = p.q_starts ? p.q_starts[s] : s;
+    q.q_len = p.q_starts ? p.q_starts[s + 1] - q.q0 : 1;
+    q.q0 = max(q.q0, 0);
+    q.q_len = max(0, min(q.q_len, p.num_tokens - q.q0));
+    const int64_t room = (int64_t)p.max_blocks * p.block_size;
+    q.kv_len = (int32_t)min((int64_t)max(p.kv_lens[s], 0), room) + p.shared_len;
+    q.prefix = p.prefix_lens ? min(max(p.prefix_lens[s], 0), q.kv_len) : p.shared_len;
+    return q;
+}
+
+// Where sequence s keeps token t: a byte offset from the caches' first block and head, or -1 for a block id outside
+// the cache, which is flagged.
+__device__ __forceinline__ int64_t token_at(const AttnParams &p, int s, int32_t t) {
+    const int32_t *table = p.block_tables + (int64_t)s * p.table_stride;
+    if (t < p.shared_len) {
+        table = p.shared_table;
+    } else {
+        t -= p.shared_len;
+    }
+    const int32_t b = p.block_shift >= 0 ? t >> p.block_shift : t / p.block_size;
+    const int32_t id = table[b];
+    if (id < 0 || id >= p.num_blocks) {
+        flag_error(p.error_word, p.status, kErrPastCache);
+        return -1;
+    }
+    return (int64_t)id * p.block_stride + (int64_t)(t - b * p.block_size) * p.token_stride;
+}
+
+// The first key that any row from position `first_position` on can see.
+__device__ __forceinline__ int32_t first_seen(const AttnParams &p, const Sequence &q, int32_t first_position) {
+    return p.window > 0 && q.prefix == 0 ? max(0, first_position - p.window + 1) : 0;
+}
+
+// 2^x for a difference of running maxima: a maximum of -inf (nothing seen yet) contributes nothing.
+__device__ __forceinline__ float weight_of(float m, float reference) {
+    return m == -INFINITY ? 0.f : exp2f(m - reference);
+}
+
+template <class T>
+struct Pack2;
+template <>
+struct Pack2<__nv_bfloat16> {
+    static __device__ __forceinline__ uint32_t of(float lo, float hi) {
+        __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
+        return *reinterpret_cast<uint32_t *>(&v);
+    }
+};
+template <>
+struct Pack2<__half> {
+    static __device__ __forceinline__ uint32_t of(float lo, float hi) {
+        __half2 v = __floats2half2_rn(lo, hi);
+        return *reinterpret_cast<uint32_t *>(&v);
+    }
+};
+
+}  // namespace kvx

@@ -45,9 +45,7 @@
 #include <time.h>
 #include <unistd.h>
 
-#include <nvtx3/nvToolsExt.h>
-
-#include "kvx.h"
+#include "kvx_internal.cuh"
 
 namespace {
 
@@ -55,7 +53,11 @@ namespace {
 
 thread_local std::string t_error;
 
-int fail(int code, const char *fmt, ...) {
+std::atomic<uint64_t> g_launches{0};
+
+}  // namespace
+
+int kvx::fail(int code, const char *fmt, ...) {
     char buf[512];
     va_list ap;
     va_start(ap, fmt);
@@ -65,20 +67,20 @@ int fail(int code, const char *fmt, ...) {
     return code;
 }
 
-#define KVX_CUDA(call)                                                                                  \
-    do {                                                                                                \
-        cudaError_t e_ = (call);                                                                        \
-        if (e_ != cudaSuccess) return fail(KVX_ERR_CUDA, "%s failed: %s", #call, cudaGetErrorString(e_)); \
-    } while (0)
+void kvx::count_launch() { g_launches.fetch_add(1, std::memory_order_relaxed); }
 
-std::atomic<uint64_t> g_launches{0};
+namespace {
 
-// An NVTX range around each entry point that launches work, so a timeline (nsys, ncu's range view) shows which call
-// queued which kernels. Without a tool attached, NVTX calls are no-ops.
-struct Range {
-    explicit Range(const char *name) { nvtxRangePushA(name); }
-    ~Range() { nvtxRangePop(); }
-};
+using kvx::fail;
+using kvx::globaltimer;
+using kvx::kErrCopyWait;
+using kvx::kErrPastCache;
+using kvx::kErrSelftest;
+using kvx::kMaxStoreDests;
+using kvx::mbar_try_wait;
+using kvx::Range;
+using kvx::smem_u32;
+using kvx::StoreDest;
 
 // ------------------------------------------------------------------------------------------------ launch params
 
@@ -122,12 +124,6 @@ using SmallParams = ParamsOf<8, 160, 256>;
 static_assert(sizeof(Params) <= 32764, "kernel parameter space is 32764 bytes");
 static_assert(sizeof(SmallParams) <= 4096, "the compact parameter block stays within 4 KB");
 
-// Errors kernels record, as bits: a copy's bounded TMA wait ran out (its bytes did not all land), a store slot or
-// block id past its cache (skipped), the wait self-test gave up. Each goes into the launch's status word, when it
-// has one, and into the device's diagnostic word (read and cleared by kvx_device_error).
-constexpr int kErrCopyWait = 1;
-constexpr int kErrPastCache = 2;
-constexpr int kErrSelftest = 4;
 __device__ int g_device_error;
 
 // Records `code` for a launch. A status word is only ever given one code per launch, so a plain store suffices (no
@@ -242,28 +238,6 @@ __global__ void __launch_bounds__(kLsuThreads) kvx_copy_lsu(const __grid_constan
 
 constexpr uint64_t kWaitLimitNs = 2000000000ull;  // a bulk load that has not landed after 2 s is an error
 
-__device__ __forceinline__ uint64_t globaltimer() {
-    uint64_t t;
-    asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
-    return t;
-}
-
-__device__ __forceinline__ uint32_t smem_u32(const void *p) {
-    return static_cast<uint32_t>(__cvta_generic_to_shared(p));
-}
-
-__device__ __forceinline__ bool mbar_try_wait(uint32_t bar, uint32_t parity) {
-    uint32_t done;
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
-        "selp.u32 %0, 1, 0, p;\n\t}"
-        : "=r"(done)
-        : "r"(bar), "r"(parity)
-        : "memory");
-    return done != 0;
-}
-
 // Bounded wait on an mbarrier phase: false if it did not complete by `deadline` (globaltimer ns).
 __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, uint64_t deadline) {
     while (!mbar_try_wait(bar, parity)) {
@@ -376,17 +350,6 @@ __global__ void __launch_bounds__(32) kvx_copy_tma(const __grid_constant__ P p) 
 // source row [token][head] is read once and written to every destination whose head range holds it. Thread t of
 // the flattened space (token, K|V, head, vector) moves one VEC-byte vector, so reads of a token's rows are
 // contiguous and each (token, head) row lands as one contiguous run of head_bytes in every cache.
-constexpr int kMaxStoreDests = 9;  // the local cache and up to 8 decode ranks
-
-struct StoreDest {
-    uint64_t k, v;
-    int64_t block_stride, token_stride, head_stride;
-    const void *slots;
-    const int32_t *block_map;
-    int32_t block_size, num_blocks, slot_bytes, src_first_head, num_heads, dst_first_head, block_map_len;
-    int32_t block_shift;  // log2(block_size) when it is a power of two (the usual 16, 64, 256), else -1
-};
-
 struct StoreParams {
     uint64_t key, value;
     int64_t key_stride, value_stride;
@@ -564,6 +527,7 @@ __global__ void __launch_bounds__(kStoreThreads, 5) kvx_store_kernel(const __gri
 
 struct DeviceInfo {
     int sms = 0;
+    int32_t *error_word = nullptr;  // this device's g_device_error
     size_t tma_smem_set[2] = {};  // dynamic shared memory allowed for kvx_copy_tma<Params, SmallParams>
     int store_ctas_per_sm[5][2] = {};  // resident kvx_store_kernel<16, 8, 4, 2, 1; FAST> CTAs per SM
 };
@@ -1111,6 +1075,55 @@ bool same_process(const kvx_ipc_handle *h) {
 
 // ================================================================================================ C ABI
 
+int kvx::fill_dests(const kvx_store_dest *dests, int n_dests, int num_tokens, int num_heads, bool has_value,
+                    StoreDest *out, uint64_t *align_bits) {
+    if (n_dests < 1 || n_dests > kMaxStoreDests)
+        return fail(KVX_ERR_INVALID, "%d destinations; 1 to %d", n_dests, kMaxStoreDests);
+    for (int d = 0; d < n_dests; ++d) {
+        const kvx_store_dest &s = dests[d];
+        if (!s.k_cache || has_value != (s.v_cache != 0))
+            return fail(KVX_ERR_INVALID, "destination %d: keys and values must match the rows given", d);
+        if (s.block_size < 1 || s.num_blocks < 0 || (s.slot_bytes != 4 && s.slot_bytes != 8))
+            return fail(KVX_ERR_INVALID, "destination %d: bad block size, block count or slot width", d);
+        if (s.block_map && (d == 0 || s.block_size != dests[0].block_size || s.block_map_len < 0))
+            return fail(KVX_ERR_INVALID, "destination %d: a block map needs a later destination of equal block size",
+                        d);
+        if (num_tokens > 0 && !s.slot_mapping && !s.block_map)
+            return fail(KVX_ERR_INVALID, "destination %d: null slots", d);
+        if (s.src_first_head < 0 || s.num_heads < 0 || s.dst_first_head < 0 ||
+            (int64_t)s.src_first_head + s.num_heads > num_heads)
+            return fail(KVX_ERR_RANGE, "destination %d: heads [%d, +%d) of %d", d, s.src_first_head, s.num_heads,
+                        num_heads);
+        if (s.block_stride < 0 || s.token_stride < 0 || s.head_stride < 0)
+            return fail(KVX_ERR_INVALID, "destination %d: negative stride", d);
+        if ((int64_t)s.num_blocks * s.block_size >= (int64_t)1 << 31)
+            return fail(KVX_ERR_INVALID, "destination %d: more than 2^31 slots", d);
+        int32_t shift = -1;
+        for (int k = 0; k < 31; ++k)
+            if (s.block_size == (1 << k)) shift = k;
+        out[d] = StoreDest{s.k_cache, s.v_cache, s.block_stride, s.token_stride, s.head_stride, s.slot_mapping,
+                           s.block_map, s.block_size, s.num_blocks, s.slot_bytes, s.src_first_head, s.num_heads,
+                           s.dst_first_head, s.block_map_len, shift};
+        *align_bits |= s.k_cache | s.v_cache | (uint64_t)s.block_stride | (uint64_t)s.token_stride |
+                       (uint64_t)s.head_stride;
+    }
+    return KVX_OK;
+}
+
+int kvx::current_device(Device *out) {
+    DeviceInfo *info;
+    if (int rc = device_info(&info)) return rc;
+    KVX_CUDA(cudaGetDevice(&out->index));
+    if (!info->error_word) {
+        void *word;
+        KVX_CUDA(cudaGetSymbolAddress(&word, g_device_error));
+        info->error_word = static_cast<int32_t *>(word);
+    }
+    out->sms = info->sms;
+    out->error_word = info->error_word;
+    return KVX_OK;
+}
+
 extern "C" {
 
 int kvx_abi_version(void) { return KVX_ABI_VERSION; }
@@ -1270,8 +1283,6 @@ int kvx_store(const void *key, const void *value, int64_t key_stride, int64_t va
     if (num_tokens < 0 || num_heads < 1 || head_bytes < 1)
         return fail(KVX_ERR_INVALID, "bad row shape: %d tokens, %d heads of %d bytes", num_tokens, num_heads,
                     head_bytes);
-    if (n_dests < 1 || n_dests > kMaxStoreDests)
-        return fail(KVX_ERR_INVALID, "%d destinations; 1 to %d", n_dests, kMaxStoreDests);
     StoreParams p{};
     p.key = (uint64_t)(uintptr_t)key;
     p.value = (uint64_t)(uintptr_t)value;
@@ -1284,34 +1295,8 @@ int kvx_store(const void *key, const void *value, int64_t key_stride, int64_t va
     p.peers_only = (flags & KVX_STORE_PEERS_ONLY) ? 1 : 0;
     p.status = status;
     uint64_t align_bits = p.key | p.value | (uint64_t)key_stride | (uint64_t)value_stride | (uint64_t)head_bytes;
-    for (int d = 0; d < n_dests; ++d) {
-        const kvx_store_dest &s = dests[d];
-        if (!s.k_cache || (!value) != (!s.v_cache))
-            return fail(KVX_ERR_INVALID, "destination %d: keys and values must match the rows given", d);
-        if (s.block_size < 1 || s.num_blocks < 0 || (s.slot_bytes != 4 && s.slot_bytes != 8))
-            return fail(KVX_ERR_INVALID, "destination %d: bad block size, block count or slot width", d);
-        if (s.block_map && (d == 0 || s.block_size != dests[0].block_size || s.block_map_len < 0))
-            return fail(KVX_ERR_INVALID, "destination %d: a block map needs a later destination of equal block size",
-                        d);
-        if (num_tokens > 0 && !s.slot_mapping && !s.block_map)
-            return fail(KVX_ERR_INVALID, "destination %d: null slots", d);
-        if (s.src_first_head < 0 || s.num_heads < 0 || s.dst_first_head < 0 ||
-            (int64_t)s.src_first_head + s.num_heads > num_heads)
-            return fail(KVX_ERR_RANGE, "destination %d: heads [%d, +%d) of %d", d, s.src_first_head, s.num_heads,
-                        num_heads);
-        if (s.block_stride < 0 || s.token_stride < 0 || s.head_stride < 0)
-            return fail(KVX_ERR_INVALID, "destination %d: negative stride", d);
-        if ((int64_t)s.num_blocks * s.block_size >= (int64_t)1 << 31)
-            return fail(KVX_ERR_INVALID, "destination %d: more than 2^31 slots", d);
-        int32_t shift = -1;
-        for (int k = 0; k < 31; ++k)
-            if (s.block_size == (1 << k)) shift = k;
-        p.dests[d] = StoreDest{s.k_cache, s.v_cache, s.block_stride, s.token_stride, s.head_stride, s.slot_mapping,
-                               s.block_map, s.block_size, s.num_blocks, s.slot_bytes, s.src_first_head, s.num_heads,
-                               s.dst_first_head, s.block_map_len, shift};
-        align_bits |= s.k_cache | s.v_cache | (uint64_t)s.block_stride | (uint64_t)s.token_stride |
-                      (uint64_t)s.head_stride;
-    }
+    if (int rc = kvx::fill_dests(dests, n_dests, num_tokens, num_heads, value != nullptr, p.dests, &align_bits))
+        return rc;
     if (num_tokens == 0) return KVX_OK;
     const int vec = (int)std::min<uint64_t>(low_bit(align_bits), 16);
     DeviceInfo *info;

@@ -1,0 +1,302 @@
+"""kvx_attention on the GPU against the definition in 64 bits: lengths from nothing to long, masks that leave a row
+empty, garbage wherever nothing is to be read, layouts, streams and graphs."""
+
+import math
+
+import pytest
+import torch
+
+from lean_vllm_b200.attention.kvx_attention import AttentionWorkspace, paged_attention, shared_prefix_attention
+from lean_vllm_b200.kv_transfer import transport
+from tests.attention_cases import attention64, check_attention, paged_case
+
+pytestmark = pytest.mark.gpu
+
+BF16, FP16 = torch.bfloat16, torch.float16
+
+
+@pytest.fixture(scope="module")
+def workspace():
+    return AttentionWorkspace("cuda")
+
+
+def run(case, workspace, **options):
+    more = {}
+    if any(n != 1 for n in case["q_lens"]):
+        more = dict(q_starts=case["q_starts"], max_q_len=max(case["q_lens"]))
+    if case["shared"]:
+        return shared_prefix_attention(case["q"], case["k_cache"], case["v_cache"], case["prefix_table"],
+                                       case["shared"], case["tables"], case["kv_lens"], workspace=workspace, **more,
+                                       **options)
+    return paged_attention(case["q"], case["k_cache"], case["v_cache"], case["tables"], case["kv_lens"],
+                           workspace=workspace, **more, **options)
+
+
+def check(case, workspace, **options):
+    transport.device_error()
+    word = transport.StatusWord()
+    got = run(case, workspace, status=word.address, **options)
+    torch.cuda.synchronize()
+    assert word.bits() == 0 and transport.device_error() == 0
+    word.close()
+    check_attention(got, case, **options)
+    return got
+
+
+@pytest.mark.parametrize("kv_lens, heads, kv_heads, dim, block, dtype, hnd", [
+    ([1], 1, 1, 64, 16, BF16, True),
+    ([317], 32, 8, 128, 256, BF16, True),
+    ([1, 2, 15, 16, 17, 63, 64, 65, 127, 128, 129, 1000], 8, 2, 128, 16, BF16, True),
+    ([0, 5, 0, 700, 0], 4, 2, 64, 16, FP16, True),                    # nothing cached: zeros
+    ([333, 77], 14, 2, 64, 24, FP16, False),                          # 7 heads a KV head, 24-token blocks, NHD
+    ([401, 90, 3], 10, 2, 128, 256, BF16, False),                     # 5 heads a KV head
+    ([2500, 10], 32, 1, 128, 64, BF16, True),                         # one KV head for 32
+    ([130, 131], 3, 3, 128, 1, FP16, True),                           # one token a block, no grouping
+    ([255, 256, 257], 4, 4, 64, 7, BF16, False),                      # odd blocks
+    ([9000, 31, 4097], 8, 1, 128, 16, BF16, True),
+    ([40] * 200, 4, 1, 64, 16, BF16, True),                           # more sequences than threads that look at them
+], ids=lambda v: None if not isinstance(v, list) else f"{len(v)}x{max(v)}")
+def test_single_tokens(kv_lens, heads, kv_heads, dim, block, dtype, hnd, workspace):
+    check(paged_case([1] * len(kv_lens), kv_lens, heads, kv_heads, dim, block, dtype, hnd, fused=True), workspace)
+
+
+@pytest.mark.parametrize("q_lens, kv_lens, heads, kv_heads, dim, block, dtype, hnd", [
+    ([5], [5], 4, 1, 64, 16, BF16, True),                             # a whole prompt
+    ([300], [300], 8, 2, 128, 64, BF16, True),
+    ([129, 1, 0, 64, 3], [129, 500, 77, 1000, 3], 8, 2, 128, 16, BF16, True),  # chunks, single tokens, none
+    ([257, 128], [1000, 128], 14, 2, 64, 24, FP16, False),
+    ([700], [4099], 4, 1, 128, 256, FP16, True),
+    ([33, 40], [40, 300], 6, 2, 128, 5, BF16, True),                  # blocks of 5
+    ([4, 4, 4], [4, 600, 2100], 32, 4, 128, 16, BF16, True),          # drafted tokens
+    ([10], [3], 4, 2, 64, 16, BF16, True),                            # more queries than keys: the first see nothing
+], ids=lambda v: None if not isinstance(v, list) else f"{len(v)}x{max(v)}")
+def test_chunks(q_lens, kv_lens, heads, kv_heads, dim, block, dtype, hnd, workspace):
+    check(paged_case(q_lens, kv_lens, heads, kv_heads, dim, block, dtype, hnd), workspace)
+
+
+MASKS = {
+    "capped": dict(softcap=3.0),
+    "window": dict(window=100),
+    "window1": dict(window=1),
+    "bias": dict(slopes=True),
+    "prefix": dict(prefix_lens=True),
+    "all": dict(softcap=5.0, window=33, slopes=True, prefix_lens=True, scale=0.3),
+}
+
+
+@pytest.mark.parametrize("mask", MASKS)
+@pytest.mark.parametrize("q_lens, kv_lens, heads, kv_heads, dim, block, dtype", [
+    ([1, 1, 1, 1], [1, 64, 333, 1500], 8, 2, 128, 16, BF16),
+    ([1, 1], [1000, 100], 4, 4, 64, 24, FP16),
+    ([200, 7, 1], [260, 1003, 300], 8, 2, 128, 16, BF16),
+    ([513], [777], 7, 1, 64, 64, FP16),
+], ids=["decode128", "decode64", "chunks128", "chunk64"])
+def test_masks_caps_and_biases(q_lens, kv_lens, heads, kv_heads, dim, block, dtype, mask, workspace):
+    options = dict(MASKS[mask])
+    if options.get("slopes"):
+        options["slopes"] = 2.0 ** (-8.0 * torch.arange(1, heads + 1, device="cuda") / heads)
+    if options.get("prefix_lens"):
+        options["prefix_lens"] = torch.tensor([0, 50, 2000, 3][: len(kv_lens)] if len(kv_lens) > 1 else [300],
+                                              dtype=torch.int32, device="cuda")
+    case = paged_case(q_lens, kv_lens, heads, kv_heads, dim, block, dtype)
+    check(case, workspace, **options)
+
+
+def test_a_window_never_reads_what_lies_before_it(workspace):
+    """Blocks ahead of every row's window may be gone: their table entries are stale and their rows NaN."""
+    case = paged_case([1, 20], [1000, 700], 8, 2, 128, 16, BF16)
+    for s, (q_len, n) in enumerate(zip(case["q_lens"], [1000, 700])):
+        first = n - q_len - 100 + 1  # the first key that any row sees
+        ids = case["tables"][s]
+        for t in range(first):
+            b, o = int(ids[t // 16]), t % 16
+            case["k_cache"][b, o] = math.nan
+            case["v_cache"][b, o] = math.nan
+        case["tables"][s, : first // 16] = -1
+    check(case, workspace, window=100)
+
+
+@pytest.mark.parametrize("q_lens, kv_lens, shared, heads, kv_heads, dim, block, dtype, hnd", [
+    ([1] * 3, [1, 17, 40], 100, 8, 2, 128, 16, BF16, True),
+    ([1] * 64, list(range(1, 65)), 1000, 32, 8, 128, 256, BF16, True),
+    ([4] * 5, [4, 129, 60, 30, 5], 3001, 32, 8, 128, 16, BF16, True),
+    ([1, 3, 2], [20, 3, 77], 333, 14, 2, 64, 24, FP16, False),
+    ([1, 1], [5, 6], 1, 4, 1, 64, 7, FP16, True),                     # a prefix of one token, odd blocks
+    ([150, 1, 30], [150, 9, 400], 500, 8, 2, 128, 64, BF16, True),    # prompts behind a prefix
+    ([1], [7], 5000, 16, 1, 128, 64, FP16, False),
+    ([1] * 300, [3] * 300, 257, 8, 1, 64, 16, BF16, True),            # 2400 rows of one KV head
+], ids=lambda v: None if not isinstance(v, list) else f"{len(v)}x{max(v)}")
+@pytest.mark.parametrize("options", [{}, {"softcap": 4.0}, {"slopes": True}], ids=["plain", "capped", "bias"])
+def test_a_shared_prefix(q_lens, kv_lens, shared, heads, kv_heads, dim, block, dtype, hnd, options, workspace):
+    options = dict(options)
+    if options.get("slopes"):
+        options["slopes"] = 2.0 ** (-8.0 * torch.arange(1, heads + 1, device="cuda") / heads)
+    case = paged_case(q_lens, kv_lens, heads, kv_heads, dim, block, dtype, hnd, shared=shared)
+    check(case, workspace, **options)
+
+
+def test_a_shared_prefix_with_nothing_behind_it(workspace):
+    """kv_lens of 0: rows that see the prefix alone."""
+    case = paged_case([1, 1], [0, 0], 8, 2, 128, 16, BF16, shared=200)
+    case["q_lens"] = [1, 1]
+    check(case, workspace)
+
+
+def test_a_long_cache(workspace):
+    """One sequence of 100,003 tokens, all the parallelism from its length, and a prefix as long."""
+    check(paged_case([1], [100003], 8, 2, 128, 64, BF16), workspace)
+    check(paged_case([1, 2], [5, 9], 8, 2, 128, 64, BF16, shared=70001), workspace)
+
+
+def test_a_cache_past_four_gigabytes(workspace):
+    blocks = 9000
+    cache = torch.zeros(2, blocks, 8, 256, 128, dtype=BF16, device="cuda")  # 2 x 4.7 GB
+    view = cache.transpose(2, 3)
+    for q_len in (1, 100):
+        case = paged_case([q_len], [700], 8, 8, 128, 256, BF16, seed=q_len)
+        ids = torch.tensor([8999, 8500, 8700], dtype=torch.int32, device="cuda")
+        both = torch.stack([case["k_cache"], case["v_cache"]])[:, case["tables"][0].long()]
+        view[:, ids.long()] = both
+        case.update(k_cache=view[0], v_cache=view[1], tables=ids[None].contiguous())
+        check(case, workspace)
+
+
+def test_scores_far_apart_and_large_values(workspace):
+    """Scores in the hundreds (the running maximum grows from tile to tile) and keys that fall steadily."""
+    for q_len in (1, 150):
+        case = paged_case([q_len], [1500], 4, 1, 128, 16, BF16)
+        case["q"].mul_(30)
+        check(case, workspace)
+        ramp = torch.linspace(-1, 1, 1500, device="cuda")[:, None, None]
+        for sign in (1, -1):
+            case = paged_case([q_len], [1500], 4, 1, 128, 16, BF16)
+            keys = (torch.ones(1500, 1, 128, device="cuda") * ramp * sign).to(BF16)
+            case["keys"] = [keys]
+            i = torch.arange(1500, device="cuda")
+            case["k_cache"][case["tables"][0][i // 16].long(), i % 16] = keys
+            case["q"].abs_()
+            check(case, workspace)
+
+
+def test_block_ids_outside_the_cache_read_as_zeros_and_are_flagged(workspace):
+    for q_len in (1, 200):
+        case = paged_case([q_len], [500], 8, 2, 128, 16, BF16, garbage=False)
+        case["tables"][0, 3] = 10**6
+        case["tables"][0, 7] = -2
+        keys, values = case["keys"][0], case["values"][0]
+        for b in (3, 7):
+            keys[b * 16 : b * 16 + 16] = 0
+            values[b * 16 : b * 16 + 16] = 0
+        transport.device_error()
+        word = transport.StatusWord()
+        got = run(case, workspace, status=word.address)
+        torch.cuda.synchronize()
+        assert word.bits() == 2 and transport.device_error() == 2
+        word.close()
+        check_attention(got, case)
+
+
+def test_a_length_past_its_table_is_cut_and_flagged(workspace):
+    for q_len in (1, 40):
+        case = paged_case([q_len], [64], 8, 2, 128, 16, BF16)
+        case["kv_lens"][0] = 5000
+        transport.device_error()
+        word = transport.StatusWord()
+        got = run(case, workspace, status=word.address)
+        torch.cuda.synchronize()
+        assert word.bits() == 2 and transport.device_error() == 2
+        word.close()
+        check_attention(got, case)
+
+
+@pytest.mark.parametrize("q_lens, kv_lens, shared", [([1] * 7, [900, 1, 30, 5000, 77, 64, 128], 0),
+                                                      ([300, 1, 9], [4000, 700, 9], 0), ([1] * 9, [50] * 9, 3000)],
+                         ids=["decode", "chunks", "shared"])
+def test_the_same_call_gives_the_same_bits(q_lens, kv_lens, shared, workspace):
+    """Parts join in a fixed order whichever CTA joins them, and the bounds on the lengths change the shape of the launch
+    only: wrong ones cost time."""
+    case = paged_case(q_lens, kv_lens, 8, 2, 128, 16, BF16, shared=shared)
+    first = run(case, workspace)
+    for _ in range(5):
+        assert torch.equal(run(case, workspace), first)
+    for bound in (1, 100000):
+        check_attention(run(case, workspace, max_kv_len=bound), case)
+
+
+def test_wrong_bounds_on_the_query_lengths_are_harmless(workspace):
+    case = paged_case([70, 1, 200], [300, 900, 200], 8, 2, 128, 16, BF16)
+    for bound in (1, 2, 17, 10000):
+        got = paged_attention(case["q"], case["k_cache"], case["v_cache"], case["tables"], case["kv_lens"],
+                              q_starts=case["q_starts"], max_q_len=bound, workspace=workspace)
+        check_attention(got, case)
+
+
+def test_strided_queries_and_outputs(workspace):
+    for q_lens in ([1, 1], [90, 5]):
+        case = paged_case(q_lens, [200, 300], 6, 2, 128, 16, BF16, fused=True)
+        want = run(case, workspace)
+        wide = torch.zeros(sum(q_lens), 10, 128, dtype=BF16, device="cuda")
+        got = run(case, workspace, out=wide[:, 3:9])
+        assert got.data_ptr() == wide[:, 3:9].data_ptr() and torch.equal(got, want)
+        assert not wide[:, :3].any() and not wide[:, 9:].any()
+
+
+def test_no_tokens_launch_nothing(workspace):
+    case = paged_case([1], [5], 4, 2, 64, 16, BF16)
+    before = transport.launch_count()
+    out = paged_attention(case["q"][:0], case["k_cache"], case["v_cache"], case["tables"][:0], case["kv_lens"][:0],
+                          workspace=workspace)
+    assert out.shape == (0, 4, 64) and transport.launch_count() == before
+
+
+def test_other_streams(workspace):
+    """A side stream with a workspace of its own beside the current one, and a raw stream handle."""
+    for q_lens, kv_lens, shared in (([1, 1], [3000, 50], 0), ([200], [900], 0), ([1] * 8, [9] * 8, 2000)):
+        case = paged_case(q_lens, kv_lens, 8, 2, 128, 16, BF16, shared=shared)
+        want = run(case, workspace)
+        torch.cuda.synchronize()
+        side = torch.cuda.Stream()
+        with torch.cuda.stream(side):
+            own = AttentionWorkspace("cuda")
+            late = dict(case, q=torch.zeros_like(case["q"]))
+            for _ in range(20):
+                late["q"].copy_(case["q"])  # the queries arrive on this stream only
+            got = [run(late, own) for _ in range(3)]
+        here = [run(case, workspace) for _ in range(3)]
+        torch.cuda.synchronize()
+        assert all(torch.equal(x, want) for x in got + here)
+        raw = run(case, None, stream=side.cuda_stream)
+        side.synchronize()
+        assert torch.equal(raw, want)
+
+
+def test_a_graph_replays_the_call_at_other_lengths(workspace):
+    """Lengths live on the device: a captured call follows them."""
+    for q_lens, kv_lens, shared in (([1, 1, 1], [800, 300, 50], 0), ([64, 64], [500, 400], 0), ([1, 1], [40, 60], 700)):
+        case = paged_case(q_lens, kv_lens, 8, 2, 128, 16, BF16, shared=shared)
+        own = AttentionWorkspace("cuda")
+        out = torch.empty_like(case["q"])
+        run(case, own, out=out)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            run(case, own, out=out)
+        for shorter in (0, 3):
+            lens = [n - shorter for n in kv_lens]
+            case["kv_lens"].copy_(torch.tensor(lens, dtype=torch.int32))
+            now = dict(case, keys=[k[: shared + n] for k, n in zip(case["keys"], lens)],
+                       values=[v[: shared + n] for v, n in zip(case["values"], lens)])
+            for _ in range(2):
+                graph.replay()
+            torch.cuda.synchronize()
+            check_attention(out, now)
+
+
+def test_the_reference_notices_one_missing_key():
+    """The oracle's own check: leave out one key of 200 on the oracle's side and the row limit is passed."""
+    case = paged_case([1], [200], 4, 4, 128, 16, BF16)
+    want, _, _ = attention64(case)
+    check_attention(want.to(BF16), case)
+    wrong = dict(case, keys=[case["keys"][0][1:]], values=[case["values"][0][1:]])
+    with pytest.raises(AssertionError):
+        check_attention(attention64(wrong)[0].to(BF16), case)
