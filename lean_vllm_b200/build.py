@@ -11,7 +11,7 @@ import tempfile
 HERE = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(HERE)
 CSRC = os.path.join(HERE, "csrc")
-SOURCES = [os.path.join(CSRC, name) for name in ("kvx.cu", "rotary.cu", "attention.cu")]
+SOURCES = [os.path.join(CSRC, name) for name in ("kvx.cu", "rotary.cu", "attention.cu", "attention_tiles.cu")]
 HEADERS = [os.path.join(ROOT, "include", "kvx.h"),
            *(os.path.join(CSRC, name) for name in sorted(os.listdir(CSRC)) if name.endswith(".cuh"))]
 OUTPUT = os.path.join(HERE, "libkvx.so")

@@ -95,7 +95,9 @@ __device__ __forceinline__ RowWork row_work(const AttnParams &p, const Sequence 
 __device__ __forceinline__ int64_t row_units(const AttnParams &p, int s) {
     if (blockIdx.x == 0 && (int64_t)p.kv_lens[s] > (int64_t)p.max_blocks * p.block_size)
         flag_error(p.error_word, p.status, kErrPastCache);
-    const RowWork w = row_work(p, sequence_of(p, s));
+    const Sequence q = sequence_of(p, s);
+    if ((int64_t)q.q_len * p.group > p.rows_limit) return 0;  // attention_tiles takes it
+    const RowWork w = row_work(p, q);
     return w.groups(p) * w.tiles;
 }
 
@@ -177,7 +179,7 @@ __global__ void __launch_bounds__(kRowThreads, 2) attention_rows(const __grid_co
     while (unit < unit_end) {
         const Sequence q = sequence_of(p, s);
         const RowWork work = row_work(p, q);
-        const int64_t s_end = s_start + work.groups(p) * work.tiles;
+        const int64_t s_end = s_start + row_units(p, s);
         if (unit >= s_end) {
             s_start = s_end;
             ++s;
@@ -360,13 +362,13 @@ __global__ void __launch_bounds__(kRowThreads, 2) attention_rows(const __grid_co
                 const int64_t at = (int64_t)token * p.q_heads + head;
                 const int64_t step = (int64_t)p.num_tokens * p.q_heads;
                 float top = mm;
-                for (int i = 0; i < p.prefix_splits; ++i) top = fmaxf(top, p.prefix_ml[at + i * step].x);
+                for (int i = 0; i < p.prefix_splits; ++i) top = fmaxf(top, p.split_ml[at + i * step].x);
                 const float own = weight_of(mm, top);
                 ll *= own, acc.x *= own, acc.y *= own, acc.z *= own, acc.w *= own;
                 for (int i = 0; i < p.prefix_splits; ++i) {
-                    const float2 ml = p.prefix_ml[at + i * step];
+                    const float2 ml = p.split_ml[at + i * step];
                     const float f = weight_of(ml.x, top);
-                    const float4 x = reinterpret_cast<const float4 *>(p.prefix_o)[(at + i * step) * kQuads + quad];
+                    const float4 x = reinterpret_cast<const float4 *>(p.split_o)[(at + i * step) * kQuads + quad];
                     ll += f * ml.y;
                     acc.x += f * x.x, acc.y += f * x.y, acc.z += f * x.z, acc.w += f * x.w;
                 }
@@ -440,7 +442,9 @@ __global__ void __launch_bounds__(kRowThreads, 2) attention_rows(const __grid_co
 // ------------------------------------------------------------------------------------------------ host side
 
 constexpr size_t kRowPartials = (size_t)kMaxRowCtas * 2 * kRowTile;
-constexpr size_t kWorkspaceBytes = KVX_ATTENTION_ZEROED + kRowPartials * (128 * sizeof(float) + sizeof(float2));
+constexpr size_t kMlBytes = sizeof(float2), kOutBytes = 128 * sizeof(float);
+constexpr size_t kSplitAt = KVX_ATTENTION_ZEROED + kRowPartials * (kMlBytes + kOutBytes);
+constexpr size_t kWorkspaceBytes = kSplitAt + kSplitRows * (kMlBytes + kOutBytes);
 static_assert(kMaxRowCtas * sizeof(int32_t) <= KVX_ATTENTION_ZEROED, "a counter per CTA");
 
 template <class T, int D>
@@ -540,19 +544,50 @@ int kvx_attention(const kvx_attention_args *args, int flags, void *stream) {
     unsigned char *work = static_cast<unsigned char *>(a.workspace);
     p.counters = reinterpret_cast<int32_t *>(work);
     p.partial_ml = reinterpret_cast<float2 *>(work + KVX_ATTENTION_ZEROED);
-    p.partial_o = reinterpret_cast<float *>(work + KVX_ATTENTION_ZEROED + kRowPartials * sizeof(float2));
-    if (a.shared_len > 0) {
-        p.shared_table = a.shared_table;
-        p.shared_len = a.shared_len;
-    }
-    const bool mods = a.softcap > 0.f || a.slopes;
+    p.partial_o = reinterpret_cast<float *>(work + KVX_ATTENTION_ZEROED + kRowPartials * kMlBytes);
+    p.split_ml = reinterpret_cast<float2 *>(work + kSplitAt);
+    p.split_o = reinterpret_cast<float *>(work + kSplitAt + kSplitRows * kMlBytes);
+    p.shared_table = a.shared_table;
+    p.shared_len = a.shared_len;
+    p.rows_limit = INT32_MAX;
+    const bool mods = a.softcap > 0.f || a.slopes || !(a.scale > 0.f);
     cudaStream_t s = static_cast<cudaStream_t>(stream);
-    const bool bf16 = a.dtype == KVX_BF16;
-    if (a.head_dim == 128)
-        return bf16 ? launch_rows<__nv_bfloat16, 128>(p, mods, device.sms, s)
-                    : launch_rows<__half, 128>(p, mods, device.sms, s);
-    return bf16 ? launch_rows<__nv_bfloat16, 64>(p, mods, device.sms, s)
-                : launch_rows<__half, 64>(p, mods, device.sms, s);
+    auto rows_kernel = [&]() {
+        if (a.head_dim == 128)
+            return a.dtype == KVX_BF16 ? launch_rows<__nv_bfloat16, 128>(p, mods, device.sms, s)
+                                       : launch_rows<__half, 128>(p, mods, device.sms, s);
+        return a.dtype == KVX_BF16 ? launch_rows<__nv_bfloat16, 64>(p, mods, device.sms, s)
+                                   : launch_rows<__half, 64>(p, mods, device.sms, s);
+    };
+
+    // ---- which kernel takes what
+    const int64_t q_rows = (int64_t)std::max(a.max_q_len, 1) * p.group;  // of the longest sequence and one KV head
+    const int64_t all_rows = (int64_t)a.num_tokens * p.group;
+    // Splits of the keys that fill the device with one CTA per SM, two tiles of keys each at least, as many as the
+    // workspace has room for.
+    auto splits_for = [&](int64_t row_tiles, int64_t keys) {
+        const int64_t fill = device.sms / std::max<int64_t>(1, row_tiles * a.kv_heads);
+        const int64_t tiles = (keys + kTileKeys - 1) / kTileKeys;
+        return (int)std::max<int64_t>(
+            1, std::min({fill, (tiles + 1) / 2, kSplitRows / std::max<int64_t>(1, (int64_t)a.num_tokens * a.q_heads)}));
+    };
+    if (tile_box(p) == 0) return rows_kernel();
+    if (a.shared_len > 0 && q_rows <= kTileKeys && (int64_t)a.num_tokens * a.q_heads <= kSplitRows) {
+        // A prefix shared by short sequences: all their rows together against it, then each against its own keys.
+        const int splits = splits_for((all_rows + kTileRows - 1) / kTileRows, a.shared_len);
+        if (int rc = launch_tiles(p, a.head_dim, a.dtype, mods, true, splits, s)) return rc;
+        p.prefix_splits = splits;
+        p.shared_len = 0;
+        return rows_kernel();
+    }
+    if (q_rows <= kRowTile) return rows_kernel();
+    // Prompt chunks, and beside them (unless every sequence may be one) the sequences of few rows.
+    const bool mixed = a.batch > 1 && a.num_tokens < (int64_t)a.batch * a.max_q_len;
+    p.rows_limit = mixed ? kRowTile : 0;
+    const int64_t row_tiles = std::max<int64_t>(1, all_rows / kTileRows);
+    if (int rc = launch_tiles(p, a.head_dim, a.dtype, mods, false, splits_for(row_tiles, (int64_t)a.max_kv_len + a.shared_len), s))
+        return rc;
+    return mixed ? rows_kernel() : KVX_OK;
 }
 
 }  // extern "C"

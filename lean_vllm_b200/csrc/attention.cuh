@@ -28,12 +28,26 @@ struct AttnParams {
     int32_t *counters;
     float *partial_o;    // [slot][row of the tile][dim]
     float2 *partial_ml;  // [slot][row of the tile]: running maximum (log2 domain) and sum
-    // Partial results over a shared prefix, by split, query token and head; none when prefix_splits is 0.
-    const float *prefix_o;
-    const float2 *prefix_ml;
+    // Partial results of attention_tiles, [split][query token][head]: for rows whose keys it split, and for a shared
+    // prefix, which attention_rows joins in when prefix_splits is above 0.
+    float *split_o;
+    float2 *split_ml;
     int32_t prefix_splits;
+    // attention_rows takes the sequences of up to rows_limit query rows (query tokens x group), attention_tiles the rest.
+    int32_t rows_limit;
     int32_t *status, *error_word;
 };
+
+// attention_tiles (attention_tiles.cu). `prefix_only`: all query rows against the shared prefix alone, as partial
+// results of `splits`; else each sequence's rows above rows_limit, joined when splits is above 1.
+int launch_tiles(const AttnParams &p, int head_dim, int dtype, bool mods, bool prefix_only, int splits,
+                 cudaStream_t stream);
+// Whether attention_tiles can read this cache, and the tokens a copy of it brings at once.
+int tile_box(const AttnParams &p);
+
+constexpr int kTileRows = 256;
+constexpr int kTileKeys = 128;
+constexpr int64_t kSplitRows = 131072;  // rows of partial results the workspace holds
 
 // A sequence's query rows and cached tokens (a shared prefix's first), with its lengths brought into range.
 struct Sequence {
