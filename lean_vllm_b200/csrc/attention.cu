@@ -355,51 +355,36 @@ __global__ void __launch_bounds__(kRowThreads, 2) attention_rows(const __grid_co
         constexpr int kWarpFloats = kRowStages * 2 * kStageBytes / 4;
         const float *all_o = reinterpret_cast<const float *>(smem);
 
-        // Writes a row's four elements, after the parts over a shared prefix.
-        auto finish = [&](int row, int quad, float mm, float ll, float4 acc) {
+        // Writes a row's four elements, after joining the parts over a shared prefix.
+        auto finish = [&](int row, int quad, Joined j) {
             const int token = q.q0 + (row0 + row) / p.group, head = h * p.group + (row0 + row) % p.group;
-            if (p.prefix_splits > 0) {
-                const int64_t at = (int64_t)token * p.q_heads + head;
-                const int64_t step = (int64_t)p.num_tokens * p.q_heads;
-                float top = mm;
-                for (int i = 0; i < p.prefix_splits; ++i) top = fmaxf(top, p.split_ml[at + i * step].x);
-                const float own = weight_of(mm, top);
-                ll *= own, acc.x *= own, acc.y *= own, acc.z *= own, acc.w *= own;
-                for (int i = 0; i < p.prefix_splits; ++i) {
-                    const float2 ml = p.split_ml[at + i * step];
-                    const float f = weight_of(ml.x, top);
-                    const float4 x = reinterpret_cast<const float4 *>(p.split_o)[(at + i * step) * kQuads + quad];
-                    ll += f * ml.y;
-                    acc.x += f * x.x, acc.y += f * x.y, acc.z += f * x.z, acc.w += f * x.w;
-                }
-            }
-            const float inverse = ll == 0.f ? 0.f : 1.f / ll;  // a row that sees nothing gets zeros
+            const int64_t at = (int64_t)token * p.q_heads + head, step = (int64_t)p.num_tokens * p.q_heads;
+            join_parts(j, p.prefix_splits, p.split_ml, p.split_o, kQuads, quad, [&](int i) { return at + i * step; });
+            const float inverse = j.sum == 0.f ? 0.f : 1.f / j.sum;  // a row that sees nothing gets zeros
             char *out = reinterpret_cast<char *>(p.out + (int64_t)token * p.out_token_stride +
                                                  (int64_t)head * p.out_head_stride) + quad * 8;
-            *reinterpret_cast<uint2 *>(out) = make_uint2(Pack2<T>::of(acc.x * inverse, acc.y * inverse),
-                                                         Pack2<T>::of(acc.z * inverse, acc.w * inverse));
+            *reinterpret_cast<uint2 *>(out) = make_uint2(Pack2<T>::of(j.o.x * inverse, j.o.y * inverse),
+                                                         Pack2<T>::of(j.o.z * inverse, j.o.w * inverse));
         };
 
         if (whole && p.prefix_splits > 0) wait_prerequisites();
         for (int item = tid; item < rows * kQuads; item += kRowThreads) {
             const int row = item / kQuads, quad = item % kQuads;
-            float top = -INFINITY;
+            Joined j;
 #pragma unroll
-            for (int w = 0; w < kRowWarps; ++w) top = fmaxf(top, warp_ml[w][row].x);
-            float ll = 0.f;
-            float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+            for (int w = 0; w < kRowWarps; ++w) j.top = fmaxf(j.top, warp_ml[w][row].x);
 #pragma unroll
             for (int w = 0; w < kRowWarps; ++w) {
-                const float f = weight_of(warp_ml[w][row].x, top);
+                const float f = weight_of(warp_ml[w][row].x, j.top);
                 const float4 x = reinterpret_cast<const float4 *>(all_o + w * kWarpFloats + row * D)[quad];
-                ll += f * warp_ml[w][row].y;
-                acc.x += f * x.x, acc.y += f * x.y, acc.z += f * x.z, acc.w += f * x.w;
+                j.sum += f * warp_ml[w][row].y;
+                j.o.x += f * x.x, j.o.y += f * x.y, j.o.z += f * x.z, j.o.w += f * x.w;
             }
             if (whole) {
-                finish(row, quad, top, ll, acc);
+                finish(row, quad, j);
             } else {
-                reinterpret_cast<float4 *>(p.partial_o)[(int64_t)(slot * kRowTile + row) * kQuads + quad] = acc;
-                if (quad == 0) p.partial_ml[slot * kRowTile + row] = make_float2(top, ll);
+                reinterpret_cast<float4 *>(p.partial_o)[(int64_t)(slot * kRowTile + row) * kQuads + quad] = j.o;
+                if (quad == 0) p.partial_ml[slot * kRowTile + row] = make_float2(j.top, j.sum);
             }
         }
         if (!whole) {
@@ -416,20 +401,10 @@ __global__ void __launch_bounds__(kRowThreads, 2) attention_rows(const __grid_co
                 if (p.prefix_splits > 0) wait_prerequisites();
                 for (int item = tid; item < rows * kQuads; item += kRowThreads) {
                     const int row = item / kQuads, quad = item % kQuads;
-                    float top = -INFINITY;
-                    for (int c = c0; c <= c1; ++c)
-                        top = fmaxf(top, __ldcg(&p.partial_ml[(2 * c + (c == c0)) * kRowTile + row].x));
-                    float ll = 0.f;
-                    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-                    for (int c = c0; c <= c1; ++c) {
-                        const int at = (2 * c + (c == c0)) * kRowTile + row;
-                        const float2 ml = __ldcg(&p.partial_ml[at]);
-                        const float f = weight_of(ml.x, top);
-                        const float4 x = __ldcg(&reinterpret_cast<const float4 *>(p.partial_o)[(int64_t)at * kQuads + quad]);
-                        ll += f * ml.y;
-                        acc.x += f * x.x, acc.y += f * x.y, acc.z += f * x.z, acc.w += f * x.w;
-                    }
-                    finish(row, quad, top, ll, acc);
+                    Joined j;
+                    join_parts(j, c1 - c0 + 1, p.partial_ml, p.partial_o, kQuads, quad,
+                               [&](int i) { return (int64_t)(2 * (c0 + i) + (i == 0)) * kRowTile + row; });
+                    finish(row, quad, j);
                 }
             }
         }

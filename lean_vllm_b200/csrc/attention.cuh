@@ -94,6 +94,45 @@ __device__ __forceinline__ float weight_of(float m, float reference) {
     return m == -INFINITY ? 0.f : exp2f(m - reference);
 }
 
+// The running join of partial results of one row: four of its output elements, relative to the maximum `top`.
+struct Joined {
+    float top = -INFINITY, sum = 0.f;
+    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+};
+
+// Joins n more parts in order; at(i) is part i's row index into `ml`, of [row][quads] float4 in `o`. Eight parts' loads
+// are in flight at once: one after another, each would wait for the L2 cache (0.5 us), 18 of them for 10 us.
+template <class At>
+__device__ __forceinline__ void join_parts(Joined &j, int n, const float2 *ml, const float *o, int quads, int quad, At at) {
+    constexpr int kAtOnce = 8;
+    for (int i0 = 0; i0 < n; i0 += kAtOnce) {
+        float2 part[kAtOnce];
+        float4 x[kAtOnce];
+#pragma unroll
+        for (int k = 0; k < kAtOnce; ++k) {
+            part[k] = make_float2(-INFINITY, 0.f);
+            x[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (i0 + k < n) {
+                const int64_t row = at(i0 + k);
+                part[k] = __ldcg(&ml[row]);
+                x[k] = __ldcg(reinterpret_cast<const float4 *>(o) + row * quads + quad);
+            }
+        }
+        float top = j.top;
+#pragma unroll
+        for (int k = 0; k < kAtOnce; ++k) top = fmaxf(top, part[k].x);
+        const float own = weight_of(j.top, top);
+        j.top = top;
+        j.sum *= own, j.o.x *= own, j.o.y *= own, j.o.z *= own, j.o.w *= own;
+#pragma unroll
+        for (int k = 0; k < kAtOnce; ++k) {
+            const float f = weight_of(part[k].x, top);
+            j.sum += f * part[k].y;
+            j.o.x += f * x[k].x, j.o.y += f * x[k].y, j.o.z += f * x[k].z, j.o.w += f * x[k].w;
+        }
+    }
+}
+
 template <class T>
 struct Pack2;
 template <>

@@ -154,6 +154,12 @@ __device__ __forceinline__ float exp2_fast(float x) {
     return y;
 }
 
+__device__ __forceinline__ float reciprocal_fast(float x) {
+    float y;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
 // Waits for a phase of `bar`, for as long as no wait of the CTA has run out.
 __device__ __forceinline__ bool wait_phase(uint32_t bar, uint32_t parity, volatile int *gave_up) {
     if (mbar_try_wait(bar, parity)) return true;
@@ -357,9 +363,10 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tiles(const __grid_cons
                 see_below = item.q.prefix - p.shared_len;
                 position = stands + p.shared_len;
             }
-            if (MODS && p.slopes && valid) slope = p.slopes[head];
+            if (MODS && p.slopes && valid) slope = p.slopes[head] * kLog2e;
 
             const float scale_log2 = p.scale * kLog2e;
+            const float cap_in = p.softcap > 0.f ? scale_log2 * 2.f / p.softcap : 0.f, cap_out = p.softcap * kLog2e;
             const uint32_t s_tmem = tmem + ((uint32_t)(warp & 3) << 21) + g * 128;
             const uint32_t o_tmem = tmem + ((uint32_t)(warp & 3) << 21) + S::kOutColumn + g * D;
             float m = -INFINITY, sum[4] = {0.f, 0.f, 0.f, 0.f};
@@ -381,13 +388,14 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tiles(const __grid_cons
                     for (int c = 0; c < 4; ++c)
 #pragma unroll
                         for (int e = 0; e < 32; ++e) {
-                            float y = x[c][e] * p.scale;
+                            float y;  // the score times log2(e)
                             if (p.softcap > 0.f) {
-                                // tanh(z) = 1 - 2 / (e^2z + 1): exact to 2^-22 of 1, where the exponent's error counts
-                                const float z = exp2_fast(y * (2.f * kLog2e / p.softcap));
-                                y = p.softcap - 2.f * p.softcap * __frcp_rn(z + 1.f);
+                                // tanh(z) = 1 - 2 / (e^2z + 1), to 2^-22 of the cap, where the exponent's error counts
+                                y = cap_out - 2.f * cap_out * reciprocal_fast(exp2_fast(x[c][e] * cap_in) + 1.f);
+                            } else {
+                                y = x[c][e] * scale_log2;
                             }
-                            x[c][e] = (y + slope * (float)(offset + c * 32 + e)) * kLog2e;
+                            x[c][e] = y + slope * (float)(offset + c * 32 + e);
                         }
                 }
                 const float unit = MODS ? 1.f : scale_log2;
@@ -663,21 +671,12 @@ __global__ void __launch_bounds__(kJoinThreads) attention_join(const __grid_cons
         const int r = item.row0 + in_item, token = r / p.group;
         const int head = item.head * p.group + r - token * p.group;
         const int64_t at = (int64_t)(item.q.q0 + token) * p.q_heads + head;
-        float top = -INFINITY;
-        for (int s = 0; s < t.splits; ++s) top = fmaxf(top, p.split_ml[at + s * step].x);
-        float total = 0.f;
-        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-        for (int s = 0; s < t.splits; ++s) {
-            const float2 ml = p.split_ml[at + s * step];
-            const float f = weight_of(ml.x, top);
-            const float4 x = reinterpret_cast<const float4 *>(p.split_o)[(at + s * step) * kQuads + quad];
-            total += f * ml.y;
-            acc.x += f * x.x, acc.y += f * x.y, acc.z += f * x.z, acc.w += f * x.w;
-        }
-        const float inverse = total == 0.f ? 0.f : 1.f / total;
+        Joined j;
+        join_parts(j, t.splits, p.split_ml, p.split_o, kQuads, quad, [&](int i) { return at + i * step; });
+        const float inverse = j.sum == 0.f ? 0.f : 1.f / j.sum;
         *reinterpret_cast<uint2 *>(p.out + (int64_t)(item.q.q0 + token) * p.out_token_stride +
                                    (int64_t)head * p.out_head_stride + quad * 8) =
-            make_uint2(Pack2<T>::of(acc.x * inverse, acc.y * inverse), Pack2<T>::of(acc.z * inverse, acc.w * inverse));
+            make_uint2(Pack2<T>::of(j.o.x * inverse, j.o.y * inverse), Pack2<T>::of(j.o.z * inverse, j.o.w * inverse));
     }
 }
 
