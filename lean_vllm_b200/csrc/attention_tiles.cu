@@ -123,6 +123,18 @@ __device__ __forceinline__ void load16(uint32_t address, uint32_t (&r)[16]) {
         : "r"(address));
 }
 
+__device__ __forceinline__ void store32(uint32_t address, const float (&r)[32]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
+        "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, "
+        "%17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};" ::"r"(address),
+        "f"(r[0]), "f"(r[1]), "f"(r[2]), "f"(r[3]), "f"(r[4]), "f"(r[5]), "f"(r[6]), "f"(r[7]), "f"(r[8]), "f"(r[9]),
+        "f"(r[10]), "f"(r[11]), "f"(r[12]), "f"(r[13]), "f"(r[14]), "f"(r[15]), "f"(r[16]), "f"(r[17]), "f"(r[18]),
+        "f"(r[19]), "f"(r[20]), "f"(r[21]), "f"(r[22]), "f"(r[23]), "f"(r[24]), "f"(r[25]), "f"(r[26]), "f"(r[27]),
+        "f"(r[28]), "f"(r[29]), "f"(r[30]), "f"(r[31])
+        : "memory");
+}
+
 __device__ __forceinline__ void store16(uint32_t address, const uint32_t (&r)[16]) {
     asm volatile(
         "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
@@ -158,6 +170,35 @@ __device__ __forceinline__ float reciprocal_fast(float x) {
     float y;
     asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
+}
+
+// Two 32-bit operations in one instruction.
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+    float2 d;
+    asm("{\n\t.reg .b64 a, b, c, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tmov.b64 c, {%6, %7};\n\t"
+        "fma.rn.f32x2 d, a, b, c;\n\tmov.b64 {%0, %1}, d;\n\t}"
+        : "=f"(d.x), "=f"(d.y)
+        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+    return d;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+    float2 d;
+    asm("{\n\t.reg .b64 a, b, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\t"
+        "add.rn.f32x2 d, a, b;\n\tmov.b64 {%0, %1}, d;\n\t}"
+        : "=f"(d.x), "=f"(d.y)
+        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return d;
+}
+
+__device__ __forceinline__ float max_of(float top, const float (&x)[32]) {
+    float a = top, b = x[0];
+#pragma unroll
+    for (int e = 1; e + 3 < 32; e += 4) {
+        asm("max.f32 %0, %0, %1, %2;" : "+f"(a) : "f"(x[e]), "f"(x[e + 1]));
+        asm("max.f32 %0, %0, %1, %2;" : "+f"(b) : "f"(x[e + 2]), "f"(x[e + 3]));
+    }
+    asm("max.f32 %0, %0, %1, %2;" : "+f"(a) : "f"(x[29]), "f"(x[30]));
+    return fmaxf(fmaxf(a, b), x[31]);
 }
 
 // Waits for a phase of `bar`, for as long as no wait of the CTA has run out.
@@ -369,7 +410,8 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tiles(const __grid_cons
             const float cap_in = p.softcap > 0.f ? scale_log2 * 2.f / p.softcap : 0.f, cap_out = p.softcap * kLog2e;
             const uint32_t s_tmem = tmem + ((uint32_t)(warp & 3) << 21) + g * 128;
             const uint32_t o_tmem = tmem + ((uint32_t)(warp & 3) << 21) + S::kOutColumn + g * D;
-            float m = -INFINITY, sum[4] = {0.f, 0.f, 0.f, 0.f};
+            float m = -INFINITY;
+            float2 sum = make_float2(0.f, 0.f);
             bool ok = true;
             for (int i = 0; i < n_tiles; ++i) {
                 const TileAt at = tile_at(p, item, i);
@@ -378,55 +420,60 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tiles(const __grid_cons
                     break;
                 }
                 fence_after();
-                float x[4][32];
-#pragma unroll
-                for (int c = 0; c < 4; ++c) load32(s_tmem + c * 32, x[c]);
+                // First pass: the tile's maximum. Scores that a mask, cap or bias changes go back to TMEM as they are then.
+                const bool sees_all = !valid ? true
+                                      : at.shared ? at.t0 + kTileKeys <= p.shared_len
+                                                  : (at.t0 >= see_lo && at.t0 + kTileKeys <= see_hi) ||
+                                                        at.t0 + kTileKeys <= see_below;
+                const bool masked = !__all_sync(~0u, sees_all);
+                float x[2][32], tile_top = -INFINITY;
+                load32(s_tmem, x[0]);
                 wait_loads();
-                if (MODS) {
-                    const int offset = (at.shared ? 0 : p.shared_len) + at.t0 - position;
+                if (!MODS && !masked) {
 #pragma unroll
-                    for (int c = 0; c < 4; ++c)
-#pragma unroll
-                        for (int e = 0; e < 32; ++e) {
-                            float y;  // the score times log2(e)
-                            if (p.softcap > 0.f) {
-                                // tanh(z) = 1 - 2 / (e^2z + 1), to 2^-22 of the cap, where the exponent's error counts
-                                y = cap_out - 2.f * cap_out * reciprocal_fast(exp2_fast(x[c][e] * cap_in) + 1.f);
-                            } else {
-                                y = x[c][e] * scale_log2;
-                            }
-                            x[c][e] = y + slope * (float)(offset + c * 32 + e);
-                        }
-                }
-                const float unit = MODS ? 1.f : scale_log2;
-                const bool sees_all = !valid ? true : at.shared ? at.t0 + kTileKeys <= p.shared_len
-                                                : (at.t0 >= see_lo && at.t0 + kTileKeys <= see_hi) ||
-                                                      at.t0 + kTileKeys <= see_below;
-                if (!__all_sync(~0u, sees_all)) {
+                    for (int c = 0; c < 4; ++c) {
+                        load32(s_tmem + ((c + 1) & 3) * 32, x[(c + 1) & 1]);  // the last one: chunk 0 again
+                        tile_top = max_of(tile_top, x[c & 1]);
+                        wait_loads();
+                    }
+                } else {
                     const int from = (at.shared ? 0 : see_lo) - at.t0;
                     const int to = (at.shared ? p.shared_len : see_hi) - at.t0;
                     const int below = (at.shared ? 0 : see_below) - at.t0;
+                    const float offset = MODS ? (float)((at.shared ? 0 : p.shared_len) + at.t0 - position) : 0.f;
 #pragma unroll
-                    for (int c = 0; c < 4; ++c)
+                    for (int c = 0; c < 4; ++c) {
+                        float(&y)[32] = x[c & 1];
 #pragma unroll
                         for (int e = 0; e < 32; ++e) {
                             const int k = c * 32 + e;
-                            if (!((k >= from && k < to) || k < below)) x[c][e] = -INFINITY;
+                            if (MODS) {  // the score times log2(e)
+                                // tanh(z) = 1 - 2 / (e^2z + 1), to 2^-22 of the cap, where the exponent's error counts
+                                y[e] = p.softcap > 0.f
+                                           ? cap_out - 2.f * cap_out * reciprocal_fast(exp2_fast(y[e] * cap_in) + 1.f)
+                                           : y[e] * scale_log2;
+                                y[e] += slope * (offset + (float)k);
+                            }
+                            if (masked && !((k >= from && k < to) || k < below)) y[e] = -INFINITY;
                         }
+                        tile_top = max_of(tile_top, y);
+                        store32(s_tmem + c * 32, y);
+                        if (c < 3) {
+                            load32(s_tmem + (c + 1) * 32, x[(c + 1) & 1]);
+                            wait_loads();
+                        }
+                    }
+                    wait_stores();
+                    load32(s_tmem, x[0]);
+                    wait_loads();
                 }
-                float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-                for (int c = 0; c < 4; ++c)
-#pragma unroll
-                    for (int e = 0; e < 32; ++e) top[e & 3] = fmaxf(top[e & 3], x[c][e]);
-                const float tile_top = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * unit;
-                // tile_top is NaN only for -inf * 0; a scale of 0 leaves every score 0.
+                const float unit = MODS ? 1.f : scale_log2;
+                tile_top *= unit;
                 const bool grow = m == -INFINITY ? tile_top > -INFINITY : tile_top > m + kLazy;
                 if (__any_sync(~0u, grow)) {
                     const float now = grow ? tile_top : m, factor = grow ? weight_of(m, now) : 1.f;
                     m = now;
-#pragma unroll
-                    for (int k = 0; k < 4; ++k) sum[k] *= factor;
+                    sum.x *= factor, sum.y *= factor;
                     if (i > 0) {  // the output so far, once the product before this tile has landed
                         if (!warp_waits(smem_u32(&outputs[g]), (i - 1) & 1, &gave_up)) {
                             ok = false;
@@ -444,17 +491,24 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tiles(const __grid_cons
                         }
                     }
                 }
-                const float reference = m == -INFINITY ? 0.f : m;
+                // Second pass: the weights, over the scores already read (16 columns for 32 scores).
+                const float2 units = make_float2(unit, unit);
+                const float below_zero = m == -INFINITY ? 0.f : -m;
+                const float2 references = make_float2(below_zero, below_zero);
 #pragma unroll
                 for (int c = 0; c < 4; ++c) {
+                    if (c < 3) load32(s_tmem + (c + 1) * 32, x[(c + 1) & 1]);
+                    const float(&y)[32] = x[c & 1];
                     uint32_t packed[16];
 #pragma unroll
                     for (int e = 0; e < 32; e += 2) {
-                        const float a = exp2_fast(x[c][e] * unit - reference);
-                        const float b = exp2_fast(x[c][e + 1] * unit - reference);
-                        sum[(e >> 1) & 3] += a + b;
-                        packed[e >> 1] = Pack2<T>::of(a, b);
+                        float2 w = fma2(make_float2(y[e], y[e + 1]), units, references);
+                        w.x = exp2_fast(w.x);
+                        w.y = exp2_fast(w.y);
+                        sum = add2(sum, w);
+                        packed[e >> 1] = Pack2<T>::of(w.x, w.y);
                     }
+                    if (c < 3) wait_loads();
                     store16(s_tmem + c * 16, packed);
                 }
                 wait_stores();
@@ -486,7 +540,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tiles(const __grid_cons
                 fence_after();
             }
             if (ok) {
-                const float total = sum[0] + sum[1] + sum[2] + sum[3];
+                const float total = sum.x + sum.y;
                 const int out_token = item.q.q0 + token;
                 const bool partial = t.prefix_only || t.splits > 1;
                 const int64_t at = ((int64_t)item.split * p.num_tokens + out_token) * p.q_heads + head;
