@@ -29,8 +29,8 @@ constexpr int kIssueWarp = 8;
 constexpr int kLoadWarp = 9;
 constexpr int kThreads = 384;
 // The launch gives each thread 168 registers; a row's 128 scores want more, the other warps less:
-// 256 x 208 + 128 x 80 = 63488, within the launch's 384 x 168 = 64512.
-constexpr int kSoftmaxRegisters = 208, kOtherRegisters = 80;
+// 256 x 224 + 128 x 56 = 64512, the launch's 384 x 168.
+constexpr int kSoftmaxRegisters = 224, kOtherRegisters = 56;
 constexpr float kLazy = 8.f;
 constexpr uint64_t kWaitNs = 2000000000ull;  // a wait that has not ended after 2 s is an error
 
@@ -95,6 +95,12 @@ __device__ __forceinline__ void mma_tensor(uint32_t d, uint32_t a, uint64_t b, u
         "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
         "r"(a), "l"(b), "r"(inst), "r"((uint32_t)accumulate)
         : "memory");
+}
+
+__device__ __forceinline__ bool elect_one() {
+    uint32_t one;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(one));
+    return one != 0;
 }
 
 // Arrives on `bar` once every product issued so far has completed.
@@ -307,7 +313,7 @@ template <class T, int D, bool MODS>
 __global__ void __launch_bounds__(kThreads, 1) attention_tiles(const __grid_constant__ TileParams t) {
     using S = Shape<D>;
     extern __shared__ unsigned char raw[];
-    __shared__ __align__(8) uint64_t full[S::kSlots], empty[S::kSlots], queries_in[2], scores[2], weights[2], outputs[2],
+    __shared__ __align__(8) uint64_t full[S::kSlots], empty[S::kSlots], queries_in[2], scores[2], weights[2][2], outputs[2],
         drain;
     __shared__ uint32_t tmem_base;
     __shared__ int gave_up;
@@ -324,7 +330,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tiles(const __grid_cons
             asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(smem_u32(bar)), "r"(count) : "memory");
         };
         for (int i = 0; i < S::kSlots; ++i) init(&full[i], 1), init(&empty[i], 1);
-        for (int i = 0; i < 2; ++i) init(&queries_in[i], 128), init(&scores[i], 1), init(&weights[i], 128), init(&outputs[i], 1);
+        for (int i = 0; i < 2; ++i) init(&queries_in[i], 128), init(&scores[i], 1), init(&weights[i][0], 128), init(&weights[i][1], 128), init(&outputs[i], 1);
         init(&drain, 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
@@ -348,6 +354,8 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tiles(const __grid_cons
     }
     __syncthreads();
     fence_after();
+    // All 512 columns there are, so the allocation starts at column 0; the issuing warp counts on it (constants stay out
+    // of its way to the tensor cores), which the softmax's addresses make good for the rest.
     const uint32_t tmem = tmem_base;
     const Item &item = shared_item;
     const int n_tiles = item.tiles;
@@ -420,30 +428,22 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tiles(const __grid_cons
                     break;
                 }
                 fence_after();
-                // First pass: the tile's maximum. Scores that a mask, cap or bias changes go back to TMEM as they are then.
+                // Scores that a mask, cap or bias changes go back to TMEM as they are then.
                 const bool sees_all = !valid ? true
                                       : at.shared ? at.t0 + kTileKeys <= p.shared_len
                                                   : (at.t0 >= see_lo && at.t0 + kTileKeys <= see_hi) ||
                                                         at.t0 + kTileKeys <= see_below;
                 const bool masked = !__all_sync(~0u, sees_all);
-                float x[2][32], tile_top = -INFINITY;
-                load32(s_tmem, x[0]);
-                wait_loads();
-                if (!MODS && !masked) {
-#pragma unroll
-                    for (int c = 0; c < 4; ++c) {
-                        load32(s_tmem + ((c + 1) & 3) * 32, x[(c + 1) & 1]);  // the last one: chunk 0 again
-                        tile_top = max_of(tile_top, x[c & 1]);
-                        wait_loads();
-                    }
-                } else {
+                if (MODS || masked) {
                     const int from = (at.shared ? 0 : see_lo) - at.t0;
                     const int to = (at.shared ? p.shared_len : see_hi) - at.t0;
                     const int below = (at.shared ? 0 : see_below) - at.t0;
                     const float offset = MODS ? (float)((at.shared ? 0 : p.shared_len) + at.t0 - position) : 0.f;
 #pragma unroll
                     for (int c = 0; c < 4; ++c) {
-                        float(&y)[32] = x[c & 1];
+                        float y[32];
+                        load32(s_tmem + c * 32, y);
+                        wait_loads();
 #pragma unroll
                         for (int e = 0; e < 32; ++e) {
                             const int k = c * 32 + e;
@@ -456,17 +456,17 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tiles(const __grid_cons
                             }
                             if (masked && !((k >= from && k < to) || k < below)) y[e] = -INFINITY;
                         }
-                        tile_top = max_of(tile_top, y);
                         store32(s_tmem + c * 32, y);
-                        if (c < 3) {
-                            load32(s_tmem + (c + 1) * 32, x[(c + 1) & 1]);
-                            wait_loads();
-                        }
                     }
                     wait_stores();
-                    load32(s_tmem, x[0]);
-                    wait_loads();
                 }
+                float x[4][32];
+#pragma unroll
+                for (int c = 0; c < 4; ++c) load32(s_tmem + c * 32, x[c]);
+                wait_loads();
+                float tile_top = -INFINITY;
+#pragma unroll
+                for (int c = 0; c < 4; ++c) tile_top = max_of(tile_top, x[c]);
                 const float unit = MODS ? 1.f : scale_log2;
                 tile_top *= unit;
                 const bool grow = m == -INFINITY ? tile_top > -INFINITY : tile_top > m + kLazy;
@@ -474,12 +474,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tiles(const __grid_cons
                     const float now = grow ? tile_top : m, factor = grow ? weight_of(m, now) : 1.f;
                     m = now;
                     sum.x *= factor, sum.y *= factor;
-                    if (i > 0) {  // the output so far, once the product before this tile has landed
-                        if (!warp_waits(smem_u32(&outputs[g]), (i - 1) & 1, &gave_up)) {
-                            ok = false;
-                            break;
-                        }
-                        fence_after();
+                    if (i > 0) {  // the output so far: the products behind it landed before this tile's scores did
 #pragma unroll
                         for (int c = 0; c < D / 16; ++c) {
                             uint32_t o[16];
@@ -491,27 +486,6 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tiles(const __grid_cons
                         }
                     }
                 }
-                // Second pass: the weights, over the scores already read (16 columns for 32 scores).
-                const float2 units = make_float2(unit, unit);
-                const float below_zero = m == -INFINITY ? 0.f : -m;
-                const float2 references = make_float2(below_zero, below_zero);
-#pragma unroll
-                for (int c = 0; c < 4; ++c) {
-                    if (c < 3) load32(s_tmem + (c + 1) * 32, x[(c + 1) & 1]);
-                    const float(&y)[32] = x[c & 1];
-                    uint32_t packed[16];
-#pragma unroll
-                    for (int e = 0; e < 32; e += 2) {
-                        float2 w = fma2(make_float2(y[e], y[e + 1]), units, references);
-                        w.x = exp2_fast(w.x);
-                        w.y = exp2_fast(w.y);
-                        sum = add2(sum, w);
-                        packed[e >> 1] = Pack2<T>::of(w.x, w.y);
-                    }
-                    if (c < 3) wait_loads();
-                    store16(s_tmem + c * 16, packed);
-                }
-                wait_stores();
                 // Values that no row sees (past the length, ahead of the window) may hold anything: 0 times NaN is NaN.
                 if (at.t0 < at.lo || at.t0 + kTileKeys > at.hi) {
                     const int slot = (2 * i + 1) % S::kSlots;
@@ -531,12 +505,33 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tiles(const __grid_cons
                     }
                     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 }
-                fence_before();
-                arrive(smem_u32(&weights[g]));
+                // The weights, over the scores already read (16 columns for 32 scores), given to the second product in
+                // two halves, so that it starts while the second is computed.
+                const float2 units = make_float2(unit, unit);
+                const float below_zero = m == -INFINITY ? 0.f : -m;
+                const float2 references = make_float2(below_zero, below_zero);
+#pragma unroll
+                for (int c = 0; c < 4; ++c) {
+                    uint32_t packed[16];
+#pragma unroll
+                    for (int e = 0; e < 32; e += 2) {
+                        float2 w = fma2(make_float2(x[c][e], x[c][e + 1]), units, references);
+                        w.x = exp2_fast(w.x);
+                        w.y = exp2_fast(w.y);
+                        sum = add2(sum, w);
+                        packed[e >> 1] = Pack2<T>::of(w.x, w.y);
+                    }
+                    store16(s_tmem + c * 16, packed);
+                    if (c & 1) {
+                        wait_stores();
+                        fence_before();
+                        arrive(smem_u32(&weights[g][c >> 1]));
+                    }
+                }
             }
             // ---- the row's output
             if (ok && n_tiles > 0) {
-                ok = warp_waits(smem_u32(&outputs[g]), (n_tiles - 1) & 1, &gave_up);
+                ok = warp_waits(smem_u32(&outputs[g]), 0, &gave_up);
                 fence_after();
             }
             if (ok) {
@@ -580,55 +575,78 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tiles(const __grid_cons
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegisters));
     }
     if (warp == kIssueWarp) {
-        if (lane == 0) {
-            constexpr uint32_t score_inst = instruction<T>(kTileKeys, false), output_inst = instruction<T>(D, true);
-            bool ok = true;
-            auto wait = [&](uint64_t *bar, uint32_t parity) {
-                if (ok) ok = wait_phase(smem_u32(bar), parity, &gave_up);
-                return ok;
-            };
-            auto score = [&](int g, int slot) {
-                const uint32_t q = base + g * S::kTileBytes, k = ring + slot * S::kTileBytes;
+        // The whole warp walks the loop, one elected lane issues: operands then stay in uniform registers. Issued from
+        // a divergent branch, a tile's 16 products took 700 cycles longer.
+        constexpr uint32_t score_inst = instruction<T>(kTileKeys, false), output_inst = instruction<T>(D, true);
+        bool ok = true;
+        auto wait = [&](uint64_t *bar, uint32_t parity) {
+            if (ok) ok = warp_waits(smem_u32(bar), parity, &gave_up);
+            return ok;
+        };
+        const uint64_t q_operand = operand(base, 16), k_operand = operand(ring, 16),
+                       v_operand = operand(ring, S::kHalfBytes);
+        auto score = [&](int g, int slot) {
+            const uint64_t q = q_operand + (uint32_t)(g * (S::kTileBytes >> 4));
+            const uint64_t k = k_operand + (uint32_t)(slot * (S::kTileBytes >> 4));
+            if (elect_one()) {
 #pragma unroll
                 for (int c = 0; c < D / 16; ++c) {
-                    const uint32_t step = (c >> 2) * S::kHalfBytes + (c & 3) * 32;
-                    mma_shared(tmem + g * 128, operand(q + step, 16), operand(k + step, 16), score_inst, c > 0);
+                    constexpr int kHalf = S::kHalfBytes >> 4;
+                    const uint32_t step = (c >> 2) * kHalf + (c & 3) * 2;
+                    mma_shared(g * 128, q + step, k + step, score_inst, c > 0);
                 }
                 commit(smem_u32(&scores[g]));
-            };
-            auto output = [&](int g, int slot, bool accumulate) {
-                const uint32_t v = ring + slot * S::kTileBytes;
+            }
+            __syncwarp();
+        };
+        auto output = [&](int g, int slot, int half, bool accumulate) {
+            const uint64_t v = v_operand + (uint32_t)(slot * (S::kTileBytes >> 4) + half * (64 * 128 >> 4));
+            if (elect_one()) {
 #pragma unroll
-                for (int c = 0; c < kTileKeys / 16; ++c)
-                    mma_tensor(tmem + S::kOutColumn + g * D, tmem + g * 128 + c * 8,
-                               operand(v + c * 16 * 128, S::kHalfBytes), output_inst, accumulate || c > 0);
-                commit(smem_u32(&outputs[g]));
-            };
-            auto slot_of = [](int n) { return n % S::kSlots; };
-            auto phase_of = [](int n) { return (uint32_t)(n / S::kSlots) & 1; };
-            // Ring order: K 0, V 0, K 1, V 1, ...
-            if (n_tiles > 0 && wait(&full[0], 0)) {
-                for (int g = 0; g < active; ++g)
-                    if (wait(&queries_in[g], 0)) {
-                        fence_after();
-                        score(g, 0);
-                    }
-                commit(smem_u32(&empty[0]));
+                for (int c = 0; c < kTileKeys / 32; ++c)
+                    mma_tensor(S::kOutColumn + g * D, g * 128 + half * 32 + c * 8, v + (uint32_t)(c * (16 * 128 >> 4)),
+                               output_inst, accumulate || c > 0);
             }
-            for (int i = 0; ok && i < n_tiles; ++i) {
-                const int v = 2 * i + 1, k = 2 * i + 2;
-                if (!wait(&full[slot_of(v)], phase_of(v))) break;
-                if (i + 1 < n_tiles && !wait(&full[slot_of(k)], phase_of(k))) break;
-                for (int g = 0; g < active; ++g) {
-                    if (!wait(&weights[g], i & 1)) break;
+            __syncwarp();
+        };
+        auto finished = [&](uint64_t *bar) {
+            if (elect_one()) commit(smem_u32(bar));
+            __syncwarp();
+        };
+        // Ring order: K 0, V 0, K 1, V 1, ...
+        if (n_tiles > 0 && wait(&full[0], 0)) {
+            for (int g = 0; g < active; ++g)
+                if (wait(&queries_in[g], 0)) {
                     fence_after();
-                    output(g, slot_of(v), i > 0);
-                    if (g + 1 == active) commit(smem_u32(&empty[slot_of(v)]));
-                    // The scores land where the weights were: the products execute in the order they are issued.
-                    if (i + 1 < n_tiles) score(g, slot_of(k));
+                    score(g, 0);
                 }
-                if (ok && i + 1 < n_tiles) commit(smem_u32(&empty[slot_of(k)]));
+            finished(&empty[0]);
+        }
+        int v_slot = 1 % S::kSlots, k_slot = 2 % S::kSlots;
+        uint32_t v_phase = 0, k_phase = 0;
+        for (int i = 0; ok && i < n_tiles; ++i) {
+            const bool more = i + 1 < n_tiles;
+            if (!wait(&full[v_slot], v_phase)) break;
+            if (more && !wait(&full[k_slot], k_phase)) break;
+            for (int g = 0; g < active; ++g) {
+                if (!wait(&weights[g][0], i & 1)) break;
+                fence_after();
+                output(g, v_slot, 0, i > 0);
+                if (!wait(&weights[g][1], i & 1)) break;
+                fence_after();
+                output(g, v_slot, 1, true);
+                // The scores land where the weights were: the products execute in the order they are issued.
+                if (more) score(g, k_slot);
+                else finished(&outputs[g]);
             }
+            if (ok) {
+                finished(&empty[v_slot]);
+                if (more) finished(&empty[k_slot]);
+            }
+            if ((v_slot += 2) >= S::kSlots) v_slot -= S::kSlots, v_phase ^= 1;
+            if ((k_slot += 2) >= S::kSlots) k_slot -= S::kSlots, k_phase ^= 1;
+        }
+        if (lane == 0) {
             if (!ok) {  // a wait ran out: let what was issued end before TMEM is freed
                 commit(smem_u32(&drain));
                 const uint64_t deadline = globaltimer() + kWaitNs;
