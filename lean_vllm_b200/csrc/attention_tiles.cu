@@ -244,20 +244,19 @@ __device__ bool find_item(const TileParams &t, int id, Item &item) {
         item.shared_tiles = (p.shared_len + kTileKeys - 1) / kTileKeys;
         item.tiles = item.shared_tiles;
     } else {
-        auto tiles_of = [&](int s) {
-            if (s >= p.batch) return 0;
-            const int64_t rows = (int64_t)sequence_of(p, s).q_len * p.group;
+        auto tiles_of = [&](const Sequence &q) {
+            const int64_t rows = (int64_t)q.q_len * p.group;
             return rows > p.rows_limit ? (int)((rows + kTileRows - 1) / kTileRows) : 0;
         };
-        int total = 0;
-        for (int s = lane; s < p.batch; s += 32) total += tiles_of(s);
-#pragma unroll
-        for (int o = 16; o; o >>= 1) total += __shfl_xor_sync(~0u, total, o);
+        auto at = [&](int s) { return s < p.batch ? sequence_of(p, s) : Sequence{0, 0, 0, 0}; };
+        Sequence mine = at(lane);  // of the 32 sequences looked at now: all there are, often
+        int n = tiles_of(mine), total = n;
+        for (int s = lane + 32; s < p.batch; s += 32) total += tiles_of(at(s));
+        total = __reduce_add_sync(~0u, total);
         const int wanted = total - 1 - r;
         if (wanted < 0) return false;
         int before = 0;
-        for (int s0 = 0;; s0 += 32) {
-            const int n = tiles_of(s0 + lane);
+        for (int s0 = 0;;) {
             int sum = n;
 #pragma unroll
             for (int o = 1; o < 32; o <<= 1) {
@@ -269,11 +268,15 @@ __device__ bool find_item(const TileParams &t, int id, Item &item) {
                 const int who = __ffs(here) - 1;
                 item.sequence = s0 + who;
                 item.row0 = (wanted - before - __shfl_sync(~0u, sum - n, who)) * kTileRows;
+                item.q = Sequence{__shfl_sync(~0u, mine.q0, who), __shfl_sync(~0u, mine.q_len, who),
+                                  __shfl_sync(~0u, mine.kv_len, who), __shfl_sync(~0u, mine.prefix, who)};
                 break;
             }
             before += __shfl_sync(~0u, sum, 31);
+            s0 += 32;
+            mine = at(s0 + lane);
+            n = tiles_of(mine);
         }
-        item.q = sequence_of(p, item.sequence);
         if (lane == 0 && (int64_t)p.kv_lens[item.sequence] > (int64_t)p.max_blocks * p.block_size)
             flag_error(p.error_word, p.status, kErrPastCache);
         item.rows = (int)min((int64_t)kTileRows, (int64_t)item.q.q_len * p.group - item.row0);
@@ -334,6 +337,12 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tiles(const __grid_cons
         init(&drain, 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
+    if (warp == kIssueWarp) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(&tmem_base))
+                     : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+        fence_before();
+    }
     wait_prerequisites();
     launch_dependents();  // after the wait: what starts now may read all that came before this kernel
     if (warp == 0) {
@@ -345,21 +354,13 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tiles(const __grid_cons
         }
     }
     __syncthreads();
-    if (!has_item) return;
-    if (warp == kIssueWarp) {
-        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(&tmem_base))
-                     : "memory");
-        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
-        fence_before();
-    }
-    __syncthreads();
     fence_after();
     // All 512 columns there are, so the allocation starts at column 0; the issuing warp counts on it (constants stay out
     // of its way to the tensor cores), which the softmax's addresses make good for the rest.
     const uint32_t tmem = tmem_base;
     const Item &item = shared_item;
-    const int n_tiles = item.tiles;
-    const int active = item.rows > 128 ? 2 : 1;  // tiles of 128 rows in use
+    const int n_tiles = has_item ? item.tiles : 0;
+    const int active = !has_item ? 0 : item.rows > 128 ? 2 : 1;  // tiles of 128 rows in use
 
     if (warp < kSoftmaxWarps) {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegisters));
@@ -374,13 +375,15 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tiles(const __grid_cons
             {
                 const uint4 *from = reinterpret_cast<const uint4 *>(
                     p.query + (int64_t)(item.q.q0 + token) * p.q_token_stride + (int64_t)head * p.q_head_stride);
+                uint4 v[D / 8];  // all in flight at once
+#pragma unroll
+                for (int c = 0; c < D / 8; ++c) v[c] = valid ? from[c] : make_uint4(0, 0, 0, 0);
                 const uint32_t to = base + g * S::kTileBytes + row * 128;
 #pragma unroll
                 for (int c = 0; c < D / 8; ++c) {
-                    const uint4 v = valid ? from[c] : make_uint4(0, 0, 0, 0);
                     const uint32_t at = to + (c >> 3) * S::kHalfBytes + (((c & 7) ^ (row & 7)) << 4);
-                    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(v.x), "r"(v.y), "r"(v.z),
-                                 "r"(v.w)
+                    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(v[c].x), "r"(v[c].y),
+                                 "r"(v[c].z), "r"(v[c].w)
                                  : "memory");
                 }
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
