@@ -34,7 +34,6 @@ constexpr int kRowThreads = kRowWarps * 32;
 constexpr int kRowStages = 3;
 constexpr int kWarpTokens = 16;
 constexpr int kTileTokens = kRowWarps * kWarpTokens;
-constexpr int kMaxRowCtas = 1024;  // slots of the workspace: two per CTA
 
 template <int D>
 constexpr int row_smem() {
@@ -420,7 +419,7 @@ constexpr size_t kRowPartials = (size_t)kMaxRowCtas * 2 * kRowTile;
 constexpr size_t kMlBytes = sizeof(float2), kOutBytes = 128 * sizeof(float);
 constexpr size_t kSplitAt = KVX_ATTENTION_ZEROED + kRowPartials * (kMlBytes + kOutBytes);
 constexpr size_t kWorkspaceBytes = kSplitAt + kSplitRows * (kMlBytes + kOutBytes);
-static_assert(kMaxRowCtas * sizeof(int32_t) <= KVX_ATTENTION_ZEROED, "a counter per CTA");
+static_assert(kMaxRowCtas <= kTileCounter && (kTileCounter + 1) * sizeof(int32_t) <= KVX_ATTENTION_ZEROED, "counters");
 
 template <class T, int D>
 int launch_rows(const AttnParams &p, bool mods, int sms, cudaStream_t stream) {
@@ -550,7 +549,7 @@ int kvx_attention(const kvx_attention_args *args, int flags, void *stream) {
     if (a.shared_len > 0 && q_rows <= kTileKeys && (int64_t)a.num_tokens * a.q_heads <= kSplitRows) {
         // A prefix shared by short sequences: all their rows together against it, then each against its own keys.
         const int splits = splits_for((all_rows + kTileRows - 1) / kTileRows, a.shared_len);
-        if (int rc = launch_tiles(p, a.head_dim, a.dtype, mods, true, splits, s)) return rc;
+        if (int rc = launch_tiles(p, a.head_dim, a.dtype, mods, true, splits, device.sms, s)) return rc;
         p.prefix_splits = splits;
         p.shared_len = 0;
         return rows_kernel();
@@ -560,8 +559,8 @@ int kvx_attention(const kvx_attention_args *args, int flags, void *stream) {
     const bool mixed = a.batch > 1 && a.num_tokens < (int64_t)a.batch * a.max_q_len;
     p.rows_limit = mixed ? kRowTile : 0;
     const int64_t row_tiles = std::max<int64_t>(1, all_rows / kTileRows);
-    if (int rc = launch_tiles(p, a.head_dim, a.dtype, mods, false, splits_for(row_tiles, (int64_t)a.max_kv_len + a.shared_len), s))
-        return rc;
+    const int splits = splits_for(row_tiles, (int64_t)a.max_kv_len + a.shared_len);
+    if (int rc = launch_tiles(p, a.head_dim, a.dtype, mods, false, splits, device.sms, s)) return rc;
     return mixed ? rows_kernel() : KVX_OK;
 }
 

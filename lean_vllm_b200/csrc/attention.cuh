@@ -41,10 +41,13 @@ struct AttnParams {
 // attention_tiles (attention_tiles.cu). `prefix_only`: all query rows against the shared prefix alone, as partial
 // results of `splits`; else each sequence's rows above rows_limit, joined when splits is above 1.
 int launch_tiles(const AttnParams &p, int head_dim, int dtype, bool mods, bool prefix_only, int splits,
-                 cudaStream_t stream);
-// Whether attention_tiles can read this cache, and the tokens a copy of it brings at once.
+                 int sms, cudaStream_t stream);
+// The tokens of this cache that one of attention_tiles' copies brings; 0 if it cannot take the call (blocks that are no
+// multiple of 8 tokens, strides that no tensor map holds, groups beyond a tile's rows).
 int tile_box(const AttnParams &p);
 
+constexpr int kMaxRowCtas = 1024;       // of attention_rows: a counter and two slots of partial results each
+constexpr int kTileCounter = 8192;      // attention_tiles' counter, on a line of its own
 constexpr int kTileRows = 256;
 constexpr int kTileKeys = 128;
 constexpr int64_t kSplitRows = 131072;  // rows of partial results the workspace holds

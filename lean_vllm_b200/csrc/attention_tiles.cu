@@ -3,12 +3,16 @@
 // rows that the products bound the time, not the cache.
 //
 // Work. The query rows of a KV head (its group of heads x the sequence's query tokens, or the whole batch's for a shared
-// prefix) share its keys. A CTA takes 256 of them, as two tiles of 128, and walks its keys in tiles of 128. For each
+// prefix) share its keys. A CTA takes two tiles of whole tokens, up to 128 rows each, so that one TMA copy brings a
+// tile's 64 columns whatever the group (7 heads: 18 tokens, 126 rows), and walks its keys in tiles of 128. For each
 // pair of tiles, S = Q K^T and O += P V are one chain of tcgen05.mma each, 128 x 128 x D and 128 x D x 128, with Q, K and
 // V in shared memory and S, P and O in TMEM (S, then P in its place, 128 columns a tile; O, D columns a tile).
 //
-// Roles. One warp copies K and V tiles by TMA into a ring; one thread issues the products; two groups of 4 warps run the
-// softmax of a tile each, one row per thread. While one tile's scores are in the softmax the other's products run.
+// Roles. One warp copies K and V tiles by TMA into a ring, one copies the queries, one issues the products, one looks up
+// what to do next; two groups of 4 warps run the softmax of a tile each, one row per thread. While one tile's scores are
+// in the softmax the other's products run, and a CTA takes item after item: the next one's keys and queries arrive and
+// its first scores are computed while the last one's output is written. One item per CTA cost 10,000 cycles between two
+// items (lookup, queries, first keys, output), a quarter of a prompt of 8192 tokens.
 //
 // The running maximum moves only when a tile's exceeds it by more than 2^8 (kLazy): the weights then stay below 2^8, which
 // costs no precision in a floating type, and the accumulated output is rescaled a few times per row, not per tile.
@@ -27,6 +31,9 @@ using namespace kvx;
 constexpr int kSoftmaxWarps = 8;
 constexpr int kIssueWarp = 8;
 constexpr int kLoadWarp = 9;
+constexpr int kQueryWarp = 10;
+constexpr int kPlanWarp = 11;
+constexpr int kItemReaders = kSoftmaxWarps + 3;  // warps that read an item
 constexpr int kThreads = 384;
 // The launch gives each thread 168 registers; a row's 128 scores want more, the other warps less:
 // 256 x 224 + 128 x 56 = 64512, the launch's 384 x 168.
@@ -39,23 +46,27 @@ struct Shape {
     static constexpr int kHalves = D / 64;                      // 128-byte columns of a row
     static constexpr int kTileBytes = kTileKeys * D * 2;        // of 128 rows: queries, keys or values
     static constexpr int kHalfBytes = kTileKeys * 128;
-    static constexpr int kSlots = D == 128 ? 5 : 10;            // ring of K and V tiles: 160 KB
-    static constexpr int kBytes = (2 + kSlots) * kTileBytes + 1024;
+    static constexpr int kSlots = D == 128 ? 4 : 8;             // ring of K and V tiles: 128 KB
+    static constexpr int kStageBytes = 32 * 128;                // of a softmax warp: its rows' output on its way out
+    static constexpr int kBytes = (2 + kSlots) * kTileBytes + kSoftmaxWarps * kStageBytes + 1024;
     static constexpr int kOutColumn = 256;                      // TMEM: S and P of both tiles, then O of both
 };
 
 struct TileParams {
     AttnParams a;
-    CUtensorMap keys, values;
+    CUtensorMap keys, values, queries;
+    int32_t tile_tokens;  // query tokens of a tile of up to 128 rows
     int32_t box;          // tokens per copy
     int32_t splits;
     int32_t prefix_only;
-    int32_t row_tiles;    // bound on the launch's tiles of 256 rows
+    int32_t row_tiles;    // bound on the launch's items per KV head and split
+    int32_t *next;        // items given out beyond each CTA's first; 0 between launches
 };
 
 struct Item {
     Sequence q;
-    int32_t sequence, head, row0, rows, split;
+    int32_t valid;               // 0: no more work
+    int32_t sequence, head, token0, tokens, split;  // tokens: of the sequence's (or the batch's) from token0 on
     int32_t lo, hi;              // own keys that any row sees
     int32_t shared_tiles, tiles; // tiles of the shared prefix walked first, and all of this split's ...
     int32_t first_tile;          // ... from this one of the item's on
@@ -226,9 +237,9 @@ __device__ __forceinline__ bool warp_waits(uint32_t bar, uint32_t parity, volati
     return __all_sync(~0u, wait_phase(bar, parity, gave_up));
 }
 
-// The CTA's item: which rows of which sequence, and which keys. Row tiles come last first, since the last ones of a
-// causal prompt see the most keys. Every thread of warp 0 calls this; false: no work.
-__device__ bool find_item(const TileParams &t, int id, Item &item) {
+// Item `id`: which rows of which sequence, and which keys. Row tiles come last first, since the last ones of a causal
+// prompt see the most keys. A whole warp calls this; false: there are no more. `count`: how many there are.
+__device__ bool find_item(const TileParams &t, int id, Item &item, int &count) {
     const AttnParams &p = t.a;
     const int lane = threadIdx.x & 31;
     const int per_tile = p.kv_heads * t.splits;
@@ -236,23 +247,25 @@ __device__ bool find_item(const TileParams &t, int id, Item &item) {
     item.split = (id - r * per_tile) / p.kv_heads;
     item.head = id - r * per_tile - item.split * p.kv_heads;
     if (t.prefix_only) {
+        count = t.row_tiles * per_tile;
+        if (id >= count) return false;
         item.sequence = 0;
         item.q = Sequence{0, p.num_tokens, p.shared_len, 0};
-        item.row0 = r * kTileRows;
-        item.rows = min(kTileRows, p.num_tokens * p.group - item.row0);
+        item.token0 = r * 2 * t.tile_tokens;
+        item.tokens = min(2 * t.tile_tokens, p.num_tokens - item.token0);
         item.lo = item.hi = item.lo_tile = 0;
         item.shared_tiles = (p.shared_len + kTileKeys - 1) / kTileKeys;
         item.tiles = item.shared_tiles;
     } else {
         auto tiles_of = [&](const Sequence &q) {
-            const int64_t rows = (int64_t)q.q_len * p.group;
-            return rows > p.rows_limit ? (int)((rows + kTileRows - 1) / kTileRows) : 0;
+            return (int64_t)q.q_len * p.group > p.rows_limit ? (q.q_len + 2 * t.tile_tokens - 1) / (2 * t.tile_tokens) : 0;
         };
         auto at = [&](int s) { return s < p.batch ? sequence_of(p, s) : Sequence{0, 0, 0, 0}; };
         Sequence mine = at(lane);  // of the 32 sequences looked at now: all there are, often
         int n = tiles_of(mine), total = n;
         for (int s = lane + 32; s < p.batch; s += 32) total += tiles_of(at(s));
         total = __reduce_add_sync(~0u, total);
+        count = total * per_tile;
         const int wanted = total - 1 - r;
         if (wanted < 0) return false;
         int before = 0;
@@ -267,7 +280,7 @@ __device__ bool find_item(const TileParams &t, int id, Item &item) {
             if (here) {
                 const int who = __ffs(here) - 1;
                 item.sequence = s0 + who;
-                item.row0 = (wanted - before - __shfl_sync(~0u, sum - n, who)) * kTileRows;
+                item.token0 = (wanted - before - __shfl_sync(~0u, sum - n, who)) * 2 * t.tile_tokens;
                 item.q = Sequence{__shfl_sync(~0u, mine.q0, who), __shfl_sync(~0u, mine.q_len, who),
                                   __shfl_sync(~0u, mine.kv_len, who), __shfl_sync(~0u, mine.prefix, who)};
                 break;
@@ -279,11 +292,10 @@ __device__ bool find_item(const TileParams &t, int id, Item &item) {
         }
         if (lane == 0 && (int64_t)p.kv_lens[item.sequence] > (int64_t)p.max_blocks * p.block_size)
             flag_error(p.error_word, p.status, kErrPastCache);
-        item.rows = (int)min((int64_t)kTileRows, (int64_t)item.q.q_len * p.group - item.row0);
+        item.tokens = min(2 * t.tile_tokens, item.q.q_len - item.token0);
         // Own keys, counted without the shared prefix, whose rows all see it.
         const int own = item.q.kv_len - p.shared_len;
-        const int first = own - item.q.q_len + item.row0 / p.group;
-        const int last = own - item.q.q_len + (item.row0 + item.rows - 1) / p.group;
+        const int first = own - item.q.q_len + item.token0, last = first + item.tokens - 1;
         const int prefix = item.q.prefix - p.shared_len;  // beyond a shared prefix there is none
         item.lo = p.window > 0 && prefix <= 0 ? max(0, first - p.window + 1) : 0;
         item.hi = max(max(0, min(own, last + 1)), prefix);
@@ -291,8 +303,13 @@ __device__ bool find_item(const TileParams &t, int id, Item &item) {
         item.shared_tiles = (p.shared_len + kTileKeys - 1) / kTileKeys;
         item.tiles = item.shared_tiles + max(0, (item.hi + kTileKeys - 1) / kTileKeys - item.lo_tile);
     }
-    item.first_tile = (int)((int64_t)item.tiles * item.split / t.splits);
-    item.tiles = (int)((int64_t)item.tiles * (item.split + 1) / t.splits) - item.first_tile;
+    item.valid = 1;
+    item.first_tile = 0;
+    if (t.splits > 1) {  // tiles x splits stays below 2^32: 2^31 tokens in tiles of 128, a split per SM at most
+        const uint32_t tiles = item.tiles, splits = t.splits;
+        item.first_tile = (int)(tiles * (uint32_t)item.split / splits);
+        item.tiles = (int)(tiles * (uint32_t)(item.split + 1) / splits) - item.first_tile;
+    }
     return true;
 }
 
@@ -316,12 +333,13 @@ template <class T, int D, bool MODS>
 __global__ void __launch_bounds__(kThreads, 1) attention_tiles(const __grid_constant__ TileParams t) {
     using S = Shape<D>;
     extern __shared__ unsigned char raw[];
-    __shared__ __align__(8) uint64_t full[S::kSlots], empty[S::kSlots], queries_in[2], scores[2], weights[2][2], outputs[2],
-        drain;
+    __shared__ __align__(8) uint64_t full[S::kSlots], empty[S::kSlots];  // ring: filled by copies, read by products
+    __shared__ __align__(8) uint64_t queries_in, queries_read;
+    __shared__ __align__(8) uint64_t scores[2], weights[2][2], outputs[2];  // by tile of 128 rows (and half of its keys)
+    __shared__ __align__(8) uint64_t item_in[2], item_read[2], drain;
     __shared__ uint32_t tmem_base;
     __shared__ int gave_up;
-    __shared__ Item shared_item;
-    __shared__ int has_item;
+    __shared__ Item items[2];
     const AttnParams &p = t.a;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const uint32_t base = (smem_u32(raw) + 1023) & ~1023u;  // swizzled tiles start on 1024 bytes
@@ -333,8 +351,11 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tiles(const __grid_cons
             asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(smem_u32(bar)), "r"(count) : "memory");
         };
         for (int i = 0; i < S::kSlots; ++i) init(&full[i], 1), init(&empty[i], 1);
-        for (int i = 0; i < 2; ++i) init(&queries_in[i], 128), init(&scores[i], 1), init(&weights[i][0], 128), init(&weights[i][1], 128), init(&outputs[i], 1);
-        init(&drain, 1);
+        for (int i = 0; i < 2; ++i) {
+            init(&scores[i], 1), init(&outputs[i], 1), init(&weights[i][0], 128), init(&weights[i][1], 128);
+            init(&item_in[i], 1), init(&item_read[i], kItemReaders);
+        }
+        init(&queries_in, 1), init(&queries_read, 1), init(&drain, 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == kIssueWarp) {
@@ -343,52 +364,44 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tiles(const __grid_cons
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
         fence_before();
     }
-    wait_prerequisites();
-    launch_dependents();  // after the wait: what starts now may read all that came before this kernel
-    if (warp == 0) {
-        Item item;
-        const bool found = find_item(t, blockIdx.x, item);
-        if (lane == 0) {
-            has_item = found;
-            if (found) shared_item = item;
-        }
-    }
     __syncthreads();
     fence_after();
+    wait_prerequisites();
+    launch_dependents();  // after the wait: what starts now may read all that came before this kernel
     // All 512 columns there are, so the allocation starts at column 0; the issuing warp counts on it (constants stay out
-    // of its way to the tensor cores), which the softmax's addresses make good for the rest.
+    // of its way to the tensor cores).
     const uint32_t tmem = tmem_base;
-    const Item &item = shared_item;
-    const int n_tiles = has_item ? item.tiles : 0;
-    const int active = !has_item ? 0 : item.rows > 128 ? 2 : 1;  // tiles of 128 rows in use
+
+    // Item n of the CTA, in turn for every warp that reads items; false: there are no more (or a wait ran out).
+    auto next_item = [&](int n, Item &item) {
+        if (!warp_waits(smem_u32(&item_in[n & 1]), (n >> 1) & 1, &gave_up)) return false;
+        item = items[n & 1];
+        __syncwarp();
+        if (lane == 0) arrive(smem_u32(&item_read[n & 1]));
+        return item.valid != 0;
+    };
+    auto active_of = [&](const Item &item) { return item.tokens > t.tile_tokens ? 2 : 1; };  // tiles of rows in use
 
     if (warp < kSoftmaxWarps) {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegisters));
         const int g = warp >> 2, row = tid & 127;
-        if (g < active) {
+        const int row_token = row / p.group, row_head = row - row_token * p.group;
+        const uint32_t s_tmem = tmem + ((uint32_t)(warp & 3) << 21) + g * 128;
+        const uint32_t o_tmem = tmem + ((uint32_t)(warp & 3) << 21) + S::kOutColumn + g * D;
+        const uint32_t stage = ring + S::kSlots * S::kTileBytes + warp * S::kStageBytes;
+        const float scale_log2 = p.scale * kLog2e;
+        const float cap_in = p.softcap > 0.f ? scale_log2 * 2.f / p.softcap : 0.f, cap_out = p.softcap * kLog2e;
+        uint32_t score_phase = 0, output_phase = 0;
+        int ring_at = 0;  // tiles of keys walked before this item
+        Item item;
+        bool ok = true;
+        for (int n = 0; ok && next_item(n, item); ring_at += item.tiles, ++n) {
+            if (g >= active_of(item)) continue;
             // ---- this thread's row
-            const int in_item = g * 128 + row;
-            const bool valid = in_item < item.rows;
-            const int r = item.row0 + in_item;
-            const int token = valid ? r / p.group : 0;
-            const int head = item.head * p.group + (valid ? r - token * p.group : 0);
-            {
-                const uint4 *from = reinterpret_cast<const uint4 *>(
-                    p.query + (int64_t)(item.q.q0 + token) * p.q_token_stride + (int64_t)head * p.q_head_stride);
-                uint4 v[D / 8];  // all in flight at once
-#pragma unroll
-                for (int c = 0; c < D / 8; ++c) v[c] = valid ? from[c] : make_uint4(0, 0, 0, 0);
-                const uint32_t to = base + g * S::kTileBytes + row * 128;
-#pragma unroll
-                for (int c = 0; c < D / 8; ++c) {
-                    const uint32_t at = to + (c >> 3) * S::kHalfBytes + (((c & 7) ^ (row & 7)) << 4);
-                    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(v[c].x), "r"(v[c].y),
-                                 "r"(v[c].z), "r"(v[c].w)
-                                 : "memory");
-                }
-                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-                arrive(smem_u32(&queries_in[g]));
-            }
+            const int in_item = g * t.tile_tokens + row_token;
+            const bool valid = row_token < t.tile_tokens && in_item < item.tokens;
+            const int token = item.token0 + (valid ? in_item : 0);
+            const int head = item.head * p.group + row_head;
             // What the row sees of its sequence's own keys: [see_lo, see_hi) and everything below see_below.
             int position = 0, see_lo = 0, see_hi = 0, see_below = 0;
             float slope = 0.f;
@@ -417,19 +430,15 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tiles(const __grid_cons
             }
             if (MODS && p.slopes && valid) slope = p.slopes[head] * kLog2e;
 
-            const float scale_log2 = p.scale * kLog2e;
-            const float cap_in = p.softcap > 0.f ? scale_log2 * 2.f / p.softcap : 0.f, cap_out = p.softcap * kLog2e;
-            const uint32_t s_tmem = tmem + ((uint32_t)(warp & 3) << 21) + g * 128;
-            const uint32_t o_tmem = tmem + ((uint32_t)(warp & 3) << 21) + S::kOutColumn + g * D;
             float m = -INFINITY;
             float2 sum = make_float2(0.f, 0.f);
-            bool ok = true;
-            for (int i = 0; i < n_tiles; ++i) {
+            for (int i = 0; i < item.tiles; ++i) {
                 const TileAt at = tile_at(p, item, i);
-                if (!warp_waits(smem_u32(&scores[g]), i & 1, &gave_up)) {
+                if (!warp_waits(smem_u32(&scores[g]), score_phase, &gave_up)) {
                     ok = false;
                     break;
                 }
+                score_phase ^= 1;
                 fence_after();
                 // Scores that a mask, cap or bias changes go back to TMEM as they are then.
                 const bool sees_all = !valid ? true
@@ -491,8 +500,8 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tiles(const __grid_cons
                 }
                 // Values that no row sees (past the length, ahead of the window) may hold anything: 0 times NaN is NaN.
                 if (at.t0 < at.lo || at.t0 + kTileKeys > at.hi) {
-                    const int slot = (2 * i + 1) % S::kSlots;
-                    if (!warp_waits(smem_u32(&full[slot]), ((2 * i + 1) / S::kSlots) & 1, &gave_up)) {
+                    const int copy = 2 * (ring_at + i) + 1, slot = copy % S::kSlots;
+                    if (!warp_waits(smem_u32(&full[slot]), (copy / S::kSlots) & 1, &gave_up)) {
                         ok = false;
                         break;
                     }
@@ -533,46 +542,71 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tiles(const __grid_cons
                 }
             }
             // ---- the row's output
-            if (ok && n_tiles > 0) {
-                ok = warp_waits(smem_u32(&outputs[g]), 0, &gave_up);
+            if (ok && item.tiles > 0) {
+                ok = warp_waits(smem_u32(&outputs[g]), output_phase, &gave_up);
+                output_phase ^= 1;
                 fence_after();
             }
-            if (ok) {
-                const float total = sum.x + sum.y;
-                const int out_token = item.q.q0 + token;
-                const bool partial = t.prefix_only || t.splits > 1;
-                const int64_t at = ((int64_t)item.split * p.num_tokens + out_token) * p.q_heads + head;
-                const float factor = partial ? 1.f : total == 0.f ? 0.f : 1.f / total;
+            if (!ok) break;
+            const float total = sum.x + sum.y;
+            const bool partial = t.prefix_only || t.splits > 1;
+            const float factor = partial ? 1.f : total == 0.f ? 0.f : 1.f / total;
+            // 128 bytes of each of the warp's 32 rows at a time go through shared memory, so that they leave in whole
+            // lines: 32 partial ones or 64 finished ones.
+            auto staged = [&](int chunk) { return stage + lane * 128 + ((chunk ^ (lane & 7)) << 4); };
+            auto write_out = [&](uint64_t to, int64_t byte) {  // `to`: this thread's row
+                __syncwarp();
 #pragma unroll
-                for (int c = 0; c < D / 32; ++c) {
-                    float o[32];
-                    if (n_tiles > 0) {
-                        load32(o_tmem + c * 32, o);
-                        wait_loads();
-                    } else {
-#pragma unroll
-                        for (int e = 0; e < 32; ++e) o[e] = 0.f;
-                    }
-                    if (!valid) continue;
-                    if (partial) {
-                        float4 *to = reinterpret_cast<float4 *>(p.split_o + at * D + c * 32);
-#pragma unroll
-                        for (int e = 0; e < 8; ++e) to[e] = make_float4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
-                    } else {
-                        uint4 *to = reinterpret_cast<uint4 *>(p.out + (int64_t)out_token * p.out_token_stride +
-                                                              (int64_t)head * p.out_head_stride + c * 64);
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            const float *v = o + 8 * e;
-                            to[e] = make_uint4(Pack2<T>::of(v[0] * factor, v[1] * factor),
-                                               Pack2<T>::of(v[2] * factor, v[3] * factor),
-                                               Pack2<T>::of(v[4] * factor, v[5] * factor),
-                                               Pack2<T>::of(v[6] * factor, v[7] * factor));
-                        }
-                    }
+                for (int k = 0; k < 8; ++k) {  // 4 rows of 8 chunks at once
+                    const int from_row = 4 * k + (lane >> 3), chunk = lane & 7;
+                    const uint64_t at = __shfl_sync(~0u, to, from_row);
+                    uint4 v;
+                    asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+                                 : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+                                 : "r"(stage + from_row * 128 + ((chunk ^ (from_row & 7)) << 4)));
+                    if (at) *reinterpret_cast<uint4 *>(at + byte + chunk * 16) = v;
                 }
-                if (partial && valid) p.split_ml[at] = make_float2(m, total);
+                __syncwarp();
+            };
+            const int out_token = item.q.q0 + token;
+            const int64_t split_row = ((int64_t)item.split * p.num_tokens + out_token) * p.q_heads + head;
+            uint64_t to = 0;
+            if (valid)
+                to = partial ? reinterpret_cast<uint64_t>(p.split_o + split_row * D)
+                             : p.out + (int64_t)out_token * p.out_token_stride + (int64_t)head * p.out_head_stride;
+#pragma unroll
+            for (int c = 0; c < D / 32; ++c) {
+                float o[32];
+                if (item.tiles > 0) {
+                    load32(o_tmem + c * 32, o);
+                    wait_loads();
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 32; ++e) o[e] = 0.f;
+                }
+                if (partial) {
+#pragma unroll
+                    for (int e = 0; e < 8; ++e)
+                        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(staged(e)), "f"(o[4 * e]),
+                                     "f"(o[4 * e + 1]), "f"(o[4 * e + 2]), "f"(o[4 * e + 3])
+                                     : "memory");
+                    write_out(to, c * 128);
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const float *v = o + 8 * e;
+                        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(staged((c & 1) * 4 + e)),
+                                     "r"(Pack2<T>::of(v[0] * factor, v[1] * factor)),
+                                     "r"(Pack2<T>::of(v[2] * factor, v[3] * factor)),
+                                     "r"(Pack2<T>::of(v[4] * factor, v[5] * factor)),
+                                     "r"(Pack2<T>::of(v[6] * factor, v[7] * factor))
+                                     : "memory");
+                    }
+                    if (c & 1) write_out(to, (c >> 1) * 128);
+                }
             }
+            if (partial && valid) p.split_ml[split_row] = make_float2(m, total);
+            fence_before();  // the next item's first product overwrites what was read
         }
     } else {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegisters));
@@ -616,94 +650,166 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tiles(const __grid_cons
             if (elect_one()) commit(smem_u32(bar));
             __syncwarp();
         };
-        // Ring order: K 0, V 0, K 1, V 1, ...
-        if (n_tiles > 0 && wait(&full[0], 0)) {
-            for (int g = 0; g < active; ++g)
-                if (wait(&queries_in[g], 0)) {
+        // The ring holds K 0, V 0, K 1, V 1, ... of item after item.
+        int k_slot = 0, v_slot = 1;
+        uint32_t ring_phase[2] = {0, 0};  // of the K and the V copy that come next
+        uint32_t weight_phase[2] = {0, 0}, query_phase = 0;
+        auto advance = [&](int &slot, uint32_t &phase) {
+            if ((slot += 2) >= S::kSlots) slot -= S::kSlots, phase ^= 1;
+        };
+        Item item;
+        for (int n = 0; ok && next_item(n, item); ++n) {
+            const int active = active_of(item);
+            if (item.tiles == 0) continue;
+            if (!wait(&queries_in, query_phase) || !wait(&full[k_slot], ring_phase[0])) break;
+            query_phase ^= 1;
+            fence_after();
+            // A tile's first scores land where the last item's weights were, behind the product that read them.
+            for (int g = 0; g < active; ++g) score(g, k_slot);
+            finished(&empty[k_slot]);
+            if (item.tiles == 1) finished(&queries_read);
+            advance(k_slot, ring_phase[0]);
+            for (int i = 0; ok && i < item.tiles; ++i) {
+                const bool more = i + 1 < item.tiles;
+                if (!wait(&full[v_slot], ring_phase[1])) break;
+                for (int g = 0; g < active; ++g) {
+                    if (!wait(&weights[g][0], weight_phase[g])) break;
                     fence_after();
-                    score(g, 0);
+                    output(g, v_slot, 0, i > 0);
+                    if (more && g == 0 && !wait(&full[k_slot], ring_phase[0])) break;
+                    if (!wait(&weights[g][1], weight_phase[g])) break;
+                    weight_phase[g] ^= 1;
+                    fence_after();
+                    output(g, v_slot, 1, true);
+                    // The scores land where the weights were: the products execute in the order they are issued.
+                    if (!more) finished(&outputs[g]);
+                    else score(g, k_slot);
                 }
-            finished(&empty[0]);
-        }
-        int v_slot = 1 % S::kSlots, k_slot = 2 % S::kSlots;
-        uint32_t v_phase = 0, k_phase = 0;
-        for (int i = 0; ok && i < n_tiles; ++i) {
-            const bool more = i + 1 < n_tiles;
-            if (!wait(&full[v_slot], v_phase)) break;
-            if (more && !wait(&full[k_slot], k_phase)) break;
-            for (int g = 0; g < active; ++g) {
-                if (!wait(&weights[g][0], i & 1)) break;
-                fence_after();
-                output(g, v_slot, 0, i > 0);
-                if (!wait(&weights[g][1], i & 1)) break;
-                fence_after();
-                output(g, v_slot, 1, true);
-                // The scores land where the weights were: the products execute in the order they are issued.
-                if (more) score(g, k_slot);
-                else finished(&outputs[g]);
-            }
-            if (ok) {
+                if (!ok) break;
                 finished(&empty[v_slot]);
-                if (more) finished(&empty[k_slot]);
-            }
-            if ((v_slot += 2) >= S::kSlots) v_slot -= S::kSlots, v_phase ^= 1;
-            if ((k_slot += 2) >= S::kSlots) k_slot -= S::kSlots, k_phase ^= 1;
-        }
-        if (lane == 0) {
-            if (!ok) {  // a wait ran out: let what was issued end before TMEM is freed
-                commit(smem_u32(&drain));
-                const uint64_t deadline = globaltimer() + kWaitNs;
-                while (!mbar_try_wait(smem_u32(&drain), 0) && globaltimer() < deadline) {
+                advance(v_slot, ring_phase[1]);
+                if (more) {
+                    finished(&empty[k_slot]);
+                    if (i + 2 == item.tiles) finished(&queries_read);
+                    advance(k_slot, ring_phase[0]);
                 }
+            }
+        }
+        if (!ok) {  // a wait ran out: let what was issued end before TMEM is freed
+            finished(&drain);
+            const uint64_t deadline = globaltimer() + kWaitNs;
+            while (!mbar_try_wait(smem_u32(&drain), 0) && globaltimer() < deadline) {
             }
         }
         __syncwarp();
     } else if (warp == kLoadWarp) {
-        // ---- loads: K 0, V 0, K 1, V 1, ... into the ring, one copy of `box` tokens x 64 elements per lane at a time
-        const int boxes = kTileKeys / t.box, copies = boxes * S::kHalves;
+        // ---- K 0, V 0, K 1, V 1, ... into the ring, one copy of `box` tokens x 64 elements per lane
+        const int boxes = kTileKeys / t.box, copies = boxes * S::kHalves;  // at most 32: 8-token boxes, 128-wide heads
+        const int half = lane / boxes, box = lane - half * boxes;
         int issued = 0;
         bool ok = true;
-        for (int n = 0; n < 2 * n_tiles; ++n) {
-            const int slot = n % S::kSlots;
-            if (n >= S::kSlots &&
-                !warp_waits(smem_u32(&empty[slot]), ((n / S::kSlots) & 1) ^ 1, &gave_up)) {
-                ok = false;
-                break;
-            }
-            const TileAt at = tile_at(p, item, n / 2);
-            const int32_t *table = at.shared ? p.shared_table : p.block_tables + (int64_t)item.sequence * p.table_stride;
-            // Up to 32 copies a tile (8-token boxes of 128-wide heads): one per lane.
-            const int half = lane / boxes, box = lane - half * boxes;
-            const int k = at.t0 + box * t.box;
-            const bool wanted = lane < copies && k < at.hi && k + t.box > at.lo;
-            int block = 0, in_block = 0;
-            if (wanted) {
-                const int b = p.block_shift >= 0 ? k >> p.block_shift : k / p.block_size;
-                in_block = k - b * p.block_size;
-                block = table[b];
-                if (block < 0 || block >= p.num_blocks) {
-                    flag_error(p.error_word, p.status, kErrPastCache);
-                    block = p.num_blocks;  // past the tensor: the copy fills in zeros
+        Item item;
+        for (int n = 0; ok && next_item(n, item); ++n) {
+            const int32_t *own_table = p.block_tables + (int64_t)item.sequence * p.table_stride;
+            for (int i = 0; ok && i < item.tiles; ++i) {
+                const TileAt at = tile_at(p, item, i);
+                const int k = at.t0 + box * t.box;
+                const bool wanted = lane < copies && k < at.hi && k + t.box > at.lo;
+                int block = 0, in_block = 0;
+                if (wanted) {
+                    const int b = p.block_shift >= 0 ? k >> p.block_shift : k / p.block_size;
+                    in_block = k - b * p.block_size;
+                    block = (at.shared ? p.shared_table : own_table)[b];
+                    if (block < 0 || block >= p.num_blocks) {
+                        flag_error(p.error_word, p.status, kErrPastCache);
+                        block = p.num_blocks;  // past the tensor: the copy fills in zeros
+                    }
+                }
+                const int bytes = __popc(__ballot_sync(~0u, wanted)) * t.box * 128;
+                for (int kv = 0; kv < 2; ++kv, ++issued) {
+                    const int slot = issued % S::kSlots;
+                    if (issued >= S::kSlots &&
+                        !warp_waits(smem_u32(&empty[slot]), ((issued / S::kSlots) & 1) ^ 1, &gave_up)) {
+                        ok = false;
+                        break;
+                    }
+                    const uint32_t bar = smem_u32(&full[slot]);
+                    if (lane == 0)
+                        asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes)
+                                     : "memory");
+                    __syncwarp();
+                    if (wanted)
+                        copy_box(ring + slot * S::kTileBytes + half * S::kHalfBytes + box * t.box * 128,
+                                 kv ? &t.values : &t.keys, half * 64, in_block, item.head, block, bar);
                 }
             }
-            const int count = __popc(__ballot_sync(~0u, wanted));
-            const uint32_t bar = smem_u32(&full[slot]);
-            if (lane == 0)
-                asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(count * t.box * 128)
-                             : "memory");
-            __syncwarp();
-            if (wanted)
-                copy_box(ring + slot * S::kTileBytes + half * S::kHalfBytes + box * t.box * 128,
-                         (n & 1) ? &t.values : &t.keys, half * 64, in_block, item.head, block, bar);
-            issued = n + 1;
         }
-        if (!ok || gave_up) {  // copies may still be landing: give each a bounded wait before the CTA ends
+        // Copies that nobody waited for (a wait ran out) may still be landing: give each a bounded wait.
+        __syncwarp();
+        if (*(volatile int *)&gave_up) {
             const uint64_t deadline = globaltimer() + kWaitNs;
-            for (int n = max(0, issued - S::kSlots); n < issued; ++n)
-                while (!mbar_try_wait(smem_u32(&full[n % S::kSlots]), (n / S::kSlots) & 1) && globaltimer() < deadline) {
+            for (int c = max(0, issued - S::kSlots); c < issued; ++c)
+                while (!mbar_try_wait(smem_u32(&full[c % S::kSlots]), (c / S::kSlots) & 1) && globaltimer() < deadline) {
                 }
         }
         __syncwarp();
+    } else if (warp == kQueryWarp) {
+        // ---- query rows: one copy per tile and 64 columns. Rows past the tokens there are come as zeros or as the next
+        // sequence's, those past a tile's whole tokens as whatever was there: each row's scores are its own.
+        const int bytes = t.tile_tokens * p.group * 128;  // of a copy
+        uint32_t read_phase = 0;
+        bool waiting = false;  // for the products that read the queries before
+        Item item;
+        for (int n = 0; next_item(n, item); ++n) {
+            if (item.tiles == 0) continue;  // nothing reads them
+            if (waiting && !warp_waits(smem_u32(&queries_read), read_phase, &gave_up)) break;
+            if (waiting) read_phase ^= 1;
+            waiting = true;
+            const int copies = active_of(item) * S::kHalves;
+            const uint32_t bar = smem_u32(&queries_in);
+            if (lane == 0)
+                asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(copies * bytes)
+                             : "memory");
+            __syncwarp();
+            if (lane < copies) {
+                const int g = lane / S::kHalves, half = lane % S::kHalves;
+                asm volatile(
+                    "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, "
+                    "%4}], [%5];" ::"r"(base + g * S::kTileBytes + half * S::kHalfBytes),
+                    "l"(&t.queries), "r"(half * 64), "r"(item.head * p.group),
+                    "r"(item.q.q0 + item.token0 + g * t.tile_tokens), "r"(bar)
+                    : "memory");
+            }
+        }
+        if (*(volatile int *)&gave_up && waiting) {  // a copy may still be landing
+            const uint64_t deadline = globaltimer() + kWaitNs;
+            while (!mbar_try_wait(smem_u32(&queries_in), read_phase) && globaltimer() < deadline) {
+            }
+        }
+        __syncwarp();
+    } else if (warp == kPlanWarp) {
+        // ---- what to do: the CTA's first item by its number, then whichever is next
+        int id = blockIdx.x;
+        for (int n = 0;; ++n) {
+            Item item;
+            int count = 0;
+            item.valid = 0;
+            const bool found = find_item(t, id, item, count);
+            if (n >= 2 && !warp_waits(smem_u32(&item_read[n & 1]), ((n >> 1) & 1) ^ 1, &gave_up)) break;
+            if (lane == 0) {
+                items[n & 1] = item;
+                if (!found) items[n & 1].valid = 0;
+                arrive(smem_u32(&item_in[n & 1]));
+                if (found) {
+                    id = gridDim.x + atomicAdd(t.next, 1);
+                    // One draw per item: the last of all puts the counter back.
+                    if (id - (int)gridDim.x == count - 1) *t.next = 0;
+                }
+            }
+            __syncwarp();
+            if (!found) break;
+            id = __shfl_sync(~0u, id, 0);
+        }
     }
     fence_before();
     __syncthreads();
@@ -728,8 +834,9 @@ __global__ void __launch_bounds__(kJoinThreads) attention_join(const __grid_cons
     const int part = blockIdx.x % kParts, id = blockIdx.x / kParts;
     if (threadIdx.x < 32) {
         Item item;
+        int count;
         // Item ids count (row tile, split, head); every split holds the same rows.
-        const bool found = find_item(t, id / p.kv_heads * p.kv_heads * t.splits + id % p.kv_heads, item);
+        const bool found = find_item(t, id / p.kv_heads * p.kv_heads * t.splits + id % p.kv_heads, item, count);
         if (threadIdx.x == 0) {
             has_item = found;
             if (found) shared_item = item;
@@ -741,10 +848,11 @@ __global__ void __launch_bounds__(kJoinThreads) attention_join(const __grid_cons
     constexpr int kQuads = D / 4;
     const int64_t step = (int64_t)p.num_tokens * p.q_heads;
     for (int k = threadIdx.x; k < kJoinRows * kQuads; k += kJoinThreads) {
-        const int in_item = part * kJoinRows + k / kQuads, quad = k % kQuads;
-        if (in_item >= item.rows) break;
-        const int r = item.row0 + in_item, token = r / p.group;
-        const int head = item.head * p.group + r - token * p.group;
+        const int r = part * kJoinRows + k / kQuads, quad = k % kQuads;
+        const int in_tile = (r & 127) / p.group, in_item = (r >> 7) * t.tile_tokens + in_tile;
+        if (in_tile >= t.tile_tokens || in_item >= item.tokens) continue;
+        const int token = item.token0 + in_item;
+        const int head = item.head * p.group + (r & 127) - in_tile * p.group;
         const int64_t at = (int64_t)(item.q.q0 + token) * p.q_heads + head;
         Joined j;
         join_parts(j, t.splits, p.split_ml, p.split_o, kQuads, quad, [&](int i) { return at + i * step; });
@@ -773,19 +881,34 @@ EncodeTiled encode_tiled() {
     return fn;
 }
 
-int make_map(CUtensorMap *map, const AttnParams &p, uint64_t cache, int head_dim, int dtype, int box) {
-    EncodeTiled encode = encode_tiled();
-    if (!encode) return fail(KVX_ERR_CUDA, "the driver has no cuTensorMapEncodeTiled");
+int encode(CUtensorMap *map, int rank, uint64_t address, int dtype, const cuuint64_t *dims, const cuuint64_t *strides,
+           const cuuint32_t *box) {
+    EncodeTiled fn = encode_tiled();
+    if (!fn) return fail(KVX_ERR_CUDA, "the driver has no cuTensorMapEncodeTiled");
+    const cuuint32_t steps[4] = {1, 1, 1, 1};
+    const CUresult rc = fn(map, dtype == KVX_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16,
+                           rank, reinterpret_cast<void *>(address), dims, strides, box, steps,
+                           CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                           CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (rc != CUDA_SUCCESS) return fail(KVX_ERR_CUDA, "cuTensorMapEncodeTiled failed: %d", (int)rc);
+    return KVX_OK;
+}
+
+// A cache by (element, token of a block, head, block), copied 64 elements of `box` tokens at a time.
+int cache_map(CUtensorMap *map, const AttnParams &p, uint64_t cache, int head_dim, int dtype, int box) {
     const cuuint64_t dims[4] = {(cuuint64_t)head_dim, (cuuint64_t)p.block_size, (cuuint64_t)p.kv_heads,
                                 (cuuint64_t)p.num_blocks};
     const cuuint64_t strides[3] = {(cuuint64_t)p.token_stride, (cuuint64_t)p.head_stride, (cuuint64_t)p.block_stride};
-    const cuuint32_t boxes[4] = {64, (cuuint32_t)box, 1, 1}, steps[4] = {1, 1, 1, 1};
-    const CUresult rc = encode(map, dtype == KVX_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16,
-                               4, reinterpret_cast<void *>(cache), dims, strides, boxes, steps,
-                               CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
-                               CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-    if (rc != CUDA_SUCCESS) return fail(KVX_ERR_CUDA, "cuTensorMapEncodeTiled failed: %d", (int)rc);
-    return KVX_OK;
+    const cuuint32_t boxes[4] = {64, (cuuint32_t)box, 1, 1};
+    return encode(map, 4, cache, dtype, dims, strides, boxes);
+}
+
+// The queries by (element, head, token), copied 64 elements of a KV head's group and some tokens at a time.
+int query_map(CUtensorMap *map, const AttnParams &p, int head_dim, int dtype, int tokens) {
+    const cuuint64_t dims[3] = {(cuuint64_t)head_dim, (cuuint64_t)p.q_heads, (cuuint64_t)p.num_tokens};
+    const cuuint64_t strides[2] = {(cuuint64_t)p.q_head_stride, (cuuint64_t)p.q_token_stride};
+    const cuuint32_t boxes[3] = {64, (cuuint32_t)p.group, (cuuint32_t)tokens};
+    return encode(map, 3, p.query, dtype, dims, strides, boxes);
 }
 
 template <class Kernel>
@@ -807,11 +930,12 @@ int launch(Kernel kernel, const TileParams &t, int64_t grid, int threads, int sm
 }
 
 template <class T, int D>
-int launch_typed(const TileParams &t, bool mods, cudaStream_t stream) {
+int launch_typed(const TileParams &t, bool mods, int sms, cudaStream_t stream) {
     auto kernel = mods ? attention_tiles<T, D, true> : attention_tiles<T, D, false>;
     KVX_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape<D>::kBytes));
     const int64_t items = (int64_t)t.row_tiles * t.a.kv_heads;
-    if (int rc = launch(kernel, t, items * t.splits, kThreads, Shape<D>::kBytes, stream)) return rc;
+    const int64_t grid = std::min<int64_t>(items * t.splits, sms);  // one CTA per SM, item after item
+    if (int rc = launch(kernel, t, grid, kThreads, Shape<D>::kBytes, stream)) return rc;
     if (t.prefix_only || t.splits == 1) return KVX_OK;
     return launch(attention_join<T, D>, t, items * (kTileRows / kJoinRows), kJoinThreads, 0, stream);
 }
@@ -821,25 +945,29 @@ int launch_typed(const TileParams &t, bool mods, cudaStream_t stream) {
 int kvx::tile_box(const AttnParams &p) {
     // A copy lies within one block and fills whole 8-row groups of the swizzle: the block size's largest power of two.
     const int box = std::min(p.block_size & -p.block_size, kTileKeys);
-    const bool strides = p.token_stride > 0 && p.head_stride > 0 && p.block_stride > 0 &&
-                         std::max({p.token_stride, p.head_stride, p.block_stride}) < (int64_t)1 << 40;
+    bool strides = p.group <= 128;  // a token's rows fit a tile
+    for (int64_t stride : {p.token_stride, p.head_stride, p.block_stride, p.q_head_stride, p.q_token_stride})
+        strides = strides && stride > 0 && stride < (int64_t)1 << 40;
     return box >= 8 && strides && p.num_blocks > 0 ? box : 0;
 }
 
 int kvx::launch_tiles(const AttnParams &p, int head_dim, int dtype, bool mods, bool prefix_only, int splits,
-                      cudaStream_t stream) {
+                      int sms, cudaStream_t stream) {
     TileParams t;
     t.a = p;
     t.box = tile_box(p);
     t.splits = splits;
     t.prefix_only = prefix_only;
-    const int64_t rows = (int64_t)p.num_tokens * p.group;
-    t.row_tiles = (int)((rows + kTileRows - 1) / kTileRows) + (prefix_only ? 0 : p.batch - 1);
-    if (int rc = make_map(&t.keys, p, p.k_cache, head_dim, dtype, t.box)) return rc;
-    if (int rc = make_map(&t.values, p, p.v_cache, head_dim, dtype, t.box)) return rc;
+    t.next = p.counters + kTileCounter;
+    t.tile_tokens = 128 / p.group;
+    const int tokens = 2 * t.tile_tokens;
+    t.row_tiles = (p.num_tokens + tokens - 1) / tokens + (prefix_only ? 0 : p.batch - 1);
+    if (int rc = cache_map(&t.keys, p, p.k_cache, head_dim, dtype, t.box)) return rc;
+    if (int rc = cache_map(&t.values, p, p.v_cache, head_dim, dtype, t.box)) return rc;
+    if (int rc = query_map(&t.queries, p, head_dim, dtype, t.tile_tokens)) return rc;
     if (head_dim == 128)
-        return dtype == KVX_BF16 ? launch_typed<__nv_bfloat16, 128>(t, mods, stream)
-                                 : launch_typed<__half, 128>(t, mods, stream);
-    return dtype == KVX_BF16 ? launch_typed<__nv_bfloat16, 64>(t, mods, stream)
-                             : launch_typed<__half, 64>(t, mods, stream);
+        return dtype == KVX_BF16 ? launch_typed<__nv_bfloat16, 128>(t, mods, sms, stream)
+                                 : launch_typed<__half, 128>(t, mods, sms, stream);
+    return dtype == KVX_BF16 ? launch_typed<__nv_bfloat16, 64>(t, mods, sms, stream)
+                             : launch_typed<__half, 64>(t, mods, sms, stream);
 }
