@@ -167,6 +167,264 @@ __global__ void __launch_bounds__(kAnyThreads) rotate_store_any(const __grid_con
     }
 }
 
+// ---- the form for the usual heads: 64, 128 or 256 wide, aligned rows, a rotary_dim that is a multiple of 8
+//
+// A row takes D / 8 lanes, each with the two 4-element pieces that rotate into each other (elements p and
+// p + rotary_dim / 2, or 8 neighbours when interleaved or not rotated), so that no element changes lanes; the sum of
+// squares is the one exchange. A warp takes PASSES x (256 / D) rows of one token, all their loads in flight at once, and
+// reads the token's angles, slot and norm weights once for them. Bound by HBM: a step's rows in and out, once.
+
+constexpr int kFastThreads = 256;
+
+template <class T>
+struct Piece {  // four elements
+    uint2 bits;
+    __device__ __forceinline__ void get(float (&x)[4]) const {
+        const T *e = reinterpret_cast<const T *>(&bits);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x[i] = to_float(e[i]);
+    }
+    __device__ __forceinline__ void set(const float (&x)[4]) {
+        T *e = reinterpret_cast<T *>(&bits);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) e[i] = from_float<T>(x[i]);
+    }
+};
+
+// Rows may be the output's own (queries rotated in place), so they are read as ordinary memory, past L1.
+template <class T>
+__device__ __forceinline__ Piece<T> load_piece(uint64_t at) {
+    Piece<T> p;
+    asm volatile("ld.global.L1::no_allocate.v2.u32 {%0, %1}, [%2];" : "=r"(p.bits.x), "=r"(p.bits.y) : "l"(at));
+    return p;
+}
+template <class T>
+__device__ __forceinline__ void store_piece(uint64_t at, const Piece<T> &p) {
+    *reinterpret_cast<uint2 *>(at) = p.bits;
+}
+
+// A lane's place in a row, and its angles.
+struct Place {
+    int32_t a, b;  // first elements of its two pieces
+    bool rotated;
+};
+template <bool INTERLEAVED>
+__device__ __forceinline__ Place place_of(int lane_in_row, int rotary_dim) {
+    Place p;
+    p.rotated = 8 * lane_in_row < rotary_dim;
+    const bool halves = !INTERLEAVED && p.rotated;
+    p.a = halves ? 4 * lane_in_row : 8 * lane_in_row;
+    p.b = halves ? rotary_dim / 2 + 4 * lane_in_row : 8 * lane_in_row + 4;
+    return p;
+}
+
+template <bool INTERLEAVED>
+__device__ __forceinline__ void rotate(float (&a)[4], float (&b)[4], const float4 &cos4, const float4 &sin4) {
+    const float c[4] = {cos4.x, cos4.y, cos4.z, cos4.w}, s[4] = {sin4.x, sin4.y, sin4.z, sin4.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        float &x = INTERLEAVED ? (i < 2 ? a[2 * i] : b[2 * i - 4]) : a[i];
+        float &y = INTERLEAVED ? (i < 2 ? a[2 * i + 1] : b[2 * i - 3]) : b[i];
+        const float turned = x * c[i] - y * s[i];
+        y = y * c[i] + x * s[i];
+        x = turned;
+    }
+}
+
+// Writes a key or value row's pieces to every destination that takes its head. `at0`: the token's place in destination 0.
+template <class T>
+__device__ __forceinline__ void store_everywhere(const RotateParams &p, int64_t token, int64_t slot, int64_t at0, int head,
+                                                 bool value, int a, int b, const Piece<T> &x, const Piece<T> &y) {
+    for (int d = p.peers_only; d < p.n_dests; ++d) {
+        const StoreDest &dst = p.dests[d];
+        if (head < dst.src_first_head || head >= dst.src_first_head + dst.num_heads) continue;
+        const int64_t at = d == 0 ? at0 : dest_offset(p, d, token, slot);
+        if (at < 0) continue;
+        const uint64_t row = (value ? dst.v : dst.k) + at +
+                             (int64_t)(head - dst.src_first_head + dst.dst_first_head) * dst.head_stride;
+        store_piece<T>(row + a * sizeof(T), x);
+        store_piece<T>(row + b * sizeof(T), y);
+    }
+}
+
+// PASSES x (32 / LANES) rows of one token from `row0` on, of `rows` there are: queries, then keys, then values.
+template <class T, int LANES, int PASSES, bool INTERLEAVED>
+__device__ __forceinline__ void rotate_rows(const RotateParams &p, int64_t token, int row0, int rows, int64_t slot,
+                                            int64_t at0, const float *angle, const Piece<T> (&q_weight)[2],
+                                            const Piece<T> (&k_weight)[2], const Place &place) {
+    const int lane = threadIdx.x & 31, lane_in_row = lane % LANES;
+    Piece<T> x[PASSES], y[PASSES];
+    int kind[PASSES], head[PASSES];
+#pragma unroll
+    for (int i = 0; i < PASSES; ++i) {
+        const int r = row0 + i * (32 / LANES) + lane / LANES;
+        kind[i] = r < p.query.heads ? 0 : r < p.query.heads + p.key.heads ? 1 : 2;
+        head[i] = r - (kind[i] == 0 ? 0 : kind[i] == 1 ? p.query.heads : p.query.heads + p.key.heads);
+        if (r >= rows) kind[i] = 3;
+        const Rows &in = kind[i] == 0 ? p.query : kind[i] == 1 ? p.key : p.value;
+        const uint64_t at = in.base + token * in.token_stride + head[i] * in.head_stride;
+        x[i].bits = y[i].bits = make_uint2(0, 0);
+        if (kind[i] < 3) {
+            x[i] = load_piece<T>(at + place.a * sizeof(T));
+            y[i] = load_piece<T>(at + place.b * sizeof(T));
+        }
+    }
+    float4 cos4 = make_float4(1.f, 1.f, 1.f, 1.f), sin4 = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (place.rotated) {
+        cos4 = __ldg(reinterpret_cast<const float4 *>(angle) + lane_in_row);
+        sin4 = __ldg(reinterpret_cast<const float4 *>(angle + p.rotary_dim / 2) + lane_in_row);
+    }
+#pragma unroll
+    for (int i = 0; i < PASSES; ++i) {
+        float a[4], b[4];
+        x[i].get(a);
+        y[i].get(b);
+        const bool normed = (kind[i] == 0 && p.query.norm_dim > 0) || (kind[i] == 1 && p.key.norm_dim > 0);
+        float sum = 0.f;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) sum += a[e] * a[e] + b[e] * b[e];
+#pragma unroll
+        for (int o = LANES / 2; o; o >>= 1) sum += __shfl_xor_sync(~0u, sum, o);
+        if (kind[i] < 2) {
+            if (normed) {
+                const float scale = rsqrtf(sum * (1.f / (LANES * 8)) + p.eps);
+                float w[4], v[4];
+                (kind[i] == 0 ? q_weight[0] : k_weight[0]).get(w);
+                (kind[i] == 0 ? q_weight[1] : k_weight[1]).get(v);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) a[e] = a[e] * scale * w[e], b[e] = b[e] * scale * v[e];
+            }
+            if (place.rotated) rotate<INTERLEAVED>(a, b, cos4, sin4);
+            x[i].set(a);
+            y[i].set(b);
+        }
+        if (kind[i] == 0) {
+            const uint64_t out = p.out + token * p.out_token_stride + head[i] * p.out_head_stride;
+            store_piece<T>(out + place.a * sizeof(T), x[i]);
+            store_piece<T>(out + place.b * sizeof(T), y[i]);
+        } else if (kind[i] < 3) {
+            store_everywhere<T>(p, token, slot, at0, head[i], kind[i] == 2, place.a, place.b, x[i], y[i]);
+        }
+    }
+}
+
+// Where destination 0 keeps a token, or -1.
+__device__ __forceinline__ int64_t first_offset(const RotateParams &p, int64_t token, int64_t slot) {
+    return p.peers_only ? -1 : dest_offset(p, 0, token, slot);
+}
+
+template <class T, int LANES, int PASSES, bool INTERLEAVED>
+__global__ void __launch_bounds__(kFastThreads) rotate_store_fast(const __grid_constant__ RotateParams p) {
+    launch_dependents();
+    const int lane = threadIdx.x & 31;
+    const Place place = place_of<INTERLEAVED>(lane % LANES, p.rotary_dim);
+    const int rows = p.query.heads + p.key.heads + p.value.heads;
+    constexpr int kRows = PASSES * (32 / LANES);
+    const uint32_t per_token = (rows + kRows - 1) / kRows, n = per_token * (uint32_t)p.num_tokens;
+    wait_prerequisites();
+    Piece<T> q_weight[2], k_weight[2];
+    if (p.query.norm_dim > 0) {
+        q_weight[0] = load_piece<T>((uint64_t)p.query.weight + place.a * sizeof(T));
+        q_weight[1] = load_piece<T>((uint64_t)p.query.weight + place.b * sizeof(T));
+    }
+    if (p.key.norm_dim > 0) {
+        k_weight[0] = load_piece<T>((uint64_t)p.key.weight + place.a * sizeof(T));
+        k_weight[1] = load_piece<T>((uint64_t)p.key.weight + place.b * sizeof(T));
+    }
+    for (uint32_t w = blockIdx.x * (kFastThreads / 32) + threadIdx.x / 32; w < n; w += gridDim.x * (kFastThreads / 32)) {
+        const uint32_t token = w / per_token, row0 = (w - token * per_token) * kRows;
+        const int64_t slot = load_index(p.dests[0].slots, p.dests[0].slot_bytes, token);
+        const float *angle = p.rotary_dim ? angles(p, token, slot < 0) : nullptr;
+        const int64_t at0 = (int)row0 + kRows > p.query.heads ? first_offset(p, token, slot) : -1;
+        rotate_rows<T, LANES, PASSES, INTERLEAVED>(p, token, row0, rows, slot, at0, angle, q_weight, k_weight, place);
+    }
+}
+
+// Latent rows of 256 x CHUNKS normed elements (or plain ones) and 64 rotated ones, a warp each, and the queries' rotated
+// parts, 64 wide, 16 rows a warp.
+template <class T, int CHUNKS, bool INTERLEAVED>
+__global__ void __launch_bounds__(kFastThreads) rotate_latents_fast(const __grid_constant__ RotateParams p) {
+    launch_dependents();
+    const int lane = threadIdx.x & 31;
+    constexpr int kLanes = 8, kPasses = 4, kRows = kPasses * (32 / kLanes), kRank = 256 * CHUNKS;
+    const Place place = place_of<INTERLEAVED>(lane % kLanes, 64);
+    const uint32_t per_token = 1 + (p.query.heads + kRows - 1) / kRows, n = per_token * (uint32_t)p.num_tokens;
+    wait_prerequisites();
+    for (uint32_t w = blockIdx.x * (kFastThreads / 32) + threadIdx.x / 32; w < n; w += gridDim.x * (kFastThreads / 32)) {
+        const uint32_t token = w / per_token, item = w - token * per_token;
+        const int64_t slot = load_index(p.dests[0].slots, p.dests[0].slot_bytes, token);
+        const float *angle = angles(p, token, slot < 0);
+        if (item > 0) {
+            const Piece<T> none[2] = {};
+            rotate_rows<T, kLanes, kPasses, INTERLEAVED>(p, token, (item - 1) * kRows, p.query.heads, slot, -1, angle, none,
+                                                         none, place);
+            continue;
+        }
+        const uint64_t row = p.key.base + (int64_t)token * p.key.token_stride;
+        Piece<T> c[CHUNKS][2], x, y;
+#pragma unroll
+        for (int k = 0; k < CHUNKS; ++k)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) c[k][h] = load_piece<T>(row + ((k * 64 + h * 32 + lane) * 4) * sizeof(T));
+        if (lane < kLanes) {
+            x = load_piece<T>(row + (kRank + place.a) * sizeof(T));
+            y = load_piece<T>(row + (kRank + place.b) * sizeof(T));
+        }
+        if (p.key.norm_dim > 0) {
+            Piece<T> weight[CHUNKS][2];
+            float sum = 0.f;
+#pragma unroll
+            for (int k = 0; k < CHUNKS; ++k)
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    weight[k][h] = load_piece<T>((uint64_t)p.key.weight + ((k * 64 + h * 32 + lane) * 4) * sizeof(T));
+                    float v[4];
+                    c[k][h].get(v);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) sum += v[e] * v[e];
+                }
+#pragma unroll
+            for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(~0u, sum, o);
+            const float scale = rsqrtf(sum * (1.f / kRank) + p.eps);
+#pragma unroll
+            for (int k = 0; k < CHUNKS; ++k)
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    float v[4], m[4];
+                    c[k][h].get(v);
+                    weight[k][h].get(m);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) v[e] = v[e] * scale * m[e];
+                    c[k][h].set(v);
+                }
+        }
+        if (lane < kLanes) {
+            float a[4], b[4];
+            x.get(a);
+            y.get(b);
+            rotate<INTERLEAVED>(a, b, __ldg(reinterpret_cast<const float4 *>(angle) + lane),
+                                __ldg(reinterpret_cast<const float4 *>(angle + 32) + lane));
+            x.set(a);
+            y.set(b);
+        }
+        for (int d = p.peers_only; d < p.n_dests; ++d) {
+            const StoreDest &dst = p.dests[d];
+            if (dst.num_heads < 1) continue;
+            const int64_t at = dest_offset(p, d, token, slot);
+            if (at < 0) continue;
+            const uint64_t to = dst.k + at + (int64_t)dst.dst_first_head * dst.head_stride;
+#pragma unroll
+            for (int k = 0; k < CHUNKS; ++k)
+#pragma unroll
+                for (int h = 0; h < 2; ++h) store_piece<T>(to + ((k * 64 + h * 32 + lane) * 4) * sizeof(T), c[k][h]);
+            if (lane < kLanes) {
+                store_piece<T>(to + (kRank + place.a) * sizeof(T), x);
+                store_piece<T>(to + (kRank + place.b) * sizeof(T), y);
+            }
+        }
+    }
+}
+
 int check_rows(const char *what, const kvx_rotate_rows &r, int rotary_dim) {
     if (r.num_heads < 0 || r.dim < 1 || r.norm_dim < 0 || r.norm_dim > r.dim)
         return fail(KVX_ERR_INVALID, "%s: bad row shape: %d heads of %d, %d normed", what, r.num_heads, r.dim,
@@ -181,6 +439,60 @@ int check_rows(const char *what, const kvx_rotate_rows &r, int rotary_dim) {
 Rows rows_of(const kvx_rotate_rows &r) {
     return Rows{(uint64_t)(uintptr_t)r.rows, r.token_stride, r.head_stride, r.weight,
                 r.num_heads, r.dim, r.norm_dim, r.rotary_first};
+}
+
+// One warp per unit of work, in one resident wave of CTAs at most: each sweeps its share.
+int launch(void (*kernel)(RotateParams), const RotateParams &p, cudaLaunchConfig_t cfg, int64_t units, int sms) {
+    static_assert(kFastThreads == kAnyThreads, "one block size");
+    constexpr int kWarps = kFastThreads / 32, kCtasPerSm = 8;
+    cfg.gridDim = dim3((unsigned)std::min<int64_t>((units + kWarps - 1) / kWarps, (int64_t)sms * kCtasPerSm));
+    cfg.blockDim = dim3(kFastThreads);
+    KVX_CUDA(cudaLaunchKernelEx(&cfg, kernel, p));
+    count_launch();
+    return KVX_OK;
+}
+
+template <class T, int LANES, int PASSES>
+int launch_rows(const RotateParams &p, const cudaLaunchConfig_t &cfg, int sms) {
+    constexpr int kRows = PASSES * (32 / LANES);
+    const int rows = p.query.heads + p.key.heads + p.value.heads;
+    return launch(p.interleaved ? rotate_store_fast<T, LANES, PASSES, true> : rotate_store_fast<T, LANES, PASSES, false>, p,
+                  cfg, (int64_t)((rows + kRows - 1) / kRows) * p.num_tokens, sms);
+}
+
+template <class T, int LANES>
+int launch_lanes(const RotateParams &p, const cudaLaunchConfig_t &cfg, int sms) {
+    // Four passes of rows a warp keep the most loads in flight; fewer where they leave warps with too little to do:
+    // rows that do not fill them, or too few tokens to give every scheduler a warp.
+    const int rows = p.query.heads + p.key.heads + p.value.heads, at_once = 32 / LANES;
+    auto fits = [&](int passes) {
+        const int units = (rows + passes * at_once - 1) / (passes * at_once);
+        return rows * 10 >= units * passes * at_once * 9 && (int64_t)units * p.num_tokens >= (int64_t)sms * 4;
+    };
+    if (fits(4)) return launch_rows<T, LANES, 4>(p, cfg, sms);
+    if (fits(2)) return launch_rows<T, LANES, 2>(p, cfg, sms);
+    return launch_rows<T, LANES, 1>(p, cfg, sms);
+}
+
+template <class T>
+int launch_fast(const RotateParams &p, const cudaLaunchConfig_t &cfg, int sms) {
+    return p.key.dim == 64    ? launch_lanes<T, 8>(p, cfg, sms)
+           : p.key.dim == 128 ? launch_lanes<T, 16>(p, cfg, sms)
+                              : launch_lanes<T, 32>(p, cfg, sms);
+}
+
+template <class T, int CHUNKS>
+int launch_chunks(const RotateParams &p, const cudaLaunchConfig_t &cfg, int sms) {
+    return launch(p.interleaved ? rotate_latents_fast<T, CHUNKS, true> : rotate_latents_fast<T, CHUNKS, false>, p, cfg,
+                  (int64_t)(1 + (p.query.heads + 15) / 16) * p.num_tokens, sms);
+}
+
+template <class T>
+int launch_latents(const RotateParams &p, const cudaLaunchConfig_t &cfg, int sms, int chunks) {
+    return chunks == 1   ? launch_chunks<T, 1>(p, cfg, sms)
+           : chunks == 2 ? launch_chunks<T, 2>(p, cfg, sms)
+           : chunks == 3 ? launch_chunks<T, 3>(p, cfg, sms)
+                         : launch_chunks<T, 4>(p, cfg, sms);
 }
 
 }  // namespace
@@ -246,12 +558,27 @@ extern "C" int kvx_rotate_store(const kvx_rotate_args *args, const kvx_store_des
     attr.val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = &attr;
     cfg.numAttrs = (flags & KVX_STORE_SERIAL) ? 0 : 1;
-    const int64_t rows = (int64_t)(p.query.heads + p.key.heads + p.value.heads) * p.num_tokens;
-    const int64_t warps = kAnyThreads / 32;
-    cfg.gridDim = dim3((unsigned)std::min<int64_t>((rows + warps - 1) / warps, (int64_t)sms * 8));
-    cfg.blockDim = dim3(kAnyThreads);
-    KVX_CUDA(cudaLaunchKernelEx(&cfg, a.dtype == KVX_BF16 ? rotate_store_any<__nv_bfloat16> : rotate_store_any<__half>,
-                                p));
-    count_launch();
-    return KVX_OK;
+    // The vector forms move 8 bytes at a time; what they do not take goes row by row, element by element.
+    const int heads = p.query.heads + p.key.heads + p.value.heads;
+    align_bits |= p.query.base | p.key.base | p.value.base | (uint64_t)p.query.token_stride |
+                  (uint64_t)p.query.head_stride | (uint64_t)p.key.token_stride | (uint64_t)p.key.head_stride |
+                  (uint64_t)p.value.token_stride | (uint64_t)p.value.head_stride | (uint64_t)(uintptr_t)p.query.weight |
+                  (uint64_t)(uintptr_t)p.key.weight | (has_query ? p.out : 0) |
+                  (has_query ? (uint64_t)p.out_token_stride | (uint64_t)p.out_head_stride : 0);
+    const bool aligned = align_bits % 8 == 0 && (uint64_t)(uintptr_t)p.table % 16 == 0 && p.rotary_dim % 8 == 0 &&
+                         (int64_t)heads * p.num_tokens < (int64_t)1 << 31;
+    const int dim = p.key.dim;
+    const bool plain = p.key.rotary_first == 0 && (p.key.norm_dim == 0 || p.key.norm_dim == dim);
+    const bool queries_plain = !has_query || (p.query.dim == dim && p.query.rotary_first == 0 &&
+                                              (p.query.norm_dim == 0 || p.query.norm_dim == dim));
+    const bool bf16 = a.dtype == KVX_BF16;
+    if (aligned && plain && queries_plain && has_value && (dim == 64 || dim == 128 || dim == 256))
+        return bf16 ? launch_fast<__nv_bfloat16>(p, cfg, sms) : launch_fast<__half>(p, cfg, sms);
+    const int rank = dim - 64;
+    if (aligned && !has_value && p.rotary_dim == 64 && p.key.heads == 1 && p.key.rotary_first == rank &&
+        (p.key.norm_dim == 0 || p.key.norm_dim == rank) && rank >= 256 && rank <= 1024 && rank % 256 == 0 &&
+        (!has_query || (p.query.dim == 64 && p.query.rotary_first == 0 && p.query.norm_dim == 0)))
+        return bf16 ? launch_latents<__nv_bfloat16>(p, cfg, sms, rank / 256) : launch_latents<__half>(p, cfg, sms, rank / 256);
+    return launch(bf16 ? rotate_store_any<__nv_bfloat16> : rotate_store_any<__half>, p, cfg,
+                  (int64_t)heads * p.num_tokens, sms);
 }
