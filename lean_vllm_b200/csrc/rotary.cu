@@ -176,18 +176,30 @@ __global__ void __launch_bounds__(kAnyThreads) rotate_store_any(const __grid_con
 
 constexpr int kFastThreads = 256;
 
+__device__ __forceinline__ float2 unpack(uint32_t bits, __nv_bfloat16) {
+    return make_float2(__uint_as_float(bits << 16), __uint_as_float(bits & 0xffff0000u));
+}
+__device__ __forceinline__ float2 unpack(uint32_t bits, __half) {
+    return __half22float2(*reinterpret_cast<const __half2 *>(&bits));
+}
+__device__ __forceinline__ uint32_t pack(float x, float y, __nv_bfloat16) {
+    const __nv_bfloat162 v = __floats2bfloat162_rn(x, y);
+    return *reinterpret_cast<const uint32_t *>(&v);
+}
+__device__ __forceinline__ uint32_t pack(float x, float y, __half) {
+    const __half2 v = __floats2half2_rn(x, y);
+    return *reinterpret_cast<const uint32_t *>(&v);
+}
+
 template <class T>
 struct Piece {  // four elements
     uint2 bits;
     __device__ __forceinline__ void get(float (&x)[4]) const {
-        const T *e = reinterpret_cast<const T *>(&bits);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) x[i] = to_float(e[i]);
+        const float2 lo = unpack(bits.x, T()), hi = unpack(bits.y, T());
+        x[0] = lo.x, x[1] = lo.y, x[2] = hi.x, x[3] = hi.y;
     }
     __device__ __forceinline__ void set(const float (&x)[4]) {
-        T *e = reinterpret_cast<T *>(&bits);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) e[i] = from_float<T>(x[i]);
+        bits = make_uint2(pack(x[0], x[1], T()), pack(x[2], x[3], T()));
     }
 };
 
@@ -231,66 +243,58 @@ __device__ __forceinline__ void rotate(float (&a)[4], float (&b)[4], const float
     }
 }
 
-// Writes a key or value row's pieces to every destination that takes its head. `at0`: the token's place in destination 0.
-template <class T>
-__device__ __forceinline__ void store_everywhere(const RotateParams &p, int64_t token, int64_t slot, int64_t at0, int head,
-                                                 bool value, int a, int b, const Piece<T> &x, const Piece<T> &y) {
-    for (int d = p.peers_only; d < p.n_dests; ++d) {
-        const StoreDest &dst = p.dests[d];
-        if (head < dst.src_first_head || head >= dst.src_first_head + dst.num_heads) continue;
-        const int64_t at = d == 0 ? at0 : dest_offset(p, d, token, slot);
-        if (at < 0) continue;
-        const uint64_t row = (value ? dst.v : dst.k) + at +
-                             (int64_t)(head - dst.src_first_head + dst.dst_first_head) * dst.head_stride;
-        store_piece<T>(row + a * sizeof(T), x);
-        store_piece<T>(row + b * sizeof(T), y);
-    }
+// Where destination 0 keeps a token, or -1.
+__device__ __forceinline__ int64_t first_offset(const RotateParams &p, int64_t token, int64_t slot) {
+    return p.peers_only ? -1 : dest_offset(p, 0, token, slot);
 }
 
-// PASSES x (32 / LANES) rows of one token from `row0` on, of `rows` there are: queries, then keys, then values.
+// PASSES x (32 / LANES) rows of one token and one kind (0 queries, 1 keys, 2 values) from head `head0` on.
 template <class T, int LANES, int PASSES, bool INTERLEAVED>
-__device__ __forceinline__ void rotate_rows(const RotateParams &p, int64_t token, int row0, int rows, int64_t slot,
-                                            int64_t at0, const float *angle, const Piece<T> (&q_weight)[2],
-                                            const Piece<T> (&k_weight)[2], const Place &place) {
+__device__ __forceinline__ void rotate_rows(const RotateParams &p, const Rows &rows, int kind, int64_t token, int head0,
+                                            const Place &place) {
+    constexpr int kAtOnce = 32 / LANES;
     const int lane = threadIdx.x & 31, lane_in_row = lane % LANES;
+    const int first = head0 + lane / LANES;
+    const uint64_t in = rows.base + token * rows.token_stride + first * rows.head_stride;
     Piece<T> x[PASSES], y[PASSES];
-    int kind[PASSES], head[PASSES];
 #pragma unroll
     for (int i = 0; i < PASSES; ++i) {
-        const int r = row0 + i * (32 / LANES) + lane / LANES;
-        kind[i] = r < p.query.heads ? 0 : r < p.query.heads + p.key.heads ? 1 : 2;
-        head[i] = r - (kind[i] == 0 ? 0 : kind[i] == 1 ? p.query.heads : p.query.heads + p.key.heads);
-        if (r >= rows) kind[i] = 3;
-        const Rows &in = kind[i] == 0 ? p.query : kind[i] == 1 ? p.key : p.value;
-        const uint64_t at = in.base + token * in.token_stride + head[i] * in.head_stride;
         x[i].bits = y[i].bits = make_uint2(0, 0);
-        if (kind[i] < 3) {
+        if (first + i * kAtOnce < rows.heads) {
+            const uint64_t at = in + i * kAtOnce * rows.head_stride;
             x[i] = load_piece<T>(at + place.a * sizeof(T));
             y[i] = load_piece<T>(at + place.b * sizeof(T));
         }
     }
-    float4 cos4 = make_float4(1.f, 1.f, 1.f, 1.f), sin4 = make_float4(0.f, 0.f, 0.f, 0.f);
-    if (place.rotated) {
-        cos4 = __ldg(reinterpret_cast<const float4 *>(angle) + lane_in_row);
-        sin4 = __ldg(reinterpret_cast<const float4 *>(angle + p.rotary_dim / 2) + lane_in_row);
-    }
+    const int64_t slot = load_index(p.dests[0].slots, p.dests[0].slot_bytes, token);
+    if (kind < 2) {
+        float4 cos4, sin4;
+        Piece<T> weight[2];
+        if (place.rotated) {
+            const float *angle = angles(p, token, slot < 0);
+            cos4 = __ldg(reinterpret_cast<const float4 *>(angle) + lane_in_row);
+            sin4 = __ldg(reinterpret_cast<const float4 *>(angle + p.rotary_dim / 2) + lane_in_row);
+        }
+        const bool normed = rows.norm_dim > 0;
+        if (normed) {
+            weight[0] = load_piece<T>((uint64_t)rows.weight + place.a * sizeof(T));
+            weight[1] = load_piece<T>((uint64_t)rows.weight + place.b * sizeof(T));
+        }
 #pragma unroll
-    for (int i = 0; i < PASSES; ++i) {
-        float a[4], b[4];
-        x[i].get(a);
-        y[i].get(b);
-        const bool normed = (kind[i] == 0 && p.query.norm_dim > 0) || (kind[i] == 1 && p.key.norm_dim > 0);
-        float sum = 0.f;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) sum += a[e] * a[e] + b[e] * b[e];
-#pragma unroll
-        for (int o = LANES / 2; o; o >>= 1) sum += __shfl_xor_sync(~0u, sum, o);
-        if (kind[i] < 2) {
+        for (int i = 0; i < PASSES; ++i) {
+            float a[4], b[4];
+            x[i].get(a);
+            y[i].get(b);
             if (normed) {
+                float sum = 0.f;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) sum += a[e] * a[e] + b[e] * b[e];
+#pragma unroll
+                for (int o = LANES / 2; o; o >>= 1) sum += __shfl_xor_sync(~0u, sum, o);
                 const float scale = rsqrtf(sum * (1.f / (LANES * 8)) + p.eps);
                 float w[4], v[4];
-                (kind[i] == 0 ? q_weight[0] : k_weight[0]).get(w);
-                (kind[i] == 0 ? q_weight[1] : k_weight[1]).get(v);
+                weight[0].get(w);
+                weight[1].get(v);
 #pragma unroll
                 for (int e = 0; e < 4; ++e) a[e] = a[e] * scale * w[e], b[e] = b[e] * scale * v[e];
             }
@@ -298,45 +302,44 @@ __device__ __forceinline__ void rotate_rows(const RotateParams &p, int64_t token
             x[i].set(a);
             y[i].set(b);
         }
-        if (kind[i] == 0) {
-            const uint64_t out = p.out + token * p.out_token_stride + head[i] * p.out_head_stride;
-            store_piece<T>(out + place.a * sizeof(T), x[i]);
-            store_piece<T>(out + place.b * sizeof(T), y[i]);
-        } else if (kind[i] < 3) {
-            store_everywhere<T>(p, token, slot, at0, head[i], kind[i] == 2, place.a, place.b, x[i], y[i]);
-        }
     }
-}
-
-// Where destination 0 keeps a token, or -1.
-__device__ __forceinline__ int64_t first_offset(const RotateParams &p, int64_t token, int64_t slot) {
-    return p.peers_only ? -1 : dest_offset(p, 0, token, slot);
+    auto store = [&](uint64_t to, int64_t head_stride, int from_head, int heads) {  // `to`: head 0's row
+#pragma unroll
+        for (int i = 0; i < PASSES; ++i) {
+            const int head = first + i * kAtOnce;
+            if (head < from_head || head >= heads) continue;
+            const uint64_t at = to + head * head_stride;
+            store_piece<T>(at + place.a * sizeof(T), x[i]);
+            store_piece<T>(at + place.b * sizeof(T), y[i]);
+        }
+    };
+    if (kind == 0) {
+        store(p.out + token * p.out_token_stride, p.out_head_stride, 0, rows.heads);
+        return;
+    }
+    for (int d = p.peers_only; d < p.n_dests; ++d) {
+        const StoreDest &dst = p.dests[d];
+        const int64_t at = dest_offset(p, d, token, slot);
+        if (at < 0) continue;
+        store((kind == 1 ? dst.k : dst.v) + at + (int64_t)(dst.dst_first_head - dst.src_first_head) * dst.head_stride,
+              dst.head_stride, dst.src_first_head, min(rows.heads, dst.src_first_head + dst.num_heads));
+    }
 }
 
 template <class T, int LANES, int PASSES, bool INTERLEAVED>
-__global__ void __launch_bounds__(kFastThreads) rotate_store_fast(const __grid_constant__ RotateParams p) {
+__global__ void __launch_bounds__(kFastThreads, 4) rotate_store_fast(const __grid_constant__ RotateParams p) {
     launch_dependents();
-    const int lane = threadIdx.x & 31;
-    const Place place = place_of<INTERLEAVED>(lane % LANES, p.rotary_dim);
-    const int rows = p.query.heads + p.key.heads + p.value.heads;
+    const Place place = place_of<INTERLEAVED>((threadIdx.x & 31) % LANES, p.rotary_dim);
     constexpr int kRows = PASSES * (32 / LANES);
-    const uint32_t per_token = (rows + kRows - 1) / kRows, n = per_token * (uint32_t)p.num_tokens;
+    const uint32_t q_units = (p.query.heads + kRows - 1) / kRows, kv_units = (p.key.heads + kRows - 1) / kRows;
+    const uint32_t per_token = q_units + 2 * kv_units, n = per_token * (uint32_t)p.num_tokens;
     wait_prerequisites();
-    Piece<T> q_weight[2], k_weight[2];
-    if (p.query.norm_dim > 0) {
-        q_weight[0] = load_piece<T>((uint64_t)p.query.weight + place.a * sizeof(T));
-        q_weight[1] = load_piece<T>((uint64_t)p.query.weight + place.b * sizeof(T));
-    }
-    if (p.key.norm_dim > 0) {
-        k_weight[0] = load_piece<T>((uint64_t)p.key.weight + place.a * sizeof(T));
-        k_weight[1] = load_piece<T>((uint64_t)p.key.weight + place.b * sizeof(T));
-    }
     for (uint32_t w = blockIdx.x * (kFastThreads / 32) + threadIdx.x / 32; w < n; w += gridDim.x * (kFastThreads / 32)) {
-        const uint32_t token = w / per_token, row0 = (w - token * per_token) * kRows;
-        const int64_t slot = load_index(p.dests[0].slots, p.dests[0].slot_bytes, token);
-        const float *angle = p.rotary_dim ? angles(p, token, slot < 0) : nullptr;
-        const int64_t at0 = (int)row0 + kRows > p.query.heads ? first_offset(p, token, slot) : -1;
-        rotate_rows<T, LANES, PASSES, INTERLEAVED>(p, token, row0, rows, slot, at0, angle, q_weight, k_weight, place);
+        const uint32_t token = w / per_token, unit = w - token * per_token;
+        const int kind = unit < q_units ? 0 : unit < q_units + kv_units ? 1 : 2;  // the same for a warp
+        const Rows &rows = kind == 0 ? p.query : kind == 1 ? p.key : p.value;
+        const int head0 = (unit - (kind == 0 ? 0 : kind == 1 ? q_units : q_units + kv_units)) * kRows;
+        rotate_rows<T, LANES, PASSES, INTERLEAVED>(p, rows, kind, token, head0, place);
     }
 }
 
@@ -352,14 +355,12 @@ __global__ void __launch_bounds__(kFastThreads) rotate_latents_fast(const __grid
     wait_prerequisites();
     for (uint32_t w = blockIdx.x * (kFastThreads / 32) + threadIdx.x / 32; w < n; w += gridDim.x * (kFastThreads / 32)) {
         const uint32_t token = w / per_token, item = w - token * per_token;
-        const int64_t slot = load_index(p.dests[0].slots, p.dests[0].slot_bytes, token);
-        const float *angle = angles(p, token, slot < 0);
         if (item > 0) {
-            const Piece<T> none[2] = {};
-            rotate_rows<T, kLanes, kPasses, INTERLEAVED>(p, token, (item - 1) * kRows, p.query.heads, slot, -1, angle, none,
-                                                         none, place);
+            rotate_rows<T, kLanes, kPasses, INTERLEAVED>(p, p.query, 0, token, (item - 1) * kRows, place);
             continue;
         }
+        const int64_t slot = load_index(p.dests[0].slots, p.dests[0].slot_bytes, token);
+        const float *angle = angles(p, token, slot < 0);
         const uint64_t row = p.key.base + (int64_t)token * p.key.token_stride;
         Piece<T> c[CHUNKS][2], x, y;
 #pragma unroll
@@ -452,22 +453,25 @@ int launch(void (*kernel)(RotateParams), const RotateParams &p, cudaLaunchConfig
     return KVX_OK;
 }
 
+// Warps a token's rows take at `at_once` rows a unit.
+int units_of(const RotateParams &p, int at_once) {
+    return (p.query.heads + at_once - 1) / at_once + 2 * ((p.key.heads + at_once - 1) / at_once);
+}
+
 template <class T, int LANES, int PASSES>
 int launch_rows(const RotateParams &p, const cudaLaunchConfig_t &cfg, int sms) {
-    constexpr int kRows = PASSES * (32 / LANES);
-    const int rows = p.query.heads + p.key.heads + p.value.heads;
     return launch(p.interleaved ? rotate_store_fast<T, LANES, PASSES, true> : rotate_store_fast<T, LANES, PASSES, false>, p,
-                  cfg, (int64_t)((rows + kRows - 1) / kRows) * p.num_tokens, sms);
+                  cfg, (int64_t)units_of(p, PASSES * (32 / LANES)) * p.num_tokens, sms);
 }
 
 template <class T, int LANES>
 int launch_lanes(const RotateParams &p, const cudaLaunchConfig_t &cfg, int sms) {
     // Four passes of rows a warp keep the most loads in flight; fewer where they leave warps with too little to do:
-    // rows that do not fill them, or too few tokens to give every scheduler a warp.
+    // heads that do not fill them, or too few tokens to give every scheduler a warp.
     const int rows = p.query.heads + p.key.heads + p.value.heads, at_once = 32 / LANES;
     auto fits = [&](int passes) {
-        const int units = (rows + passes * at_once - 1) / (passes * at_once);
-        return rows * 10 >= units * passes * at_once * 9 && (int64_t)units * p.num_tokens >= (int64_t)sms * 4;
+        const int units = units_of(p, passes * at_once);
+        return rows * 4 >= units * passes * at_once * 3 && (int64_t)units * p.num_tokens >= (int64_t)sms * 4;
     };
     if (fits(4)) return launch_rows<T, LANES, 4>(p, cfg, sms);
     if (fits(2)) return launch_rows<T, LANES, 2>(p, cfg, sms);
