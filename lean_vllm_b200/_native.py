@@ -8,6 +8,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+import struct
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(HERE, "libkvx.so")
@@ -203,6 +204,14 @@ class AttentionArgs(ctypes.Structure):
     ]
 
 
+# The same structs as one pack() each: a call that a decode step makes per layer spends a third of the time that filling
+# a ctypes struct field by field takes.
+STORE_DEST = struct.Struct("<QQqqqiiQiiiiQii")
+ROTATE_ROWS = struct.Struct("<QqqiiiiQ")
+ROTATE_ARGS = struct.Struct("<" + 3 * "QqqiiiiQ" + "QqqQQiiiiiifi")
+ATTENTION_ARGS = struct.Struct("<QqqQqqQQqqqQqQQQQQQQ14i2f")
+
+
 # Every symbol include/kvx.h declares, with its argtypes and restype.
 _P = ctypes.c_void_p
 SIGNATURES: dict[str, tuple[list, object]] = {
@@ -221,10 +230,10 @@ SIGNATURES: dict[str, tuple[list, object]] = {
                      ctypes.c_int, ctypes.c_int, ctypes.c_int, ctypes.c_int, _P], ctypes.c_int),
     "kvx_store": ([_P, _P, ctypes.c_int64, ctypes.c_int64, ctypes.c_int, ctypes.c_int, ctypes.c_int,
                    ctypes.POINTER(StoreDest), ctypes.c_int, _P, ctypes.c_int, _P], ctypes.c_int),
-    "kvx_rotate_store": ([ctypes.POINTER(RotateArgs), ctypes.POINTER(StoreDest), ctypes.c_int, _P, ctypes.c_int, _P],
-                         ctypes.c_int),
+    # Their structs go as packed bytes (ROTATE_ARGS, STORE_DEST, ATTENTION_ARGS) or as the ctypes structs' addresses.
+    "kvx_rotate_store": ([_P, _P, ctypes.c_int, _P, ctypes.c_int, _P], ctypes.c_int),
     "kvx_attention_workspace_bytes": ([], ctypes.c_uint64),
-    "kvx_attention": ([ctypes.POINTER(AttentionArgs), ctypes.c_int, _P], ctypes.c_int),
+    "kvx_attention": ([_P, ctypes.c_int, _P], ctypes.c_int),
     "kvx_transfer": ([ctypes.POINTER(Cache), ctypes.c_int, ctypes.POINTER(Job), ctypes.c_int, ctypes.c_int, _P, _P,
                       ctypes.POINTER(ctypes.c_void_p)], ctypes.c_int),
     "kvx_transfer_after": ([ctypes.POINTER(Cache), ctypes.c_int, ctypes.POINTER(Job), ctypes.c_int, ctypes.c_int, _P,

@@ -8,13 +8,13 @@ it. There is no fallback: without libkvx.so the calls raise.
 
 from __future__ import annotations
 
-import math
-
 import torch
 
 from lean_vllm_b200 import _native
-from lean_vllm_b200._native import AttentionArgs, check, lib
+from lean_vllm_b200._native import lib
+from lean_vllm_b200.attention.device import call, raw_stream
 
+_INT32_MAX = 2**31 - 1
 _DTYPES = {torch.bfloat16: _native.BF16, torch.float16: _native.FP16}
 
 
@@ -32,75 +32,80 @@ class AttentionWorkspace:
             self.tensor[: _native.ATTENTION_ZEROED].zero_()
         self.address = self.tensor.data_ptr()
         self.device = self.tensor.device
+        self.index = self.tensor.get_device()
 
 
-def _int32(name: str, t: torch.Tensor, shape: tuple, device) -> None:
-    if t.dtype != torch.int32 or t.device != device or tuple(t.shape) != shape or not t.is_contiguous():
+def _int32(name: str, t: torch.Tensor, shape: tuple, device: int) -> int:
+    if t.dtype != torch.int32 or t.get_device() != device or t.shape != shape or not t.is_contiguous():
         raise ValueError(f"{name} must be a contiguous int32 tensor {shape} on the queries' device, not "
                          f"{t.dtype} {tuple(t.shape)} on {t.device}")
+    return t.data_ptr()
 
 
 def _attention(query, k_cache, v_cache, block_tables, kv_lens, scale, q_starts, max_q_len, max_kv_len, softcap, window,
                slopes, prefix_lens, shared_table, shared_len, out, workspace, stream, flags, status):
-    if query.dim() != 3 or k_cache.dim() != 4 or k_cache.shape != v_cache.shape:
+    shape, cache_shape = query.shape, k_cache.shape
+    if len(shape) != 3 or len(cache_shape) != 4 or cache_shape != v_cache.shape:
         raise ValueError(f"queries {tuple(query.shape)} [num_tokens, heads, dim] over caches {tuple(k_cache.shape)} / "
                          f"{tuple(v_cache.shape)} [num_blocks, block_size, heads, dim]")
-    num_tokens, q_heads, head_dim = query.shape
-    num_blocks, block_size, kv_heads, cache_dim = k_cache.shape
+    num_tokens, q_heads, head_dim = shape
+    num_blocks, block_size, kv_heads, cache_dim = cache_shape
     if cache_dim != head_dim or kv_heads < 1 or q_heads % kv_heads:
         raise ValueError(f"{q_heads} query heads of {head_dim} over {kv_heads} KV heads of {cache_dim}")
-    dtype, device = query.dtype, query.device
+    dtype, device = query.dtype, query.get_device()
     if dtype not in _DTYPES or not dtype == k_cache.dtype == v_cache.dtype:
         raise TypeError(f"queries and caches must share a dtype, bfloat16 or float16: {dtype}, {k_cache.dtype}, "
                         f"{v_cache.dtype}")
-    if not device == k_cache.device == v_cache.device:
+    if not device == k_cache.get_device() == v_cache.get_device():
         raise ValueError("queries and caches must be on one device")
-    strides = k_cache.stride()
-    if strides != v_cache.stride() or strides[3] != 1 or query.stride(2) != 1:
+    (q0, q1, q2), strides = query.stride(), k_cache.stride()
+    if strides != v_cache.stride() or strides[3] != 1 or q2 != 1:
         raise ValueError("key and value caches must share strides; a head's elements must be contiguous")
-    if block_tables.dim() != 2 or block_tables.dtype != torch.int32 or block_tables.device != device:
+    if block_tables.dim() != 2 or block_tables.dtype != torch.int32 or block_tables.get_device() != device:
         raise ValueError("block tables are an int32 tensor [batch, blocks] on the queries' device")
     batch, max_blocks = block_tables.shape
-    if max_blocks > 1 and block_tables.stride(1) != 1:
+    table_stride, unit = block_tables.stride()
+    if max_blocks > 1 and unit != 1:
         raise ValueError("a sequence's block ids must be contiguous")
-    _int32("kv_lens", kv_lens, (batch,), device)
+    lens = _int32("kv_lens", kv_lens, (batch,), device)
+    starts = prefixes = biases = shared = shared_blocks = 0
     if q_starts is not None:
-        _int32("q_starts", q_starts, (batch + 1,), device)
+        starts = _int32("q_starts", q_starts, (batch + 1,), device)
     elif num_tokens != batch:
         raise ValueError(f"{num_tokens} query tokens of {batch} sequences: more than one each needs q_starts")
     if prefix_lens is not None:
-        _int32("prefix_lens", prefix_lens, (batch,), device)
-    if slopes is not None and (slopes.dtype != torch.float32 or slopes.device != device or not slopes.is_contiguous()
-                               or slopes.shape != (q_heads,)):
-        raise ValueError(f"slopes are {q_heads} contiguous float32 on the queries' device")
-    shared_blocks = 0
+        prefixes = _int32("prefix_lens", prefix_lens, (batch,), device)
+    if slopes is not None:
+        if (slopes.dtype != torch.float32 or slopes.get_device() != device or not slopes.is_contiguous()
+                or slopes.shape != (q_heads,)):
+            raise ValueError(f"slopes are {q_heads} contiguous float32 on the queries' device")
+        biases = slopes.data_ptr()
     if shared_table is not None:
         shared_blocks = shared_table.numel()
-        _int32("prefix_table", shared_table, (shared_blocks,), device)
+        shared = _int32("prefix_table", shared_table, (shared_blocks,), device)
     if out is None:
-        out = torch.empty((num_tokens, q_heads, head_dim), dtype=dtype, device=device)
-        if stream is not None:
-            out.record_stream(torch.cuda.ExternalStream(stream, device))
-    elif out.shape != query.shape or out.dtype != dtype or out.device != device or out.stride(2) != 1:
-        raise ValueError("`out` must have the queries' shape, dtype and device, a head's elements contiguous")
+        out = torch.empty_like(query, memory_format=torch.contiguous_format)  # half the cost of torch.empty
+        o0, o1 = q_heads * head_dim, head_dim
+        if stream is not None:  # the caching allocator has to know who writes it
+            out.record_stream(torch.cuda.ExternalStream(stream, query.device))
+    else:
+        o0, o1, o2 = out.stride() if out.dim() == 3 else (0, 0, 0)
+        if out.shape != shape or out.dtype != dtype or out.get_device() != device or o2 != 1:
+            raise ValueError("`out` must have the queries' shape, dtype and device, a head's elements contiguous")
     if workspace is None:
-        workspace = AttentionWorkspace(device, stream)
+        workspace = AttentionWorkspace(query.device, stream)
         if stream is not None:
-            workspace.tensor.record_stream(torch.cuda.ExternalStream(stream, device))
-    elif workspace.device != device:
+            workspace.tensor.record_stream(torch.cuda.ExternalStream(stream, query.device))
+    elif workspace.index != device:
         raise ValueError("the workspace must be on the queries' device")
-    q_strides, o_strides = query.stride(), out.stride()
-    args = AttentionArgs(
-        query.data_ptr(), q_strides[0] * 2, q_strides[1] * 2, out.data_ptr(), o_strides[0] * 2, o_strides[1] * 2,
-        k_cache.data_ptr(), v_cache.data_ptr(), strides[0] * 2, strides[1] * 2, strides[2] * 2,
-        block_tables.data_ptr(), block_tables.stride(0), kv_lens.data_ptr(),
-        q_starts.data_ptr() if q_starts is not None else None, slopes.data_ptr() if slopes is not None else None,
-        prefix_lens.data_ptr() if prefix_lens is not None else None,
-        shared_table.data_ptr() if shared_table is not None else None, workspace.address, status or None, shared_len,
-        shared_blocks, block_size, num_blocks, max_blocks, batch, num_tokens, q_heads, kv_heads, head_dim,
-        _DTYPES[dtype], max_q_len, max_blocks * block_size if max_kv_len is None else max_kv_len, window,
-        1.0 / math.sqrt(head_dim) if scale is None else scale, softcap)
-    check(lib().kvx_attention(args, flags, stream if stream is not None else torch.cuda.current_stream(device).cuda_stream))
+    args = _native.ATTENTION_ARGS.pack(
+        query.data_ptr(), 2 * q0, 2 * q1, out.data_ptr(), 2 * o0, 2 * o1, k_cache.data_ptr(), v_cache.data_ptr(),
+        2 * strides[0], 2 * strides[1], 2 * strides[2], block_tables.data_ptr(), table_stride, lens, starts, biases,
+        prefixes, shared, workspace.address, status, shared_len, shared_blocks, block_size, num_blocks, max_blocks, batch,
+        num_tokens, q_heads, kv_heads, head_dim, _DTYPES[dtype], min(max_q_len, _INT32_MAX),
+        min(max_blocks * block_size if max_kv_len is None else max_kv_len, _INT32_MAX), window,
+        head_dim**-0.5 if scale is None else scale, softcap)
+    call(device, lib().kvx_attention, args, flags, raw_stream(device) if stream is None else stream)
     return out
 
 

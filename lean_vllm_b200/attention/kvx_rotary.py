@@ -16,10 +16,12 @@ from dataclasses import dataclass
 import torch
 
 from lean_vllm_b200 import _native
-from lean_vllm_b200._native import RotateArgs, RotateRows, StoreDest, check, lib
+from lean_vllm_b200._native import lib
+from lean_vllm_b200.attention.device import call, raw_stream
 from lean_vllm_b200.attention.kvx_cache import PushTarget, _dest, _slots, _target_slots
 
 _DTYPES = {torch.bfloat16: _native.BF16, torch.float16: _native.FP16}
+_INDEX_BYTES = {torch.int32: 4, torch.int64: 8}
 
 
 @dataclass
@@ -82,52 +84,68 @@ class RotaryTable:
         return cls(table.float().to(device), interleaved)
 
 
-def _positions(positions: torch.Tensor, num_tokens: int, device) -> torch.Tensor:
+def _positions(positions: torch.Tensor, num_tokens: int, device: int) -> int:
+    """The positions' element size, after checking them."""
     if positions.numel() != num_tokens:
         raise ValueError(f"{positions.numel()} positions for {num_tokens} rows")
-    if positions.dtype not in (torch.int32, torch.int64):
+    size = _INDEX_BYTES.get(positions.dtype)
+    if size is None:
         raise TypeError(f"positions are int32 or int64, not {positions.dtype}")
-    if positions.device != device or not positions.is_contiguous():
+    if positions.get_device() != device or not positions.is_contiguous():
         raise ValueError("positions must be contiguous on the storing device")
-    return positions
+    return size
 
 
-def _rows(x: torch.Tensor, weight, norm_dim: int, rotary_first: int) -> RotateRows:
+def _weight(weight: torch.Tensor | None, dim: int, dtype, device: int) -> tuple[int, int]:
+    """(normed elements, address) of a norm's weight."""
     if weight is None:
-        norm_dim = 0
-    elif weight.dtype != x.dtype or weight.numel() != norm_dim or weight.device != x.device or not weight.is_contiguous():
-        raise ValueError(f"a norm's weight is {norm_dim} contiguous elements of the rows' dtype on their device")
-    if x.stride(-1) != 1:
-        raise ValueError("a head's elements must be contiguous")
-    size = x.element_size()
-    head_stride, heads = (x.stride(1) * size, x.size(1)) if x.dim() == 3 else (0, 1)
-    return RotateRows(x.data_ptr(), x.stride(0) * size, head_stride, heads, x.size(-1), norm_dim, rotary_first,
-                      weight.data_ptr() if norm_dim else None)
+        return 0, 0
+    if weight.dtype != dtype or weight.numel() != dim or weight.get_device() != device or not weight.is_contiguous():
+        raise ValueError(f"a norm's weight is {dim} contiguous elements of the rows' dtype on their device")
+    return dim, weight.data_ptr()
 
 
-def _launch(rows, out, rotary, positions, num_tokens, dtype, eps, dests, stream, flags, status, device):
-    query, key, value = rows
+_NO_ROWS = (0, 0, 0, 0, 0, 0, 0, 0)
+
+
+def _dests(k_addr: int, v_addr: int, strides: tuple, block_size: int, num_blocks: int, slots: torch.Tensor, heads: int,
+           push_to, num_tokens: int, device) -> bytes:
+    packed = _native.STORE_DEST.pack(k_addr, v_addr, *strides, block_size, num_blocks, slots.data_ptr(),
+                                     _INDEX_BYTES[slots.dtype], 0, heads, 0, 0, 0, 0)
+    for target in push_to:
+        t_slots = _target_slots(target, num_tokens, device)
+        count = heads - target.src_first_head if target.num_heads is None else target.num_heads
+        dest = _dest(target.k_cache, target.v_cache if v_addr else 0, target.block_stride, target.token_stride,
+                     target.head_stride if v_addr else 0, target.block_size, target.num_blocks, t_slots,
+                     target.src_first_head if v_addr else 0, count if v_addr else 1,
+                     target.dst_first_head if v_addr else 0, target.block_map)
+        packed += bytes(dest)
+    return packed
+
+
+def _launch(rows: tuple, out, rotary: RotaryTable, positions: torch.Tensor, position_bytes: int, num_tokens: int, dtype,
+            eps: float, dests: bytes, stream, flags: int, status: int, device: int) -> None:
     table = rotary.table
-    if table.device != device:
+    if table.get_device() != device:
         raise ValueError("the rotary table must be on the storing device")
-    size = 2
-    args = RotateArgs(query, key, value, out.data_ptr() if out is not None else None,
-                      out.stride(0) * size if out is not None else 0, out.stride(1) * size if out is not None else 0,
-                      table.data_ptr(), positions.data_ptr(), table.size(0), table.size(1), int(rotary.interleaved),
-                      positions.element_size(), num_tokens, dtype, eps, 0)
-    array = (StoreDest * len(dests))(*dests)
-    s = stream if stream is not None else torch.cuda.current_stream(device).cuda_stream
-    check(lib().kvx_rotate_store(args, array, len(dests), status or None, flags, s))
+    if out is not None:
+        o0, o1, _ = out.stride()
+        to = (out.data_ptr(), 2 * o0, 2 * o1)
+    else:
+        to = (0, 0, 0)
+    table_rows, rotary_dim = table.shape
+    args = _native.ROTATE_ARGS.pack(*rows, *to, table.data_ptr(), positions.data_ptr(), table_rows, rotary_dim,
+                                    rotary.interleaved, position_bytes, num_tokens, _DTYPES[dtype], eps, 0)
+    s = raw_stream(device) if stream is None else stream
+    call(device, lib().kvx_rotate_store, args, dests, len(dests) // _native.STORE_DEST.size, status or None, flags, s)
 
 
-def _output(query, out, stream):
+def _output(query: torch.Tensor, out: torch.Tensor | None, stream: int | None) -> torch.Tensor:
     if out is None:
+        out = torch.empty_like(query, memory_format=torch.contiguous_format)  # half the cost of torch.empty
         if stream is not None and query.is_cuda:  # the caching allocator has to know who writes it
-            out = torch.empty(query.shape, dtype=query.dtype, device=query.device)
             out.record_stream(torch.cuda.ExternalStream(stream, query.device))
-            return out
-        return torch.empty(query.shape, dtype=query.dtype, device=query.device)
-    if out.shape != query.shape or out.dtype != query.dtype or out.device != query.device or out.stride(-1) != 1:
+    elif out.shape != query.shape or out.dtype != query.dtype or out.device != query.device or out.stride(-1) != 1:
         raise ValueError("`out` must have the queries' shape, dtype and device, a head's elements contiguous")
     return out
 
@@ -145,21 +163,24 @@ def rotate_store_kvcache(query: torch.Tensor, key: torch.Tensor, value: torch.Te
     if query.dim() != 3 or key.dim() != 3:
         raise ValueError("queries, keys and values are [num_tokens, heads, dim]")
     num_tokens, num_heads, head_dim = key.shape
-    if value.shape != key.shape or k_cache.dim() != 4 or k_cache.shape != v_cache.shape:
+    cache_shape, dtype, device = k_cache.shape, query.dtype, query.get_device()
+    if value.shape != key.shape or len(cache_shape) != 4 or cache_shape != v_cache.shape:
         raise ValueError(f"keys {tuple(key.shape)} and values {tuple(value.shape)} into caches "
                          f"{tuple(k_cache.shape)} / {tuple(v_cache.shape)}: shapes must match")
-    if k_cache.size(2) != num_heads or k_cache.size(3) != head_dim:
-        raise ValueError(f"{num_heads} heads of {head_dim} into a cache of {k_cache.size(2)} heads of "
-                         f"{k_cache.size(3)}")
-    if query.size(0) != num_tokens or query.size(2) != head_dim:
+    num_blocks, block_size, cache_heads, cache_dim = cache_shape
+    if cache_heads != num_heads or cache_dim != head_dim:
+        raise ValueError(f"{num_heads} heads of {head_dim} into a cache of {cache_heads} heads of {cache_dim}")
+    q_tokens, q_heads, q_dim = query.shape
+    if q_tokens != num_tokens or q_dim != head_dim:
         raise ValueError(f"queries {tuple(query.shape)} beside keys {tuple(key.shape)}")
-    dtype = query.dtype
     if dtype not in _DTYPES or not dtype == key.dtype == value.dtype == k_cache.dtype == v_cache.dtype:
         raise TypeError(f"queries, keys, values and caches must share a dtype, bfloat16 or float16: {dtype}, "
                         f"{key.dtype}, {value.dtype}, {k_cache.dtype}, {v_cache.dtype}")
-    device = query.device
-    if not device == key.device == value.device == k_cache.device == v_cache.device:
+    if not device == key.get_device() == value.get_device() == k_cache.get_device() == v_cache.get_device():
         raise ValueError("queries, keys, values and the local caches must be on one device")
+    (q0, q1, q2), (k0, k1, k2), (v0, v1, v2) = query.stride(), key.stride(), value.stride()
+    if q2 != 1 or k2 != 1 or v2 != 1:
+        raise ValueError("a head's elements must be contiguous")
     strides = k_cache.stride()
     if strides != v_cache.stride() or strides[3] != 1:
         raise ValueError("key and value caches must share strides with contiguous head_dim")
@@ -167,19 +188,17 @@ def rotate_store_kvcache(query: torch.Tensor, key: torch.Tensor, value: torch.Te
         raise ValueError(f"a rotary table of {rotary.table.size(1)} elements for heads of {head_dim}")
     if len(push_to) > 8:
         raise ValueError("at most 8 peers per store")
-    slots = _slots(slot_mapping, num_tokens, device)
-    _positions(positions, num_tokens, device)
-    rows = (_rows(query, q_weight, head_dim, 0), _rows(key, k_weight, head_dim, 0), _rows(value, None, 0, 0))
-    dests = [_dest(k_cache.data_ptr(), v_cache.data_ptr(), strides[0] * 2, strides[1] * 2, strides[2] * 2,
-                   k_cache.size(1), k_cache.size(0), slots, 0, num_heads, 0)]
-    for target in push_to:
-        t_slots = _target_slots(target, num_tokens, device)
-        count = num_heads - target.src_first_head if target.num_heads is None else target.num_heads
-        dests.append(_dest(target.k_cache, target.v_cache, target.block_stride, target.token_stride,
-                           target.head_stride, target.block_size, target.num_blocks, t_slots, target.src_first_head,
-                           count, target.dst_first_head, target.block_map))
+    slots = _slots(slot_mapping, num_tokens, key.device)
+    position_bytes = _positions(positions, num_tokens, device)
+    q_norm, q_scale = _weight(q_weight, head_dim, dtype, device)
+    k_norm, k_scale = _weight(k_weight, head_dim, dtype, device)
+    rows = (query.data_ptr(), 2 * q0, 2 * q1, q_heads, head_dim, q_norm, 0, q_scale,
+            key.data_ptr(), 2 * k0, 2 * k1, num_heads, head_dim, k_norm, 0, k_scale,
+            value.data_ptr(), 2 * v0, 2 * v1, num_heads, head_dim, 0, 0, 0)
+    dests = _dests(k_cache.data_ptr(), v_cache.data_ptr(), (2 * strides[0], 2 * strides[1], 2 * strides[2]), block_size,
+                   num_blocks, slots, num_heads, push_to, num_tokens, key.device)
     out = _output(query, out, stream)
-    _launch(rows, out, rotary, positions, num_tokens, _DTYPES[dtype], eps, dests, stream, flags, status, device)
+    _launch(rows, out, rotary, positions, position_bytes, num_tokens, dtype, eps, dests, stream, flags, status, device)
     return out
 
 
@@ -195,37 +214,42 @@ def rotate_store_latents(latent: torch.Tensor, latent_cache: torch.Tensor, slot_
     if latent.dim() != 2 or latent_cache.dim() != 3 or latent_cache.size(2) != latent.size(1):
         raise ValueError(f"latents {tuple(latent.shape)} into a cache {tuple(latent_cache.shape)}")
     num_tokens, dim = latent.shape
+    num_blocks, block_size, _ = latent_cache.shape
     rotary_dim = rotary.table.size(1)
     if rotary_dim > dim:
         raise ValueError(f"a rotary table of {rotary_dim} elements for latents of {dim}")
-    dtype, device = latent.dtype, latent.device
+    dtype, device = latent.dtype, latent.get_device()
     if dtype not in _DTYPES or dtype != latent_cache.dtype or (query_pe is not None and query_pe.dtype != dtype):
         raise TypeError(f"latents, queries and cache must share a dtype, bfloat16 or float16: {dtype}, "
                         f"{latent_cache.dtype}")
-    if device != latent_cache.device or (query_pe is not None and query_pe.device != device):
+    if device != latent_cache.get_device() or (query_pe is not None and query_pe.get_device() != device):
         raise ValueError("latents, queries and the local cache must be on one device")
-    if latent_cache.stride(-2) != dim or latent_cache.stride(-1) != 1:
+    block_stride, token_stride, unit = latent_cache.stride()
+    if token_stride != dim or unit != 1:
         raise ValueError("cache tokens must be contiguous")
-    if query_pe is not None and (query_pe.dim() != 3 or query_pe.size(0) != num_tokens or query_pe.size(2) != rotary_dim):
-        raise ValueError(f"queries' rotated part {tuple(query_pe.shape)} for {num_tokens} rows of {rotary_dim}")
+    l0, l1 = latent.stride()
+    if l1 != 1:
+        raise ValueError("a latent's elements must be contiguous")
     if len(push_to) > 8:
         raise ValueError("at most 8 peers per store")
-    slots = _slots(slot_mapping, num_tokens, device)
-    _positions(positions, num_tokens, device)
+    slots = _slots(slot_mapping, num_tokens, latent.device)
+    position_bytes = _positions(positions, num_tokens, device)
     rank = dim - rotary_dim
-    rows = (_rows(query_pe, None, 0, 0) if query_pe is not None else RotateRows(),
-            _rows(latent, weight, rank, rank), RotateRows())
-    dests = [_dest(latent_cache.data_ptr(), 0, latent_cache.stride(0) * 2, dim * 2, 0, latent_cache.size(1),
-                   latent_cache.size(0), slots, 0, 1, 0)]
-    for target in push_to:
-        t_slots = _target_slots(target, num_tokens, device)
-        dests.append(_dest(target.k_cache, 0, target.block_stride, target.token_stride, 0, target.block_size,
-                           target.num_blocks, t_slots, 0, 1, 0, target.block_map))
+    normed, scale = _weight(weight, rank, dtype, device)
     if query_pe is not None:
+        if query_pe.dim() != 3 or query_pe.size(0) != num_tokens or query_pe.size(2) != rotary_dim:
+            raise ValueError(f"queries' rotated part {tuple(query_pe.shape)} for {num_tokens} rows of {rotary_dim}")
+        q0, q1, q2 = query_pe.stride()
+        if q2 != 1:
+            raise ValueError("a head's elements must be contiguous")
+        query = (query_pe.data_ptr(), 2 * q0, 2 * q1, query_pe.size(1), rotary_dim, 0, 0, 0)
         out = _output(query_pe, out, stream)
     else:
-        out = None
-    _launch(rows, out, rotary, positions, num_tokens, _DTYPES[dtype], eps, dests, stream, flags, status, device)
+        query, out = _NO_ROWS, None
+    rows = (*query, latent.data_ptr(), 2 * l0, 0, 1, dim, normed, rank, scale, *_NO_ROWS)
+    dests = _dests(latent_cache.data_ptr(), 0, (2 * block_stride, 2 * dim, 0), block_size, num_blocks, slots, 1, push_to,
+                   num_tokens, latent.device)
+    _launch(rows, out, rotary, positions, position_bytes, num_tokens, dtype, eps, dests, stream, flags, status, device)
     return out
 
 

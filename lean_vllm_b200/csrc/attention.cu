@@ -422,9 +422,10 @@ constexpr size_t kWorkspaceBytes = kSplitAt + kSplitRows * (kMlBytes + kOutBytes
 static_assert(kMaxRowCtas <= kTileCounter && (kTileCounter + 1) * sizeof(int32_t) <= KVX_ATTENTION_ZEROED, "counters");
 
 template <class T, int D>
-int launch_rows(const AttnParams &p, bool mods, int sms, cudaStream_t stream) {
+int launch_rows(const AttnParams &p, bool mods, const Device &device, cudaStream_t stream) {
+    static AllowedSmem allowed[2];
     auto kernel = mods ? attention_rows<T, D, true> : attention_rows<T, D, false>;
-    KVX_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, row_smem<D>()));
+    if (int rc = allowed[mods].allow(kernel, row_smem<D>(), device.index)) return rc;
     cudaLaunchConfig_t cfg = {};
     cfg.stream = stream;
     cudaLaunchAttribute attr;
@@ -432,7 +433,7 @@ int launch_rows(const AttnParams &p, bool mods, int sms, cudaStream_t stream) {
     attr.val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = &attr;
     cfg.numAttrs = 1;
-    cfg.gridDim = dim3((unsigned)std::min(2 * sms, kMaxRowCtas));
+    cfg.gridDim = dim3((unsigned)std::min(2 * device.sms, kMaxRowCtas));
     cfg.blockDim = dim3(kRowThreads);
     cfg.dynamicSmemBytes = row_smem<D>();
     KVX_CUDA(cudaLaunchKernelEx(&cfg, kernel, p));
@@ -528,10 +529,10 @@ int kvx_attention(const kvx_attention_args *args, int flags, void *stream) {
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     auto rows_kernel = [&]() {
         if (a.head_dim == 128)
-            return a.dtype == KVX_BF16 ? launch_rows<__nv_bfloat16, 128>(p, mods, device.sms, s)
-                                       : launch_rows<__half, 128>(p, mods, device.sms, s);
-        return a.dtype == KVX_BF16 ? launch_rows<__nv_bfloat16, 64>(p, mods, device.sms, s)
-                                   : launch_rows<__half, 64>(p, mods, device.sms, s);
+            return a.dtype == KVX_BF16 ? launch_rows<__nv_bfloat16, 128>(p, mods, device, s)
+                                       : launch_rows<__half, 128>(p, mods, device, s);
+        return a.dtype == KVX_BF16 ? launch_rows<__nv_bfloat16, 64>(p, mods, device, s)
+                                   : launch_rows<__half, 64>(p, mods, device, s);
     };
 
     // ---- which kernel takes what
@@ -549,7 +550,7 @@ int kvx_attention(const kvx_attention_args *args, int flags, void *stream) {
     if (a.shared_len > 0 && q_rows <= kTileKeys && (int64_t)a.num_tokens * a.q_heads <= kSplitRows) {
         // A prefix shared by short sequences: all their rows together against it, then each against its own keys.
         const int splits = splits_for((all_rows + kTileRows - 1) / kTileRows, a.shared_len);
-        if (int rc = launch_tiles(p, a.head_dim, a.dtype, mods, true, splits, device.sms, s)) return rc;
+        if (int rc = launch_tiles(p, a.head_dim, a.dtype, mods, true, splits, device, s)) return rc;
         p.prefix_splits = splits;
         p.shared_len = 0;
         return rows_kernel();
@@ -560,7 +561,7 @@ int kvx_attention(const kvx_attention_args *args, int flags, void *stream) {
     p.rows_limit = mixed ? kRowTile : 0;
     const int64_t row_tiles = std::max<int64_t>(1, all_rows / kTileRows);
     const int splits = splits_for(row_tiles, (int64_t)a.max_kv_len + a.shared_len);
-    if (int rc = launch_tiles(p, a.head_dim, a.dtype, mods, false, splits, device.sms, s)) return rc;
+    if (int rc = launch_tiles(p, a.head_dim, a.dtype, mods, false, splits, device, s)) return rc;
     return mixed ? rows_kernel() : KVX_OK;
 }
 

@@ -4,6 +4,8 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include <atomic>
+
 #include "kvx_internal.cuh"
 
 namespace kvx {
@@ -38,10 +40,22 @@ struct AttnParams {
     int32_t *status, *error_word;
 };
 
+// Which devices a kernel has its dynamic shared memory allowed on: asked for once per device, not per launch.
+struct AllowedSmem {
+    std::atomic<bool> on[64] = {};
+    template <class Kernel>
+    int allow(Kernel kernel, int bytes, int device) {
+        if (device < 64 && on[device].load(std::memory_order_relaxed)) return KVX_OK;
+        KVX_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
+        if (device < 64) on[device].store(true, std::memory_order_relaxed);
+        return KVX_OK;
+    }
+};
+
 // attention_tiles (attention_tiles.cu). `prefix_only`: all query rows against the shared prefix alone, as partial
 // results of `splits`; else each sequence's rows above rows_limit, joined when splits is above 1.
 int launch_tiles(const AttnParams &p, int head_dim, int dtype, bool mods, bool prefix_only, int splits,
-                 int sms, cudaStream_t stream);
+                 const Device &device, cudaStream_t stream);
 // The tokens of this cache that one of attention_tiles' copies brings; 0 if it cannot take the call (blocks that are no
 // multiple of 8 tokens, strides that no tensor map holds, groups beyond a tile's rows).
 int tile_box(const AttnParams &p);

@@ -930,11 +930,12 @@ int launch(Kernel kernel, const TileParams &t, int64_t grid, int threads, int sm
 }
 
 template <class T, int D>
-int launch_typed(const TileParams &t, bool mods, int sms, cudaStream_t stream) {
+int launch_typed(const TileParams &t, bool mods, const Device &device, cudaStream_t stream) {
+    static AllowedSmem allowed[2];
     auto kernel = mods ? attention_tiles<T, D, true> : attention_tiles<T, D, false>;
-    KVX_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape<D>::kBytes));
+    if (int rc = allowed[mods].allow(kernel, Shape<D>::kBytes, device.index)) return rc;
     const int64_t items = (int64_t)t.row_tiles * t.a.kv_heads;
-    const int64_t grid = std::min<int64_t>(items * t.splits, sms);  // one CTA per SM, item after item
+    const int64_t grid = std::min<int64_t>(items * t.splits, device.sms);  // one CTA per SM, item after item
     if (int rc = launch(kernel, t, grid, kThreads, Shape<D>::kBytes, stream)) return rc;
     if (t.prefix_only || t.splits == 1) return KVX_OK;
     return launch(attention_join<T, D>, t, items * (kTileRows / kJoinRows), kJoinThreads, 0, stream);
@@ -952,7 +953,7 @@ int kvx::tile_box(const AttnParams &p) {
 }
 
 int kvx::launch_tiles(const AttnParams &p, int head_dim, int dtype, bool mods, bool prefix_only, int splits,
-                      int sms, cudaStream_t stream) {
+                      const Device &device, cudaStream_t stream) {
     TileParams t;
     t.a = p;
     t.box = tile_box(p);
@@ -966,8 +967,8 @@ int kvx::launch_tiles(const AttnParams &p, int head_dim, int dtype, bool mods, b
     if (int rc = cache_map(&t.values, p, p.v_cache, head_dim, dtype, t.box)) return rc;
     if (int rc = query_map(&t.queries, p, head_dim, dtype, t.tile_tokens)) return rc;
     if (head_dim == 128)
-        return dtype == KVX_BF16 ? launch_typed<__nv_bfloat16, 128>(t, mods, sms, stream)
-                                 : launch_typed<__half, 128>(t, mods, sms, stream);
-    return dtype == KVX_BF16 ? launch_typed<__nv_bfloat16, 64>(t, mods, sms, stream)
-                             : launch_typed<__half, 64>(t, mods, sms, stream);
+        return dtype == KVX_BF16 ? launch_typed<__nv_bfloat16, 128>(t, mods, device, stream)
+                                 : launch_typed<__half, 128>(t, mods, device, stream);
+    return dtype == KVX_BF16 ? launch_typed<__nv_bfloat16, 64>(t, mods, device, stream)
+                             : launch_typed<__half, 64>(t, mods, device, stream);
 }

@@ -175,6 +175,10 @@ __global__ void __launch_bounds__(kAnyThreads) rotate_store_any(const __grid_con
 // reads the token's angles, slot and norm weights once for them. Bound by HBM: a step's rows in and out, once.
 
 constexpr int kFastThreads = 256;
+// One resident wave of 4 CTAs per SM at 64 registers. 8192 tokens of 32 + 8 + 8 heads of 128: 37.5 us (5.48 TB/s); with
+// twice as many CTAs 38.5, with a CTA for every 8 units 47; 5 resident CTAs (48 registers) 43.2, 6 with half the loads in
+// flight 54.7.
+constexpr int kFastCtas = 4;
 
 __device__ __forceinline__ float2 unpack(uint32_t bits, __nv_bfloat16) {
     return make_float2(__uint_as_float(bits << 16), __uint_as_float(bits & 0xffff0000u));
@@ -327,7 +331,7 @@ __device__ __forceinline__ void rotate_rows(const RotateParams &p, const Rows &r
 }
 
 template <class T, int LANES, int PASSES, bool INTERLEAVED>
-__global__ void __launch_bounds__(kFastThreads, 4) rotate_store_fast(const __grid_constant__ RotateParams p) {
+__global__ void __launch_bounds__(kFastThreads, kFastCtas) rotate_store_fast(const __grid_constant__ RotateParams p) {
     launch_dependents();
     const Place place = place_of<INTERLEAVED>((threadIdx.x & 31) % LANES, p.rotary_dim);
     constexpr int kRows = PASSES * (32 / LANES);
@@ -442,11 +446,12 @@ Rows rows_of(const kvx_rotate_rows &r) {
                 r.num_heads, r.dim, r.norm_dim, r.rotary_first};
 }
 
-// One warp per unit of work, in one resident wave of CTAs at most: each sweeps its share.
-int launch(void (*kernel)(RotateParams), const RotateParams &p, cudaLaunchConfig_t cfg, int64_t units, int sms) {
+// One warp per unit of work, `ctas_per_sm` CTAs at most: each sweeps its share.
+int launch(void (*kernel)(RotateParams), const RotateParams &p, cudaLaunchConfig_t cfg, int64_t units, int sms,
+           int ctas_per_sm) {
     static_assert(kFastThreads == kAnyThreads, "one block size");
-    constexpr int kWarps = kFastThreads / 32, kCtasPerSm = 8;
-    cfg.gridDim = dim3((unsigned)std::min<int64_t>((units + kWarps - 1) / kWarps, (int64_t)sms * kCtasPerSm));
+    constexpr int kWarps = kFastThreads / 32;
+    cfg.gridDim = dim3((unsigned)std::min<int64_t>((units + kWarps - 1) / kWarps, (int64_t)sms * ctas_per_sm));
     cfg.blockDim = dim3(kFastThreads);
     KVX_CUDA(cudaLaunchKernelEx(&cfg, kernel, p));
     count_launch();
@@ -461,7 +466,7 @@ int units_of(const RotateParams &p, int at_once) {
 template <class T, int LANES, int PASSES>
 int launch_rows(const RotateParams &p, const cudaLaunchConfig_t &cfg, int sms) {
     return launch(p.interleaved ? rotate_store_fast<T, LANES, PASSES, true> : rotate_store_fast<T, LANES, PASSES, false>, p,
-                  cfg, (int64_t)units_of(p, PASSES * (32 / LANES)) * p.num_tokens, sms);
+                  cfg, (int64_t)units_of(p, PASSES * (32 / LANES)) * p.num_tokens, sms, kFastCtas);
 }
 
 template <class T, int LANES>
@@ -488,7 +493,7 @@ int launch_fast(const RotateParams &p, const cudaLaunchConfig_t &cfg, int sms) {
 template <class T, int CHUNKS>
 int launch_chunks(const RotateParams &p, const cudaLaunchConfig_t &cfg, int sms) {
     return launch(p.interleaved ? rotate_latents_fast<T, CHUNKS, true> : rotate_latents_fast<T, CHUNKS, false>, p, cfg,
-                  (int64_t)(1 + (p.query.heads + 15) / 16) * p.num_tokens, sms);
+                  (int64_t)(1 + (p.query.heads + 15) / 16) * p.num_tokens, sms, 8);
 }
 
 template <class T>
@@ -584,5 +589,5 @@ extern "C" int kvx_rotate_store(const kvx_rotate_args *args, const kvx_store_des
         (!has_query || (p.query.dim == 64 && p.query.rotary_first == 0 && p.query.norm_dim == 0)))
         return bf16 ? launch_latents<__nv_bfloat16>(p, cfg, sms, rank / 256) : launch_latents<__half>(p, cfg, sms, rank / 256);
     return launch(bf16 ? rotate_store_any<__nv_bfloat16> : rotate_store_any<__half>, p, cfg,
-                  (int64_t)heads * p.num_tokens, sms);
+                  (int64_t)heads * p.num_tokens, sms, 8);
 }

@@ -163,7 +163,7 @@ def test_the_abi_refuses_attention_arguments(change, message):
     if not os.path.exists(_native.LIB_PATH):
         pytest.skip("libkvx.so is not built here")
     with pytest.raises(_native.KvxError, match=message):
-        _native.check(_native.lib().kvx_attention(attention_struct(**change), 0, None))
+        _native.check(_native.lib().kvx_attention(ctypes.addressof(struct := attention_struct(**change)), 0, None))
 
 
 def test_the_abi_refuses_rotate_arguments():
@@ -179,7 +179,8 @@ def test_the_abi_refuses_rotate_arguments():
         fields = dict(query=rows(), key=rows(), value=rows(), query_out=16, table=16, positions=16, num_positions=8,
                       rotary_dim=64, position_bytes=8, num_tokens=4, eps=1e-6)
         fields.update(change)
-        _native.check(lib.kvx_rotate_store(_native.RotateArgs(**fields), dests, n, None, 0, None))
+        args = _native.RotateArgs(**fields)
+        _native.check(lib.kvx_rotate_store(ctypes.addressof(args), ctypes.addressof(dests), n, None, 0, None))
 
     for change, message in [
         (dict(dtype=9), "element type 9"), (dict(num_tokens=-1), "-1 tokens"), (dict(rotary_dim=7), "not an even"),
@@ -219,6 +220,23 @@ def test_the_structs_are_the_header_s(tmp_path):
         want.append(ctypes.sizeof(struct))
         want += [getattr(struct, field).offset for field, _ in struct._fields_]
     assert got == want + [_native.ATTENTION_ZEROED]
+
+
+@pytest.mark.parametrize("struct, packed", [(_native.StoreDest, _native.STORE_DEST), (_native.RotateArgs, _native.ROTATE_ARGS),
+                                            (_native.AttentionArgs, _native.ATTENTION_ARGS)])
+def test_packed_structs_are_the_ctypes_structs(struct, packed):
+    """A pack() of 1, 2, 3, ... reads back, field by field, as the ctypes struct's values in order."""
+    def fields(s):
+        for name, kind in s._fields_:
+            value = getattr(s, name)
+            if isinstance(value, ctypes.Structure):
+                yield from fields(value)
+            else:
+                yield value
+
+    assert packed.size == ctypes.sizeof(struct)
+    n = len(packed.unpack(bytes(packed.size)))
+    assert [int(v) for v in fields(struct.from_buffer_copy(packed.pack(*range(1, n + 1))))] == list(range(1, n + 1))
 
 
 def test_rotary_angles():
