@@ -16,28 +16,43 @@ using namespace kvx;
 
 // ------------------------------------------------------------------------------------------------ rows kernel
 //
-// attention_rows: up to 16 query rows of one KV head (its group of query heads x the sequence's query tokens) against
-// a stretch of a sequence's keys: the form for single tokens, bound by reading the cache.
+// attention_rows: up to 8 or 16 query rows of one KV head (its group of query heads x the sequence's query tokens)
+// against a stretch of a sequence's keys: the form for single tokens, bound by reading the cache.
 //
-// Work. The rows of a KV head share its keys, so a (sequence, KV head, tile of 16 rows) group reads them once. Its
-// keys are cut into tiles of 64 tokens; the tiles of all groups of all sequences, counted on the device from the
-// lengths, are dealt out in equal contiguous runs to a grid of two CTAs per SM, whatever the lengths. A CTA's run
-// covers whole groups and at most two partial ones; a partial group leaves (m, sum, o) in the workspace, and the CTA
-// that brings the last part joins them in a fixed order (the result does not depend on which one that is).
+// Work. The rows of a KV head share its keys, so a (sequence, KV head, tile of rows) group reads them once. Its keys are
+// cut into tiles of 64 tokens; the tiles of all groups of all sequences, counted on the device from the lengths, are
+// dealt out in equal contiguous runs to one wave of CTAs, whatever the lengths. A CTA's run covers whole groups and at
+// most two partial ones; a partial group leaves (m, sum, o) in the workspace, and the CTA that brings the last part joins
+// them in a fixed order (the result does not depend on which one that is). A run is kMinRun tiles at least: below that a
+// part costs more to join than to compute.
 //
 // Inside a CTA each of the 4 warps takes its own 16 tokens of every tile with its own running maximum, sum and output,
-// and loads them itself with cp.async into its own ring of 3 stages: no barrier until the group's end.
+// and loads them itself with cp.async into its own ring: no barrier until the group's end.
+//
+// Up to 8 rows the products run transposed, S^T = K Q^T and O^T = V^T P^T, with the rows as the tensor cores' 8 columns:
+// half the instructions and registers of a 16-row tile that would be half padding.
 
-constexpr int kRowTile = 16;
 constexpr int kRowWarps = 4;
 constexpr int kRowThreads = kRowWarps * 32;
-constexpr int kRowStages = 3;
 constexpr int kWarpTokens = 16;
 constexpr int kTileTokens = kRowWarps * kWarpTokens;
+#ifndef STAGES8
+#define STAGES8 2
+#define CTAS8 3
+#define STAGES16 3
+#define MINRUN 1
+#endif
+constexpr int kMinRun = MINRUN;
 
-template <int D>
+template <int ROWS>
+struct RowShape {
+    static constexpr int kStages = ROWS == 8 ? STAGES8 : STAGES16;
+    static constexpr int kCtas = ROWS == 8 ? CTAS8 : 2;  // per SM
+};
+
+template <int D, int ROWS>
 constexpr int row_smem() {
-    return kRowWarps * kRowStages * kWarpTokens * D * 2 * 2;
+    return kRowWarps * RowShape<ROWS>::kStages * kWarpTokens * D * 2 * 2;
 }
 
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void *src, bool valid) {
@@ -76,27 +91,36 @@ __device__ __forceinline__ void mma16816<__half>(float (&c)[4], const uint32_t *
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
+// The transpose of an 8 x 8 matrix of 16-bit elements, two of a row per lane.
+__device__ __forceinline__ uint32_t transpose8(uint32_t x) {
+    uint32_t y;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+    return y;
+}
+
 // A sequence's share of the launch's tiles.
 struct RowWork {
     int32_t lo, row_tiles, tiles;  // first key, tiles of rows, tiles of keys per group
     __device__ __forceinline__ int64_t groups(const AttnParams &p) const { return (int64_t)row_tiles * p.kv_heads; }
 };
 
+template <int ROWS>
 __device__ __forceinline__ RowWork row_work(const AttnParams &p, const Sequence &q) {
     RowWork w;
     w.lo = first_seen(p, q, q.kv_len - q.q_len);
-    w.row_tiles = (int32_t)(((int64_t)q.q_len * p.group + kRowTile - 1) / kRowTile);
+    w.row_tiles = (int32_t)(((int64_t)q.q_len * p.group + ROWS - 1) / ROWS);
     // An empty cache still gets one (empty) tile: its rows have to be written.
     w.tiles = max(1, (q.kv_len + kTileTokens - 1) / kTileTokens - w.lo / kTileTokens);
     return w;
 }
 
+template <int ROWS>
 __device__ __forceinline__ int64_t row_units(const AttnParams &p, int s) {
     if (blockIdx.x == 0 && (int64_t)p.kv_lens[s] > (int64_t)p.max_blocks * p.block_size)
         flag_error(p.error_word, p.status, kErrPastCache);
     const Sequence q = sequence_of(p, s);
     if ((int64_t)q.q_len * p.group > p.rows_limit) return 0;  // attention_tiles takes it
-    const RowWork w = row_work(p, q);
+    const RowWork w = row_work<ROWS>(p, q);
     return w.groups(p) * w.tiles;
 }
 
@@ -107,32 +131,34 @@ __device__ __forceinline__ uint64_t row_address(const AttnParams &p, uint64_t ba
     return base + (int64_t)(q.q0 + token) * token_stride + (int64_t)(h * p.group + row - token * p.group) * head_stride;
 }
 
-template <class T, int D, bool MODS>
-__global__ void __launch_bounds__(kRowThreads, 2) attention_rows(const __grid_constant__ AttnParams p) {
+template <class T, int D, int ROWS, bool MODS>
+__global__ void __launch_bounds__(kRowThreads, RowShape<ROWS>::kCtas)
+attention_rows(const __grid_constant__ AttnParams p) {
+    constexpr int kStages = RowShape<ROWS>::kStages;
     extern __shared__ __align__(128) unsigned char smem[];
     __shared__ int64_t scan[kRowWarps + 1];
     __shared__ int64_t found_start;
     __shared__ int found_sequence;
-    __shared__ float2 warp_ml[kRowWarps][kRowTile];
+    __shared__ float2 warp_ml[kRowWarps][ROWS];
     __shared__ int is_last;
 
     launch_dependents();
-    // Behind a kernel that computes the shared prefix's part, only the joining below has to wait for it: that kernel
-    // lets this one start after its own wait, so everything before it is complete.
+    // Beside attention_tiles' part over a shared prefix nothing here waits for it: that kernel lets this one start after
+    // its own wait, so everything before it is complete, and attention_join takes both parts.
     if (p.prefix_splits == 0) wait_prerequisites();
 
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
 
     // ---- this CTA's run of tiles
     int64_t mine = 0;
-    for (int s = tid; s < p.batch; s += kRowThreads) mine += row_units(p, s);
+    for (int s = tid; s < p.batch; s += kRowThreads) mine += row_units<ROWS>(p, s);
 #pragma unroll
     for (int o = 16; o; o >>= 1) mine += __shfl_xor_sync(~0u, mine, o);
     if (lane == 0) scan[warp] = mine;
     __syncthreads();
     int64_t total = 0;
     for (int w = 0; w < kRowWarps; ++w) total += scan[w];
-    const int64_t per_cta = (total + gridDim.x - 1) / gridDim.x;
+    const int64_t per_cta = max((int64_t)kMinRun, (total + gridDim.x - 1) / gridDim.x);
     int64_t unit = (int64_t)blockIdx.x * per_cta;
     const int64_t unit_end = min(total, unit + per_cta);
     if (unit >= unit_end) {
@@ -142,7 +168,7 @@ __global__ void __launch_bounds__(kRowThreads, 2) attention_rows(const __grid_co
     int64_t before = 0;  // tiles of the sequences looked at so far
     for (int s0 = 0;; s0 += kRowThreads) {
         const int s = s0 + tid;
-        int64_t n = s < p.batch ? row_units(p, s) : 0, sum = n;
+        int64_t n = s < p.batch ? row_units<ROWS>(p, s) : 0, sum = n;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
             const int64_t up = __shfl_up_sync(~0u, sum, o);
@@ -171,14 +197,21 @@ __global__ void __launch_bounds__(kRowThreads, 2) attention_rows(const __grid_co
     constexpr int kPerCopy = 32 / kChunks;         // tokens one warp-wide copy covers
     constexpr int kCopies = kWarpTokens / kPerCopy;
     constexpr int kStageBytes = kWarpTokens * D * 2;  // keys; as much again for values
-    const uint32_t ring = smem_u32(smem) + warp * kRowStages * 2 * kStageBytes;
-    float *my_o = reinterpret_cast<float *>(smem + warp * kRowStages * 2 * kStageBytes);  // once the ring is done with
+    constexpr int kOutRow = D + 4;                    // floats of a row of a warp's output on its way to the join
+    static_assert(ROWS * kOutRow * 4 <= kStages * 2 * kStageBytes, "a warp's output fits its ring");
+    const uint32_t ring = smem_u32(smem) + warp * kStages * 2 * kStageBytes;
+    float *my_o = reinterpret_cast<float *>(smem + warp * kStages * 2 * kStageBytes);  // once the ring is done with
     const float scale_log2 = p.scale * kLog2e;
+    const float cap_in = p.softcap > 0.f ? scale_log2 * 2.f / p.softcap : 0.f, cap_out = p.softcap * kLog2e;
+    // Blocks of whole stages: one lookup and one address a stage, the copies' a constant step apart.
+    const bool stage_in_block = p.block_size % kWarpTokens == 0 && p.shared_len == 0;
+    const int64_t copy_step = kPerCopy * p.token_stride;
+    const uint32_t lane_to = (lane / kChunks) * D * 2;
 
     while (unit < unit_end) {
         const Sequence q = sequence_of(p, s);
-        const RowWork work = row_work(p, q);
-        const int64_t s_end = s_start + row_units(p, s);
+        const RowWork work = row_work<ROWS>(p, q);
+        const int64_t s_end = s_start + row_units<ROWS>(p, s);
         if (unit >= s_end) {
             s_start = s_end;
             ++s;
@@ -188,57 +221,90 @@ __global__ void __launch_bounds__(kRowThreads, 2) attention_rows(const __grid_co
         const int64_t group_index = in_sequence / work.tiles;
         const int tile0 = (int)(in_sequence - group_index * work.tiles);
         const int h = (int)(group_index / work.row_tiles);
-        const int row0 = (int)(group_index - (int64_t)h * work.row_tiles) * kRowTile;
+        const int row0 = (int)(group_index - (int64_t)h * work.row_tiles) * ROWS;
         const int64_t group_start = s_start + group_index * work.tiles, group_end = group_start + work.tiles;
         const int n_tiles = (int)(min(unit_end, group_end) - unit);
-        const int rows = min(kRowTile, q.q_len * p.group - row0);
+        const int rows = min(ROWS, q.q_len * p.group - row0);
         const int first_token = work.lo / kTileTokens * kTileTokens + tile0 * kTileTokens + warp * kWarpTokens;
-        const int64_t head_offset = (int64_t)h * p.head_stride;
+        const int64_t lane_from = (int64_t)h * p.head_stride +
+                                  (stage_in_block ? (lane / kChunks) * p.token_stride + (lane % kChunks) * 16 : 0);
 
-        // The byte offset of this lane's token (lanes 0-15) in stage i, or -1 where nothing is to be read.
-        auto token_offset = [&](int i) -> int64_t {
-            const int t = first_token + i * kTileTokens + lane;
-            if (i >= n_tiles || lane >= kWarpTokens || t < work.lo || t >= q.kv_len) return -1;
+        // Where stage i's tokens lie: in one block, this lane's first copy; else this lane's token (lanes 0-15). A byte
+        // offset, or -1 where nothing is to be read.
+        auto stage_offset = [&](int i) -> int64_t {
+            const int t = first_token + i * kTileTokens + (stage_in_block ? 0 : lane);
+            if (i >= n_tiles || t >= q.kv_len) return -1;
+            if (stage_in_block ? t + kWarpTokens <= work.lo : lane >= kWarpTokens || t < work.lo) return -1;
             const int64_t at = token_at(p, s, t);
-            return at < 0 ? -1 : at + head_offset;
+            return at < 0 ? -1 : at + lane_from;
         };
         auto load_stage = [&](int i, int64_t offset) {
-            const uint32_t k_stage = ring + (i % kRowStages) * 2 * kStageBytes, v_stage = k_stage + kStageBytes;
+            const uint32_t k_stage = ring + (i % kStages) * 2 * kStageBytes + lane_to;
+            if (stage_in_block) {
+                const int t = first_token + i * kTileTokens + lane / kChunks;
+                uint64_t key = p.k_cache + (offset < 0 ? 0 : offset), value = p.v_cache + (offset < 0 ? 0 : offset);
 #pragma unroll
-            for (int c = 0; c < kCopies; ++c) {
-                const int token = c * kPerCopy + lane / kChunks, chunk = lane % kChunks;
-                const int64_t at = __shfl_sync(~0u, offset, token);
-                const uint32_t to = token * D * 2 + ((chunk ^ (token & 7)) << 4);
-                const int64_t from = at < 0 ? 0 : at + chunk * 16;
-                cp_async16(k_stage + to, reinterpret_cast<const void *>(p.k_cache + from), at >= 0);
-                cp_async16(v_stage + to, reinterpret_cast<const void *>(p.v_cache + from), at >= 0);
+                for (int c = 0; c < kCopies; ++c) {
+                    const int token = c * kPerCopy + lane / kChunks;
+                    const bool valid = offset >= 0 && t + c * kPerCopy >= work.lo && t + c * kPerCopy < q.kv_len;
+                    const uint32_t to = k_stage + c * kPerCopy * D * 2 + (((lane % kChunks) ^ (token & 7)) << 4);
+                    cp_async16(to, reinterpret_cast<const void *>(key), valid);
+                    cp_async16(to + kStageBytes, reinterpret_cast<const void *>(value), valid);
+                    if (offset >= 0) key += copy_step, value += copy_step;
+                }
+            } else {
+#pragma unroll
+                for (int c = 0; c < kCopies; ++c) {
+                    const int token = c * kPerCopy + lane / kChunks, chunk = lane % kChunks;
+                    const int64_t at = __shfl_sync(~0u, offset, token);
+                    const uint32_t to = k_stage + c * kPerCopy * D * 2 + ((chunk ^ (token & 7)) << 4);
+                    const int64_t from = at < 0 ? 0 : at + chunk * 16;
+                    cp_async16(to, reinterpret_cast<const void *>(p.k_cache + from), at >= 0);
+                    cp_async16(to + kStageBytes, reinterpret_cast<const void *>(p.v_cache + from), at >= 0);
+                }
             }
         };
 #pragma unroll
-        for (int i = 0; i < kRowStages - 1; ++i) {
-            if (i < n_tiles) load_stage(i, token_offset(i));
+        for (int i = 0; i < kStages - 1; ++i) {
+            if (i < n_tiles) load_stage(i, stage_offset(i));
             asm volatile("cp.async.commit_group;" ::: "memory");
         }
-        int64_t next_offset = token_offset(kRowStages - 1);
+        int64_t next_offset = stage_offset(kStages - 1);
 
-        // ---- queries, in the registers of the first product
-        uint32_t qa[D / 16][4];
-        int position[2], prefix[2];  // of rows lane / 4 and lane / 4 + 8
-        float slope[2];
-#pragma unroll
-        for (int r = 0; r < 2; ++r) {
-            const int row = lane / 4 + 8 * r;
-            const bool valid = row < rows;
-            const uint64_t at = valid ? row_address(p, p.query, p.q_token_stride, p.q_head_stride, q, h, row0 + row) : 0;
-            position[r] = valid ? q.kv_len - q.q_len + (row0 + row) / p.group : -1;
-            prefix[r] = valid ? q.prefix : 0;
-            slope[r] = MODS && valid && p.slopes ? p.slopes[h * p.group + (row0 + row) % p.group] : 0.f;
+        // ---- queries, in the registers of the first product, and what this lane's two rows see
+        constexpr int kQueryRegs = ROWS == 8 ? 2 : 4;
+        uint32_t qf[D / 16][kQueryRegs];
+        if (ROWS == 8) {  // row lane / 4 as a column
+            const int row = lane / 4;
+            const uint64_t at = row < rows ? row_address(p, p.query, p.q_token_stride, p.q_head_stride, q, h, row0 + row) : 0;
 #pragma unroll
             for (int k = 0; k < D / 16; ++k)
 #pragma unroll
                 for (int half = 0; half < 2; ++half)
-                    qa[k][r + 2 * half] =
-                        valid ? *reinterpret_cast<const uint32_t *>(at + (k * 16 + half * 8 + (lane & 3) * 2) * 2) : 0u;
+                    qf[k][half] = at ? *reinterpret_cast<const uint32_t *>(at + (k * 16 + half * 8 + (lane & 3) * 2) * 2) : 0u;
+        } else {  // rows lane / 4 and lane / 4 + 8
+#pragma unroll
+            for (int r = 0; r < 2; ++r) {
+                const int row = lane / 4 + 8 * r;
+                const uint64_t at =
+                    row < rows ? row_address(p, p.query, p.q_token_stride, p.q_head_stride, q, h, row0 + row) : 0;
+#pragma unroll
+                for (int k = 0; k < D / 16; ++k)
+#pragma unroll
+                    for (int half = 0; half < 2; ++half)
+                        qf[k][(r + 2 * half) % kQueryRegs] =
+                            at ? *reinterpret_cast<const uint32_t *>(at + (k * 16 + half * 8 + (lane & 3) * 2) * 2) : 0u;
+            }
+        }
+        int position[2], prefix[2];  // of rows 2 (lane % 4) + r, or lane / 4 + 8 r
+        float slope[2];
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+            const int row = ROWS == 8 ? 2 * (lane & 3) + r : lane / 4 + 8 * r;
+            const bool valid = row < rows;
+            position[r] = valid ? q.kv_len - q.q_len + (row0 + row) / p.group : -1;
+            prefix[r] = valid ? q.prefix : 0;
+            slope[r] = MODS && valid && p.slopes ? p.slopes[h * p.group + (row0 + row) % p.group] * kLog2e : 0.f;
         }
         // Every row of the tile sees the keys from see_lo up to see_hi: whole stages in there need no mask.
         const int first_position = q.kv_len - q.q_len + row0 / p.group;
@@ -246,40 +312,58 @@ __global__ void __launch_bounds__(kRowThreads, 2) attention_rows(const __grid_co
         const int see_lo = p.window > 0 ? max(work.lo, last_position - p.window + 1) : 0;
         const int see_hi = min(q.kv_len, first_position + 1);
 
-        float m[2] = {-INFINITY, -INFINITY}, sum[2] = {0.f, 0.f}, o[D / 8][4];
+        // ---- the walk over the keys. c holds a stage's 16 tokens x ROWS scores: c[n][e] belongs to this lane's row
+        // e / 2 (16 rows: token 8 n + 2 (lane % 4) + e % 2) or e % 2 (8 rows: token lane / 4 + 8 (e / 2)).
+        constexpr int kScores = ROWS == 8 ? 1 : 2, kOut = ROWS == 8 ? D / 16 : D / 8;
+        float m[2] = {-INFINITY, -INFINITY}, sum[2] = {0.f, 0.f}, o[kOut][4];
 #pragma unroll
-        for (int n = 0; n < D / 8; ++n) o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.f;
+        for (int n = 0; n < kOut; ++n) o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.f;
 
         for (int i = 0; i < n_tiles; ++i) {
-            if (i + kRowStages - 1 < n_tiles) load_stage(i + kRowStages - 1, next_offset);
+            if (i + kStages - 1 < n_tiles) load_stage(i + kStages - 1, next_offset);
             asm volatile("cp.async.commit_group;" ::: "memory");
-            next_offset = token_offset(i + kRowStages);
-            asm volatile("cp.async.wait_group %0;" ::"n"(kRowStages - 1) : "memory");
+            next_offset = stage_offset(i + kStages);
+            asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 1) : "memory");
             __syncwarp();
-            const uint32_t k_stage = ring + (i % kRowStages) * 2 * kStageBytes, v_stage = k_stage + kStageBytes;
+            const uint32_t k_stage = ring + (i % kStages) * 2 * kStageBytes, v_stage = k_stage + kStageBytes;
             const int t0 = first_token + i * kTileTokens;
 
-            float c[2][4] = {};
+            float c[kScores][4] = {};
+            if (ROWS == 8) {
+                float odd[4] = {};
 #pragma unroll
-            for (int k = 0; k < D / 16; ++k) {
-                uint32_t b[4];
-                const int token = (lane & 7) + ((lane & 16) >> 1), chunk = 2 * k + ((lane >> 3) & 1);
-                ldmatrix4(b, k_stage + token * D * 2 + ((chunk ^ (token & 7)) << 4));
-                mma16816<T>(c[0], qa[k], b[0], b[1]);
-                mma16816<T>(c[1], qa[k], b[2], b[3]);
+                for (int k = 0; k < D / 16; ++k) {
+                    uint32_t a[4];
+                    const int token = lane & 15, chunk = 2 * k + (lane >> 4);
+                    ldmatrix4(a, k_stage + token * D * 2 + ((chunk ^ (token & 7)) << 4));
+                    mma16816<T>(k & 1 ? odd : c[0], a, qf[k][0], qf[k][1]);
+                }
+#pragma unroll
+                for (int e = 0; e < 4; ++e) c[0][e] += odd[e];
+            } else {
+#pragma unroll
+                for (int k = 0; k < D / 16; ++k) {
+                    uint32_t b[4];
+                    const int token = (lane & 7) + ((lane & 16) >> 1), chunk = 2 * k + ((lane >> 3) & 1);
+                    ldmatrix4(b, k_stage + token * D * 2 + ((chunk ^ (token & 7)) << 4));
+                    mma16816<T>(c[0], qf[k], b[0], b[1]);
+                    mma16816<T>(c[kScores - 1], qf[k], b[2], b[3]);
+                }
             }
             const bool masked = t0 < see_lo || t0 + kWarpTokens > see_hi;
             float stage_max[2] = {-INFINITY, -INFINITY};
 #pragma unroll
-            for (int n = 0; n < 2; ++n)
+            for (int n = 0; n < kScores; ++n)
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    const int r = e >> 1, t = t0 + n * 8 + (lane & 3) * 2 + (e & 1);
-                    float x;
+                    const int r = ROWS == 8 ? e & 1 : e >> 1;
+                    const int t = t0 + (ROWS == 8 ? lane / 4 + 8 * (e >> 1) : n * 8 + (lane & 3) * 2 + (e & 1));
+                    float x;  // the score times log2(e)
                     if (MODS) {
-                        x = c[n][e] * p.scale;
-                        if (p.softcap > 0.f) x = p.softcap * tanhf(x / p.softcap);
-                        x = (x + slope[r] * (float)(t - position[r])) * kLog2e;
+                        // tanh(z) = 1 - 2 / (e^2z + 1), to 2^-22 of the cap, where the exponent's error counts
+                        x = p.softcap > 0.f ? cap_out - 2.f * cap_out * reciprocal_fast(exp2_fast(c[n][e] * cap_in) + 1.f)
+                                            : c[n][e] * scale_log2;
+                        x += slope[r] * (float)(t - position[r]);
                     } else {
                         x = c[n][e] * scale_log2;
                     }
@@ -292,12 +376,17 @@ __global__ void __launch_bounds__(kRowThreads, 2) attention_rows(const __grid_co
                     c[n][e] = x;
                     stage_max[r] = fmaxf(stage_max[r], x);
                 }
-            float reference[2];
             bool grown = false;
 #pragma unroll
             for (int r = 0; r < 2; ++r) {
-                stage_max[r] = fmaxf(stage_max[r], __shfl_xor_sync(~0u, stage_max[r], 1));
-                stage_max[r] = fmaxf(stage_max[r], __shfl_xor_sync(~0u, stage_max[r], 2));
+                if (ROWS == 8) {
+                    stage_max[r] = fmaxf(stage_max[r], __shfl_xor_sync(~0u, stage_max[r], 4));
+                    stage_max[r] = fmaxf(stage_max[r], __shfl_xor_sync(~0u, stage_max[r], 8));
+                    stage_max[r] = fmaxf(stage_max[r], __shfl_xor_sync(~0u, stage_max[r], 16));
+                } else {
+                    stage_max[r] = fmaxf(stage_max[r], __shfl_xor_sync(~0u, stage_max[r], 1));
+                    stage_max[r] = fmaxf(stage_max[r], __shfl_xor_sync(~0u, stage_max[r], 2));
+                }
                 grown |= stage_max[r] > m[r];
             }
             if (__any_sync(~0u, grown)) {
@@ -307,27 +396,44 @@ __global__ void __launch_bounds__(kRowThreads, 2) attention_rows(const __grid_co
                     m[r] = now;
                     sum[r] *= factor;
 #pragma unroll
-                    for (int n = 0; n < D / 8; ++n) o[n][2 * r] *= factor, o[n][2 * r + 1] *= factor;
+                    for (int n = 0; n < kOut; ++n) {
+                        o[n][ROWS == 8 ? r : 2 * r] *= factor;
+                        o[n][ROWS == 8 ? r + 2 : 2 * r + 1] *= factor;
+                    }
                 }
             }
+            const float reference[2] = {m[0] == -INFINITY ? 0.f : m[0], m[1] == -INFINITY ? 0.f : m[1]};
 #pragma unroll
-            for (int r = 0; r < 2; ++r) reference[r] = m[r] == -INFINITY ? 0.f : m[r];
-#pragma unroll
-            for (int n = 0; n < 2; ++n)
+            for (int n = 0; n < kScores; ++n)
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    c[n][e] = exp2f(c[n][e] - reference[e >> 1]);
-                    sum[e >> 1] += c[n][e];
+                    const int r = ROWS == 8 ? e & 1 : e >> 1;
+                    c[n][e] = exp2_fast(c[n][e] - reference[r]);
+                    sum[r] += c[n][e];
                 }
-            const uint32_t pa[4] = {Pack2<T>::of(c[0][0], c[0][1]), Pack2<T>::of(c[0][2], c[0][3]),
-                                    Pack2<T>::of(c[1][0], c[1][1]), Pack2<T>::of(c[1][2], c[1][3])};
+            if (ROWS == 8) {
+                // Weights by (token, row) pairs become the second product's (row, token) ones.
+                const uint32_t b0 = transpose8(Pack2<T>::of(c[0][0], c[0][1]));
+                const uint32_t b1 = transpose8(Pack2<T>::of(c[0][2], c[0][3]));
 #pragma unroll
-            for (int n = 0; n < D / 8; n += 2) {
-                uint32_t b[4];
-                const int token = (lane & 7) + (lane & 8), chunk = n + (lane >> 4);
-                ldmatrix4_trans(b, v_stage + token * D * 2 + ((chunk ^ (token & 7)) << 4));
-                mma16816<T>(o[n], pa, b[0], b[1]);
-                mma16816<T>(o[n + 1], pa, b[2], b[3]);
+                for (int n = 0; n < D / 16; ++n) {
+                    uint32_t a[4];
+                    const int token = (lane & 7) + ((lane & 16) >> 1), chunk = 2 * n + ((lane >> 3) & 1);
+                    ldmatrix4_trans(a, v_stage + token * D * 2 + ((chunk ^ (token & 7)) << 4));
+                    mma16816<T>(o[n], a, b0, b1);
+                }
+            } else {
+                constexpr int kLast = kScores - 1;
+                const uint32_t pa[4] = {Pack2<T>::of(c[0][0], c[0][1]), Pack2<T>::of(c[0][2], c[0][3]),
+                                        Pack2<T>::of(c[kLast][0], c[kLast][1]), Pack2<T>::of(c[kLast][2], c[kLast][3])};
+#pragma unroll
+                for (int n = 0; n < D / 8; n += 2) {
+                    uint32_t b[4];
+                    const int token = lane & 15, chunk = n + (lane >> 4);
+                    ldmatrix4_trans(b, v_stage + token * D * 2 + ((chunk ^ (token & 7)) << 4));
+                    mma16816<T>(o[n % kOut], pa, b[0], b[1]);
+                    mma16816<T>(o[(n + 1) % kOut], pa, b[2], b[3]);
+                }
             }
             __syncwarp();
         }
@@ -337,36 +443,47 @@ __global__ void __launch_bounds__(kRowThreads, 2) attention_rows(const __grid_co
         // ---- join the warps
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
-            sum[r] += __shfl_xor_sync(~0u, sum[r], 1);
-            sum[r] += __shfl_xor_sync(~0u, sum[r], 2);
-            const int row = lane / 4 + 8 * r;
-            if ((lane & 3) == 0) warp_ml[warp][row] = make_float2(m[r], sum[r]);
+            if (ROWS == 8) {
+                sum[r] += __shfl_xor_sync(~0u, sum[r], 4);
+                sum[r] += __shfl_xor_sync(~0u, sum[r], 8);
+                sum[r] += __shfl_xor_sync(~0u, sum[r], 16);
+                const int row = 2 * (lane & 3) + r;
+                if (lane < 4) warp_ml[warp][row] = make_float2(m[r], sum[r]);
 #pragma unroll
-            for (int n = 0; n < D / 8; ++n)
-                *reinterpret_cast<float2 *>(my_o + row * D + n * 8 + (lane & 3) * 2) =
-                    make_float2(o[n][2 * r], o[n][2 * r + 1]);
+                for (int n = 0; n < kOut; ++n) {
+                    my_o[row * kOutRow + n * 16 + lane / 4] = o[n][r];
+                    my_o[row * kOutRow + n * 16 + lane / 4 + 8] = o[n][r + 2];
+                }
+            } else {
+                sum[r] += __shfl_xor_sync(~0u, sum[r], 1);
+                sum[r] += __shfl_xor_sync(~0u, sum[r], 2);
+                const int row = (lane / 4 + 8 * r) % ROWS;
+                if ((lane & 3) == 0) warp_ml[warp][row] = make_float2(m[r], sum[r]);
+#pragma unroll
+                for (int n = 0; n < kOut; ++n)
+                    *reinterpret_cast<float2 *>(my_o + row * kOutRow + n * 8 + (lane & 3) * 2) =
+                        make_float2(o[n][2 * r], o[n][2 * r + 1]);
+            }
         }
         __syncthreads();
         const bool whole = unit == group_start && n_tiles == work.tiles;
         const int c0 = (int)(group_start / per_cta), c1 = (int)((group_end - 1) / per_cta);
         const int slot = 2 * blockIdx.x + (unit == group_start ? 1 : 0);
         constexpr int kQuads = D / 4;
-        constexpr int kWarpFloats = kRowStages * 2 * kStageBytes / 4;
+        constexpr int kWarpFloats = kStages * 2 * kStageBytes / 4;
         const float *all_o = reinterpret_cast<const float *>(smem);
 
-        // Writes a row's four elements, after joining the parts over a shared prefix.
-        auto finish = [&](int row, int quad, Joined j) {
+        // A row's four elements, done but for a shared prefix: into the output, or as one more part for attention_join.
+        auto finish = [&](int row, int quad, const Joined &j) {
             const int token = q.q0 + (row0 + row) / p.group, head = h * p.group + (row0 + row) % p.group;
-            const int64_t at = (int64_t)token * p.q_heads + head, step = (int64_t)p.num_tokens * p.q_heads;
-            join_parts(j, p.prefix_splits, p.split_ml, p.split_o, kQuads, quad, [&](int i) { return at + i * step; });
-            const float inverse = j.sum == 0.f ? 0.f : 1.f / j.sum;  // a row that sees nothing gets zeros
-            char *out = reinterpret_cast<char *>(p.out + (int64_t)token * p.out_token_stride +
-                                                 (int64_t)head * p.out_head_stride) + quad * 8;
-            *reinterpret_cast<uint2 *>(out) = make_uint2(Pack2<T>::of(j.o.x * inverse, j.o.y * inverse),
-                                                         Pack2<T>::of(j.o.z * inverse, j.o.w * inverse));
+            if (p.prefix_splits > 0) {
+                const int64_t at = ((int64_t)p.prefix_splits * p.num_tokens + token) * p.q_heads + head;
+                reinterpret_cast<float4 *>(p.split_o)[at * kQuads + quad] = j.o;
+                if (quad == 0) p.split_ml[at] = make_float2(j.top, j.sum);
+            } else {
+                write_row<T>(p, token, head, quad, j);
+            }
         };
-
-        if (whole && p.prefix_splits > 0) wait_prerequisites();
         for (int item = tid; item < rows * kQuads; item += kRowThreads) {
             const int row = item / kQuads, quad = item % kQuads;
             Joined j;
@@ -375,7 +492,7 @@ __global__ void __launch_bounds__(kRowThreads, 2) attention_rows(const __grid_co
 #pragma unroll
             for (int w = 0; w < kRowWarps; ++w) {
                 const float f = weight_of(warp_ml[w][row].x, j.top);
-                const float4 x = reinterpret_cast<const float4 *>(all_o + w * kWarpFloats + row * D)[quad];
+                const float4 x = reinterpret_cast<const float4 *>(all_o + w * kWarpFloats + row * kOutRow)[quad];
                 j.sum += f * warp_ml[w][row].y;
                 j.o.x += f * x.x, j.o.y += f * x.y, j.o.z += f * x.z, j.o.w += f * x.w;
             }
@@ -397,7 +514,6 @@ __global__ void __launch_bounds__(kRowThreads, 2) attention_rows(const __grid_co
             __syncthreads();
             if (is_last) {
                 __threadfence();
-                if (p.prefix_splits > 0) wait_prerequisites();
                 for (int item = tid; item < rows * kQuads; item += kRowThreads) {
                     const int row = item / kQuads, quad = item % kQuads;
                     Joined j;
@@ -413,6 +529,23 @@ __global__ void __launch_bounds__(kRowThreads, 2) attention_rows(const __grid_co
     wait_prerequisites();
 }
 
+// Joins each row's parts: attention_tiles' over the shared prefix and attention_rows' over the sequence's own keys.
+constexpr int kJoinThreads = 128;
+
+template <class T, int D>
+__global__ void __launch_bounds__(kJoinThreads) attention_join(const __grid_constant__ AttnParams p) {
+    constexpr int kQuads = D / 4;
+    const int64_t rows = (int64_t)p.num_tokens * p.q_heads;
+    const int64_t item = (int64_t)blockIdx.x * kJoinThreads + threadIdx.x, row = item / kQuads;
+    const int quad = (int)(item % kQuads);
+    launch_dependents();
+    wait_prerequisites();
+    if (row >= rows) return;
+    Joined j;
+    join_parts(j, p.prefix_splits + 1, p.split_ml, p.split_o, kQuads, quad, [&](int i) { return row + i * rows; });
+    write_row<T>(p, (int)(row / p.q_heads), (int)(row % p.q_heads), quad, j);
+}
+
 // ------------------------------------------------------------------------------------------------ host side
 
 constexpr size_t kRowPartials = (size_t)kMaxRowCtas * 2 * kRowTile;
@@ -421,11 +554,8 @@ constexpr size_t kSplitAt = KVX_ATTENTION_ZEROED + kRowPartials * (kMlBytes + kO
 constexpr size_t kWorkspaceBytes = kSplitAt + kSplitRows * (kMlBytes + kOutBytes);
 static_assert(kMaxRowCtas <= kTileCounter && (kTileCounter + 1) * sizeof(int32_t) <= KVX_ATTENTION_ZEROED, "counters");
 
-template <class T, int D>
-int launch_rows(const AttnParams &p, bool mods, const Device &device, cudaStream_t stream) {
-    static AllowedSmem allowed[2];
-    auto kernel = mods ? attention_rows<T, D, true> : attention_rows<T, D, false>;
-    if (int rc = allowed[mods].allow(kernel, row_smem<D>(), device.index)) return rc;
+template <class Kernel>
+int launch(Kernel kernel, const AttnParams &p, int64_t grid, int threads, int smem, cudaStream_t stream) {
     cudaLaunchConfig_t cfg = {};
     cfg.stream = stream;
     cudaLaunchAttribute attr;
@@ -433,12 +563,33 @@ int launch_rows(const AttnParams &p, bool mods, const Device &device, cudaStream
     attr.val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = &attr;
     cfg.numAttrs = 1;
-    cfg.gridDim = dim3((unsigned)std::min(2 * device.sms, kMaxRowCtas));
-    cfg.blockDim = dim3(kRowThreads);
-    cfg.dynamicSmemBytes = row_smem<D>();
+    cfg.gridDim = dim3((unsigned)grid);
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = smem;
     KVX_CUDA(cudaLaunchKernelEx(&cfg, kernel, p));
     count_launch();
     return KVX_OK;
+}
+
+template <class T, int D, int ROWS, bool MODS>
+int launch_rows(const AttnParams &p, const Device &device, cudaStream_t stream) {
+    static AllowedSmem allowed;
+    auto kernel = attention_rows<T, D, ROWS, MODS>;
+    if (int rc = allowed.allow(kernel, row_smem<D, ROWS>(), device.index)) return rc;
+    return launch(kernel, p, std::min(RowShape<ROWS>::kCtas * device.sms, kMaxRowCtas), kRowThreads, row_smem<D, ROWS>(),
+                  stream);
+}
+
+template <class T, int D>
+int launch_rows(const AttnParams &p, int rows, bool mods, const Device &device, cudaStream_t stream) {
+    if (rows <= 8) return mods ? launch_rows<T, D, 8, true>(p, device, stream) : launch_rows<T, D, 8, false>(p, device, stream);
+    return mods ? launch_rows<T, D, 16, true>(p, device, stream) : launch_rows<T, D, 16, false>(p, device, stream);
+}
+
+template <class T, int D>
+int launch_join(const AttnParams &p, cudaStream_t stream) {
+    const int64_t items = (int64_t)p.num_tokens * p.q_heads * (D / 4);
+    return launch(attention_join<T, D>, p, (items + kJoinThreads - 1) / kJoinThreads, kJoinThreads, 0, stream);
 }
 
 }  // namespace
@@ -527,42 +678,46 @@ int kvx_attention(const kvx_attention_args *args, int flags, void *stream) {
     p.rows_limit = INT32_MAX;
     const bool mods = a.softcap > 0.f || a.slopes || !(a.scale > 0.f);
     cudaStream_t s = static_cast<cudaStream_t>(stream);
-    auto rows_kernel = [&]() {
+    const int64_t q_rows = (int64_t)std::max(a.max_q_len, 1) * p.group;  // of the longest sequence and one KV head
+    const int64_t all_rows = (int64_t)a.num_tokens * p.group;
+    auto rows_kernel = [&](int64_t rows) {
+        const int n = rows <= 8 ? 8 : 16;
         if (a.head_dim == 128)
-            return a.dtype == KVX_BF16 ? launch_rows<__nv_bfloat16, 128>(p, mods, device, s)
-                                       : launch_rows<__half, 128>(p, mods, device, s);
-        return a.dtype == KVX_BF16 ? launch_rows<__nv_bfloat16, 64>(p, mods, device, s)
-                                   : launch_rows<__half, 64>(p, mods, device, s);
+            return a.dtype == KVX_BF16 ? launch_rows<__nv_bfloat16, 128>(p, n, mods, device, s)
+                                       : launch_rows<__half, 128>(p, n, mods, device, s);
+        return a.dtype == KVX_BF16 ? launch_rows<__nv_bfloat16, 64>(p, n, mods, device, s)
+                                   : launch_rows<__half, 64>(p, n, mods, device, s);
     };
 
     // ---- which kernel takes what
-    const int64_t q_rows = (int64_t)std::max(a.max_q_len, 1) * p.group;  // of the longest sequence and one KV head
-    const int64_t all_rows = (int64_t)a.num_tokens * p.group;
     // Splits of the keys that fill the device with one CTA per SM, two tiles of keys each at least, as many as the
-    // workspace has room for.
-    auto splits_for = [&](int64_t row_tiles, int64_t keys) {
+    // workspace has room for (beside `more` parts).
+    auto splits_for = [&](int64_t row_tiles, int64_t keys, int more) {
         const int64_t fill = device.sms / std::max<int64_t>(1, row_tiles * a.kv_heads);
         const int64_t tiles = (keys + kTileKeys - 1) / kTileKeys;
         return (int)std::max<int64_t>(
-            1, std::min({fill, (tiles + 1) / 2, kSplitRows / std::max<int64_t>(1, (int64_t)a.num_tokens * a.q_heads)}));
+            1, std::min({fill, (tiles + 1) / 2, kSplitRows / ((int64_t)a.num_tokens * a.q_heads) - more}));
     };
-    if (tile_box(p) == 0) return rows_kernel();
-    if (a.shared_len > 0 && q_rows <= kTileKeys && (int64_t)a.num_tokens * a.q_heads <= kSplitRows) {
-        // A prefix shared by short sequences: all their rows together against it, then each against its own keys.
-        const int splits = splits_for((all_rows + kTileRows - 1) / kTileRows, a.shared_len);
+    if (tile_box(p) == 0) return rows_kernel(q_rows);
+    if (a.shared_len > 0 && q_rows <= kTileKeys && 2 * (int64_t)a.num_tokens * a.q_heads <= kSplitRows) {
+        // A prefix shared by short sequences: all their rows together against it, each against its own keys, both joined.
+        const int splits = splits_for((all_rows + kTileRows - 1) / kTileRows, a.shared_len, 1);
         if (int rc = launch_tiles(p, a.head_dim, a.dtype, mods, true, splits, device, s)) return rc;
         p.prefix_splits = splits;
         p.shared_len = 0;
-        return rows_kernel();
+        if (int rc = rows_kernel(q_rows)) return rc;
+        if (a.head_dim == 128)
+            return a.dtype == KVX_BF16 ? launch_join<__nv_bfloat16, 128>(p, s) : launch_join<__half, 128>(p, s);
+        return a.dtype == KVX_BF16 ? launch_join<__nv_bfloat16, 64>(p, s) : launch_join<__half, 64>(p, s);
     }
-    if (q_rows <= kRowTile) return rows_kernel();
+    if (q_rows <= kRowTile) return rows_kernel(q_rows);
     // Prompt chunks, and beside them (unless every sequence may be one) the sequences of few rows.
     const bool mixed = a.batch > 1 && a.num_tokens < (int64_t)a.batch * a.max_q_len;
-    p.rows_limit = mixed ? kRowTile : 0;
+    p.rows_limit = !mixed ? 0 : p.group <= 8 ? 8 : kRowTile;
     const int64_t row_tiles = std::max<int64_t>(1, all_rows / kTileRows);
-    const int splits = splits_for(row_tiles, (int64_t)a.max_kv_len + a.shared_len);
+    const int splits = splits_for(row_tiles, (int64_t)a.max_kv_len + a.shared_len, 0);
     if (int rc = launch_tiles(p, a.head_dim, a.dtype, mods, false, splits, device, s)) return rc;
-    return mixed ? rows_kernel() : KVX_OK;
+    return mixed ? rows_kernel(p.rows_limit) : KVX_OK;
 }
 
 }  // extern "C"

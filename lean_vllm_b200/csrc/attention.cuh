@@ -31,7 +31,7 @@ struct AttnParams {
     float *partial_o;    // [slot][row of the tile][dim]
     float2 *partial_ml;  // [slot][row of the tile]: running maximum (log2 domain) and sum
     // Partial results of attention_tiles, [split][query token][head]: for rows whose keys it split, and for a shared
-    // prefix, which attention_rows joins in when prefix_splits is above 0.
+    // prefix, behind whose prefix_splits parts attention_rows leaves its own when there are any.
     float *split_o;
     float2 *split_ml;
     int32_t prefix_splits;
@@ -62,6 +62,7 @@ int tile_box(const AttnParams &p);
 
 constexpr int kMaxRowCtas = 1024;       // of attention_rows: a counter and two slots of partial results each
 constexpr int kTileCounter = 8192;      // attention_tiles' counter, on a line of its own
+constexpr int kRowTile = 16;            // rows of attention_rows' widest tile
 constexpr int kTileRows = 256;
 constexpr int kTileKeys = 128;
 constexpr int64_t kSplitRows = 131072;  // rows of partial results the workspace holds
@@ -150,6 +151,18 @@ __device__ __forceinline__ void join_parts(Joined &j, int n, const float2 *ml, c
     }
 }
 
+__device__ __forceinline__ float exp2_fast(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+__device__ __forceinline__ float reciprocal_fast(float x) {
+    float y;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
 template <class T>
 struct Pack2;
 template <>
@@ -166,5 +179,13 @@ struct Pack2<__half> {
         return *reinterpret_cast<uint32_t *>(&v);
     }
 };
+
+// Writes four elements of a finished row; one that sees nothing gets zeros.
+template <class T>
+__device__ __forceinline__ void write_row(const AttnParams &p, int token, int head, int quad, const Joined &j) {
+    const float inverse = j.sum == 0.f ? 0.f : 1.f / j.sum;
+    *reinterpret_cast<uint2 *>(p.out + (int64_t)token * p.out_token_stride + (int64_t)head * p.out_head_stride + quad * 8) =
+        make_uint2(Pack2<T>::of(j.o.x * inverse, j.o.y * inverse), Pack2<T>::of(j.o.z * inverse, j.o.w * inverse));
+}
 
 }  // namespace kvx

@@ -177,18 +177,6 @@ __device__ __forceinline__ void arrive(uint32_t bar) {
     asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
 }
 
-__device__ __forceinline__ float exp2_fast(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
-
-__device__ __forceinline__ float reciprocal_fast(float x) {
-    float y;
-    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
-
 // Two 32-bit operations in one instruction.
 __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
     float2 d;
@@ -824,7 +812,7 @@ constexpr int kJoinRows = 16;
 constexpr int kJoinThreads = 128;
 
 template <class T, int D>
-__global__ void __launch_bounds__(kJoinThreads) attention_join(const __grid_constant__ TileParams t) {
+__global__ void __launch_bounds__(kJoinThreads) attention_join_splits(const __grid_constant__ TileParams t) {
     __shared__ Item shared_item;
     __shared__ int has_item;
     const AttnParams &p = t.a;
@@ -856,10 +844,7 @@ __global__ void __launch_bounds__(kJoinThreads) attention_join(const __grid_cons
         const int64_t at = (int64_t)(item.q.q0 + token) * p.q_heads + head;
         Joined j;
         join_parts(j, t.splits, p.split_ml, p.split_o, kQuads, quad, [&](int i) { return at + i * step; });
-        const float inverse = j.sum == 0.f ? 0.f : 1.f / j.sum;
-        *reinterpret_cast<uint2 *>(p.out + (int64_t)(item.q.q0 + token) * p.out_token_stride +
-                                   (int64_t)head * p.out_head_stride + quad * 8) =
-            make_uint2(Pack2<T>::of(j.o.x * inverse, j.o.y * inverse), Pack2<T>::of(j.o.z * inverse, j.o.w * inverse));
+        write_row<T>(p, item.q.q0 + token, head, quad, j);
     }
 }
 
@@ -938,7 +923,7 @@ int launch_typed(const TileParams &t, bool mods, const Device &device, cudaStrea
     const int64_t grid = std::min<int64_t>(items * t.splits, device.sms);  // one CTA per SM, item after item
     if (int rc = launch(kernel, t, grid, kThreads, Shape<D>::kBytes, stream)) return rc;
     if (t.prefix_only || t.splits == 1) return KVX_OK;
-    return launch(attention_join<T, D>, t, items * (kTileRows / kJoinRows), kJoinThreads, 0, stream);
+    return launch(attention_join_splits<T, D>, t, items * (kTileRows / kJoinRows), kJoinThreads, 0, stream);
 }
 
 }  // namespace
