@@ -23,8 +23,7 @@ using namespace kvx;
 // cut into tiles of 64 tokens; the tiles of all groups of all sequences, counted on the device from the lengths, are
 // dealt out in equal contiguous runs to one wave of CTAs, whatever the lengths. A CTA's run covers whole groups and at
 // most two partial ones; a partial group leaves (m, sum, o) in the workspace, and the CTA that brings the last part joins
-// them in a fixed order (the result does not depend on which one that is). A run is kMinRun tiles at least: below that a
-// part costs more to join than to compute.
+// them in a fixed order (the result does not depend on which one that is).
 //
 // Inside a CTA each of the 4 warps takes its own 16 tokens of every tile with its own running maximum, sum and output,
 // and loads them itself with cp.async into its own ring: no barrier until the group's end.
@@ -36,18 +35,13 @@ constexpr int kRowWarps = 4;
 constexpr int kRowThreads = kRowWarps * 32;
 constexpr int kWarpTokens = 16;
 constexpr int kTileTokens = kRowWarps * kWarpTokens;
-#ifndef STAGES8
-#define STAGES8 2
-#define CTAS8 3
-#define STAGES16 3
-#define MINRUN 1
-#endif
-constexpr int kMinRun = MINRUN;
 
+// Ring stages and CTAs per SM: 12 warps with 2 stages each or, where registers allow 8, with 3: 64 ragged requests take
+// 162 us with 12 x 2 and 175 with 8 x 3, one of 131k tokens 98 and 96.
 template <int ROWS>
 struct RowShape {
-    static constexpr int kStages = ROWS == 8 ? STAGES8 : STAGES16;
-    static constexpr int kCtas = ROWS == 8 ? CTAS8 : 2;  // per SM
+    static constexpr int kStages = ROWS == 8 ? 2 : 3;
+    static constexpr int kCtas = ROWS == 8 ? 3 : 2;
 };
 
 template <int D, int ROWS>
@@ -158,7 +152,7 @@ attention_rows(const __grid_constant__ AttnParams p) {
     __syncthreads();
     int64_t total = 0;
     for (int w = 0; w < kRowWarps; ++w) total += scan[w];
-    const int64_t per_cta = max((int64_t)kMinRun, (total + gridDim.x - 1) / gridDim.x);
+    const int64_t per_cta = max((int64_t)1, (total + gridDim.x - 1) / gridDim.x);
     int64_t unit = (int64_t)blockIdx.x * per_cta;
     const int64_t unit_end = min(total, unit + per_cta);
     if (unit >= unit_end) {
@@ -517,7 +511,7 @@ attention_rows(const __grid_constant__ AttnParams p) {
                 for (int item = tid; item < rows * kQuads; item += kRowThreads) {
                     const int row = item / kQuads, quad = item % kQuads;
                     Joined j;
-                    join_parts(j, c1 - c0 + 1, p.partial_ml, p.partial_o, kQuads, quad,
+                    join_parts<8>(j, c1 - c0 + 1, p.partial_ml, p.partial_o, kQuads, quad,
                                [&](int i) { return (int64_t)(2 * (c0 + i) + (i == 0)) * kRowTile + row; });
                     finish(row, quad, j);
                 }
@@ -529,21 +523,34 @@ attention_rows(const __grid_constant__ AttnParams p) {
     wait_prerequisites();
 }
 
-// Joins each row's parts: attention_tiles' over the shared prefix and attention_rows' over the sequence's own keys.
+// Joins each row's parts, four elements a thread: attention_tiles' splits, or its splits of a shared prefix and
+// attention_rows' part over the sequence's own keys. Rows of sequences that attention_rows took whole have none.
 constexpr int kJoinThreads = 128;
 
 template <class T, int D>
-__global__ void __launch_bounds__(kJoinThreads) attention_join(const __grid_constant__ AttnParams p) {
-    constexpr int kQuads = D / 4;
-    const int64_t rows = (int64_t)p.num_tokens * p.q_heads;
-    const int64_t item = (int64_t)blockIdx.x * kJoinThreads + threadIdx.x, row = item / kQuads;
-    const int quad = (int)(item % kQuads);
-    launch_dependents();
+__global__ void __launch_bounds__(kJoinThreads) attention_join(const __grid_constant__ AttnParams p, int parts, bool mixed) {
+    constexpr uint32_t kQuads = D / 4;
+    const uint32_t rows = (uint32_t)p.num_tokens * p.q_heads;  // at most kSplitRows
+    const uint32_t item = blockIdx.x * kJoinThreads + threadIdx.x, row = item / kQuads, quad = item % kQuads;
+    const int token = (int)(row / (uint32_t)p.q_heads);
     wait_prerequisites();
+    launch_dependents();
     if (row >= rows) return;
+    if (mixed) {
+        int low = 0, high = p.batch;  // the last sequence that starts at or before the token
+        while (high - low > 1) {
+            const int mid = (low + high) / 2;
+            if (p.q_starts[mid] <= token) low = mid;
+            else high = mid;
+        }
+        if ((int64_t)sequence_of(p, low).q_len * p.group <= p.rows_limit) return;
+    }
     Joined j;
-    join_parts(j, p.prefix_splits + 1, p.split_ml, p.split_o, kQuads, quad, [&](int i) { return row + i * rows; });
-    write_row<T>(p, (int)(row / p.q_heads), (int)(row % p.q_heads), quad, j);
+    if (parts <= 2)
+        join_parts<2>(j, parts, p.split_ml, p.split_o, kQuads, quad, [&](int i) { return row + i * rows; });
+    else
+        join_parts<8>(j, parts, p.split_ml, p.split_o, kQuads, quad, [&](int i) { return row + i * rows; });
+    write_row<T>(p, token, (int)(row - token * p.q_heads), quad, j);
 }
 
 // ------------------------------------------------------------------------------------------------ host side
@@ -554,8 +561,9 @@ constexpr size_t kSplitAt = KVX_ATTENTION_ZEROED + kRowPartials * (kMlBytes + kO
 constexpr size_t kWorkspaceBytes = kSplitAt + kSplitRows * (kMlBytes + kOutBytes);
 static_assert(kMaxRowCtas <= kTileCounter && (kTileCounter + 1) * sizeof(int32_t) <= KVX_ATTENTION_ZEROED, "counters");
 
-template <class Kernel>
-int launch(Kernel kernel, const AttnParams &p, int64_t grid, int threads, int smem, cudaStream_t stream) {
+template <class Kernel, class... Args>
+int launch(Kernel kernel, int64_t grid, int threads, int smem, cudaStream_t stream, const Args &...args) {
+    if (grid > 0x7fffffff) return fail(KVX_ERR_INVALID, "more rows than a launch holds");
     cudaLaunchConfig_t cfg = {};
     cfg.stream = stream;
     cudaLaunchAttribute attr;
@@ -566,7 +574,7 @@ int launch(Kernel kernel, const AttnParams &p, int64_t grid, int threads, int sm
     cfg.gridDim = dim3((unsigned)grid);
     cfg.blockDim = dim3(threads);
     cfg.dynamicSmemBytes = smem;
-    KVX_CUDA(cudaLaunchKernelEx(&cfg, kernel, p));
+    KVX_CUDA(cudaLaunchKernelEx(&cfg, kernel, args...));
     count_launch();
     return KVX_OK;
 }
@@ -576,8 +584,8 @@ int launch_rows(const AttnParams &p, const Device &device, cudaStream_t stream) 
     static AllowedSmem allowed;
     auto kernel = attention_rows<T, D, ROWS, MODS>;
     if (int rc = allowed.allow(kernel, row_smem<D, ROWS>(), device.index)) return rc;
-    return launch(kernel, p, std::min(RowShape<ROWS>::kCtas * device.sms, kMaxRowCtas), kRowThreads, row_smem<D, ROWS>(),
-                  stream);
+    return launch(kernel, std::min(RowShape<ROWS>::kCtas * device.sms, kMaxRowCtas), kRowThreads, row_smem<D, ROWS>(),
+                  stream, p);
 }
 
 template <class T, int D>
@@ -587,9 +595,27 @@ int launch_rows(const AttnParams &p, int rows, bool mods, const Device &device, 
 }
 
 template <class T, int D>
-int launch_join(const AttnParams &p, cudaStream_t stream) {
+int launch_join(const AttnParams &p, int parts, bool mixed, cudaStream_t stream) {
     const int64_t items = (int64_t)p.num_tokens * p.q_heads * (D / 4);
-    return launch(attention_join<T, D>, p, (items + kJoinThreads - 1) / kJoinThreads, kJoinThreads, 0, stream);
+    return launch(attention_join<T, D>, (items + kJoinThreads - 1) / kJoinThreads, kJoinThreads, 0, stream, p, parts, mixed);
+}
+
+// How many parts attention_tiles' items are cut into along the keys: more items fill SMs that would idle, but every part
+// of a row is written and read once more. By what both take on B200 (us): a pair of tiles 1.85, an item's ends 1.2, the
+// join 3 and its traffic at 4 TB/s. 200 tokens of 32 heads behind 4k take 67 us in one part, 32 in four; 512 new tokens
+// 16.5 in one, 18.8 in two.
+int choose_splits(int64_t items, int64_t keys, int64_t rows, int head_dim, int sms) {
+    const int64_t tiles = std::max<int64_t>(1, (keys + kTileKeys - 1) / kTileKeys);
+    const double part_bytes = 2.0 * rows * (4 * head_dim + 8);
+    int best = 1;
+    double least = 0;
+    for (int splits = 1; splits <= sms && splits * rows <= kSplitRows && (splits == 1 || 2 * splits <= tiles + 1); ++splits) {
+        const double rounds = (double)((items * splits + sms - 1) / sms);
+        double us = rounds * (1.85 * (double)((tiles + splits - 1) / splits) + 1.2);
+        if (splits > 1) us += 3 + splits * part_bytes / 4e6;
+        if (splits == 1 || us < least) best = splits, least = us;
+    }
+    return best;
 }
 
 }  // namespace
@@ -679,7 +705,6 @@ int kvx_attention(const kvx_attention_args *args, int flags, void *stream) {
     const bool mods = a.softcap > 0.f || a.slopes || !(a.scale > 0.f);
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     const int64_t q_rows = (int64_t)std::max(a.max_q_len, 1) * p.group;  // of the longest sequence and one KV head
-    const int64_t all_rows = (int64_t)a.num_tokens * p.group;
     auto rows_kernel = [&](int64_t rows) {
         const int n = rows <= 8 ? 8 : 16;
         if (a.head_dim == 128)
@@ -689,34 +714,43 @@ int kvx_attention(const kvx_attention_args *args, int flags, void *stream) {
                                    : launch_rows<__half, 64>(p, n, mods, device, s);
     };
 
-    // ---- which kernel takes what
-    // Splits of the keys that fill the device with one CTA per SM, two tiles of keys each at least, as many as the
-    // workspace has room for (beside `more` parts).
-    auto splits_for = [&](int64_t row_tiles, int64_t keys, int more) {
-        const int64_t fill = device.sms / std::max<int64_t>(1, row_tiles * a.kv_heads);
-        const int64_t tiles = (keys + kTileKeys - 1) / kTileKeys;
-        return (int)std::max<int64_t>(
-            1, std::min({fill, (tiles + 1) / 2, kSplitRows / ((int64_t)a.num_tokens * a.q_heads) - more}));
+    auto join = [&](int parts, bool mixed) {
+        if (a.head_dim == 128)
+            return a.dtype == KVX_BF16 ? launch_join<__nv_bfloat16, 128>(p, parts, mixed, s)
+                                       : launch_join<__half, 128>(p, parts, mixed, s);
+        return a.dtype == KVX_BF16 ? launch_join<__nv_bfloat16, 64>(p, parts, mixed, s)
+                                   : launch_join<__half, 64>(p, parts, mixed, s);
     };
+
+    // ---- which kernel takes what
     if (tile_box(p) == 0) return rows_kernel(q_rows);
-    if (a.shared_len > 0 && q_rows <= kTileKeys && 2 * (int64_t)a.num_tokens * a.q_heads <= kSplitRows) {
+    const int64_t rows = (int64_t)a.num_tokens * a.q_heads;
+    const int64_t item_tokens = 2 * (128 / p.group);  // of attention_tiles' items
+    if (a.shared_len > 0 && q_rows <= kTileKeys && 2 * rows <= kSplitRows) {
         // A prefix shared by short sequences: all their rows together against it, each against its own keys, both joined.
-        const int splits = splits_for((all_rows + kTileRows - 1) / kTileRows, a.shared_len, 1);
+        // One item per SM: its parts are a part more of every row either way.
+        const int64_t items = (a.num_tokens + item_tokens - 1) / item_tokens * p.kv_heads;
+        const int64_t tiles = (a.shared_len + kTileKeys - 1) / kTileKeys;
+        const int splits =
+            (int)std::max<int64_t>(1, std::min({device.sms / items, (tiles + 1) / 2, kSplitRows / rows - 1}));
         if (int rc = launch_tiles(p, a.head_dim, a.dtype, mods, true, splits, device, s)) return rc;
         p.prefix_splits = splits;
         p.shared_len = 0;
         if (int rc = rows_kernel(q_rows)) return rc;
-        if (a.head_dim == 128)
-            return a.dtype == KVX_BF16 ? launch_join<__nv_bfloat16, 128>(p, s) : launch_join<__half, 128>(p, s);
-        return a.dtype == KVX_BF16 ? launch_join<__nv_bfloat16, 64>(p, s) : launch_join<__half, 64>(p, s);
+        return join(splits + 1, false);
     }
     if (q_rows <= kRowTile) return rows_kernel(q_rows);
     // Prompt chunks, and beside them (unless every sequence may be one) the sequences of few rows.
     const bool mixed = a.batch > 1 && a.num_tokens < (int64_t)a.batch * a.max_q_len;
     p.rows_limit = !mixed ? 0 : p.group <= 8 ? 8 : kRowTile;
-    const int64_t row_tiles = std::max<int64_t>(1, all_rows / kTileRows);
-    const int splits = splits_for(row_tiles, (int64_t)a.max_kv_len + a.shared_len, 0);
+    int64_t keys = (int64_t)a.max_kv_len + a.shared_len;
+    if (a.window > 0 && !a.prefix_lens) keys = std::min<int64_t>(keys, a.window + item_tokens);
+    const int64_t items = std::min<int64_t>(a.batch * (((int64_t)a.max_q_len + item_tokens - 1) / item_tokens),
+                                            (a.num_tokens + item_tokens - 1) / item_tokens + (a.batch - 1) / 2);
+    const int splits = choose_splits(std::max<int64_t>(1, items) * p.kv_heads, keys, rows, a.head_dim, device.sms);
     if (int rc = launch_tiles(p, a.head_dim, a.dtype, mods, false, splits, device, s)) return rc;
+    if (splits > 1)
+        if (int rc = join(splits, mixed)) return rc;
     return mixed ? rows_kernel(p.rows_limit) : KVX_OK;
 }
 

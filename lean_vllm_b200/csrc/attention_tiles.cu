@@ -195,6 +195,46 @@ __device__ __forceinline__ float2 add2(float2 a, float2 b) {
     return d;
 }
 
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+    float2 d;
+    asm("{\n\t.reg .b64 a, b, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\t"
+        "mul.rn.f32x2 d, a, b;\n\tmov.b64 {%0, %1}, d;\n\t}"
+        : "=f"(d.x), "=f"(d.y)
+        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return d;
+}
+
+// 2^x of two values between -127 (0 below) and 60 (2^60 above) on the multiply-add pipe. x = n + f with n the nearest
+// integer (left in the low bits by adding 1.5 * 2^23) and f in [-1/2, 1/2]; 2^f by a polynomial with p(0) = 1 whose
+// coefficients are a least-maximum fit of the relative error (1e-7); n goes into the exponent. NaN stays not finite.
+__device__ __forceinline__ float2 exp2_polynomial(float2 x) {
+    asm("{\n\tmax.NaN.f32 %0, %0, %1;\n\tmin.NaN.f32 %0, %0, %2;\n\t}" : "+f"(x.x) : "f"(-127.f), "f"(60.f));
+    asm("{\n\tmax.NaN.f32 %0, %0, %1;\n\tmin.NaN.f32 %0, %0, %2;\n\t}" : "+f"(x.y) : "f"(-127.f), "f"(60.f));
+    const float2 shifted = add2(x, make_float2(12582912.f, 12582912.f));
+    const float2 whole = add2(shifted, make_float2(-12582912.f, -12582912.f));
+    const float2 f = fma2(whole, make_float2(-1.f, -1.f), x);
+    float2 y = fma2(f, make_float2(0.0013264727f, 0.0013264727f), make_float2(0.00967151265f, 0.00967151265f));
+    y = fma2(y, f, make_float2(0.0555073374f, 0.0555073374f));
+    y = fma2(y, f, make_float2(0.240222421f, 0.240222421f));
+    y = fma2(y, f, make_float2(0.693146978f, 0.693146978f));
+    y = fma2(y, f, make_float2(1.f, 1.f));
+    return make_float2(__int_as_float(__float_as_int(y.x) + (__float_as_int(shifted.x) << 23)),
+                       __int_as_float(__float_as_int(y.y) + (__float_as_int(shifted.y) << 23)));
+}
+
+// Two scores x to cap tanh(x / cap), times log2(e): tanh(z) = 1 - 2 / (e^2z + 1), so that the error is 1e-7 of the cap,
+// which is what counts in an exponent. The special-function unit gives 16 results a cycle for the CTA's 32,768 scores a
+// pair of tiles, and the weights take one each: the cap takes half a one, a reciprocal for two scores, and has its
+// exponential from the polynomial above.
+__device__ __forceinline__ void capped(float &x, float &y, float cap_in, float cap_out) {
+    const float2 e = exp2_polynomial(mul2(make_float2(x, y), make_float2(cap_in, cap_in)));
+    const float2 d = add2(e, make_float2(1.f, 1.f));
+    const float r = reciprocal_fast(d.x * d.y) * (-2.f * cap_out);
+    const float2 capped = fma2(make_float2(d.y, d.x), make_float2(r, r), make_float2(cap_out, cap_out));
+    x = capped.x;
+    y = capped.y;
+}
+
 __device__ __forceinline__ float max_of(float top, const float (&x)[32]) {
     float a = top, b = x[0];
 #pragma unroll
@@ -428,33 +468,43 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tiles(const __grid_cons
                 }
                 score_phase ^= 1;
                 fence_after();
-                // Scores that a mask, cap or bias changes go back to TMEM as they are then.
+                // Scores that a mask, cap or bias changes go back to TMEM as they are then, 32 columns at a time.
                 const bool sees_all = !valid ? true
                                       : at.shared ? at.t0 + kTileKeys <= p.shared_len
                                                   : (at.t0 >= see_lo && at.t0 + kTileKeys <= see_hi) ||
                                                         at.t0 + kTileKeys <= see_below;
                 const bool masked = !__all_sync(~0u, sees_all);
                 if (MODS || masked) {
-                    const int from = (at.shared ? 0 : see_lo) - at.t0;
-                    const int to = (at.shared ? p.shared_len : see_hi) - at.t0;
-                    const int below = (at.shared ? 0 : see_below) - at.t0;
-                    const float offset = MODS ? (float)((at.shared ? 0 : p.shared_len) + at.t0 - position) : 0.f;
-#pragma unroll
-                    for (int c = 0; c < 4; ++c) {
+                    int from = (at.shared ? 0 : see_lo) - at.t0, to = (at.shared ? p.shared_len : see_hi) - at.t0;
+                    int below = (at.shared ? 0 : see_below) - at.t0;
+                    float offset = MODS ? (float)((at.shared ? 0 : p.shared_len) + at.t0 - position) : 0.f;
+#pragma unroll 1
+                    for (int c = 0; c < 4; ++c, from -= 32, to -= 32, below -= 32, offset += 32.f) {
                         float y[32];
                         load32(s_tmem + c * 32, y);
                         wait_loads();
+                        if (MODS) {  // scores times log2(e)
+                            if (p.softcap > 0.f) {
+                                if (masked) {  // what is not seen may be NaN, and pairs share a reciprocal
 #pragma unroll
-                        for (int e = 0; e < 32; ++e) {
-                            const int k = c * 32 + e;
-                            if (MODS) {  // the score times log2(e)
-                                // tanh(z) = 1 - 2 / (e^2z + 1), to 2^-22 of the cap, where the exponent's error counts
-                                y[e] = p.softcap > 0.f
-                                           ? cap_out - 2.f * cap_out * reciprocal_fast(exp2_fast(y[e] * cap_in) + 1.f)
-                                           : y[e] * scale_log2;
-                                y[e] += slope * (offset + (float)k);
+                                    for (int e = 0; e < 32; ++e)
+                                        if (!((e >= from && e < to) || e < below)) y[e] = 0.f;
+                                }
+#pragma unroll
+                                for (int e = 0; e < 32; e += 2) capped(y[e], y[e + 1], cap_in, cap_out);
+                            } else {
+#pragma unroll
+                                for (int e = 0; e < 32; ++e) y[e] *= scale_log2;
                             }
-                            if (masked && !((k >= from && k < to) || k < below)) y[e] = -INFINITY;
+                            if (p.slopes) {
+#pragma unroll
+                                for (int e = 0; e < 32; ++e) y[e] += slope * (offset + (float)e);
+                            }
+                        }
+                        if (masked) {
+#pragma unroll
+                            for (int e = 0; e < 32; ++e)
+                                if (!((e >= from && e < to) || e < below)) y[e] = -INFINITY;
                         }
                         store32(s_tmem + c * 32, y);
                     }
@@ -807,47 +857,6 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tiles(const __grid_cons
     if (tid == 0 && gave_up) flag_error(p.error_word, p.status, kErrAttentionWait);
 }
 
-// Joins the splits of rows that attention_tiles took, 16 rows per CTA.
-constexpr int kJoinRows = 16;
-constexpr int kJoinThreads = 128;
-
-template <class T, int D>
-__global__ void __launch_bounds__(kJoinThreads) attention_join_splits(const __grid_constant__ TileParams t) {
-    __shared__ Item shared_item;
-    __shared__ int has_item;
-    const AttnParams &p = t.a;
-    wait_prerequisites();
-    launch_dependents();
-    constexpr int kParts = kTileRows / kJoinRows;
-    const int part = blockIdx.x % kParts, id = blockIdx.x / kParts;
-    if (threadIdx.x < 32) {
-        Item item;
-        int count;
-        // Item ids count (row tile, split, head); every split holds the same rows.
-        const bool found = find_item(t, id / p.kv_heads * p.kv_heads * t.splits + id % p.kv_heads, item, count);
-        if (threadIdx.x == 0) {
-            has_item = found;
-            if (found) shared_item = item;
-        }
-    }
-    __syncthreads();
-    if (!has_item) return;
-    const Item &item = shared_item;
-    constexpr int kQuads = D / 4;
-    const int64_t step = (int64_t)p.num_tokens * p.q_heads;
-    for (int k = threadIdx.x; k < kJoinRows * kQuads; k += kJoinThreads) {
-        const int r = part * kJoinRows + k / kQuads, quad = k % kQuads;
-        const int in_tile = (r & 127) / p.group, in_item = (r >> 7) * t.tile_tokens + in_tile;
-        if (in_tile >= t.tile_tokens || in_item >= item.tokens) continue;
-        const int token = item.token0 + in_item;
-        const int head = item.head * p.group + (r & 127) - in_tile * p.group;
-        const int64_t at = (int64_t)(item.q.q0 + token) * p.q_heads + head;
-        Joined j;
-        join_parts(j, t.splits, p.split_ml, p.split_o, kQuads, quad, [&](int i) { return at + i * step; });
-        write_row<T>(p, item.q.q0 + token, head, quad, j);
-    }
-}
-
 // ------------------------------------------------------------------------------------------------ host side
 
 using EncodeTiled = CUresult (*)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *,
@@ -921,9 +930,7 @@ int launch_typed(const TileParams &t, bool mods, const Device &device, cudaStrea
     if (int rc = allowed[mods].allow(kernel, Shape<D>::kBytes, device.index)) return rc;
     const int64_t items = (int64_t)t.row_tiles * t.a.kv_heads;
     const int64_t grid = std::min<int64_t>(items * t.splits, device.sms);  // one CTA per SM, item after item
-    if (int rc = launch(kernel, t, grid, kThreads, Shape<D>::kBytes, stream)) return rc;
-    if (t.prefix_only || t.splits == 1) return KVX_OK;
-    return launch(attention_join_splits<T, D>, t, items * (kTileRows / kJoinRows), kJoinThreads, 0, stream);
+    return launch(kernel, t, grid, kThreads, Shape<D>::kBytes, stream);
 }
 
 }  // namespace

@@ -247,11 +247,6 @@ __device__ __forceinline__ void rotate(float (&a)[4], float (&b)[4], const float
     }
 }
 
-// Where destination 0 keeps a token, or -1.
-__device__ __forceinline__ int64_t first_offset(const RotateParams &p, int64_t token, int64_t slot) {
-    return p.peers_only ? -1 : dest_offset(p, 0, token, slot);
-}
-
 // PASSES x (32 / LANES) rows of one token and one kind (0 queries, 1 keys, 2 values) from head `head0` on.
 template <class T, int LANES, int PASSES, bool INTERLEAVED>
 __device__ __forceinline__ void rotate_rows(const RotateParams &p, const Rows &rows, int kind, int64_t token, int head0,
