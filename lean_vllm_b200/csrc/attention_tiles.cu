@@ -235,6 +235,30 @@ __device__ __forceinline__ void capped(float &x, float &y, float cap_in, float c
     y = capped.y;
 }
 
+// The same for scores within three quarters of the cap, where tanh(z) / z is a polynomial of z^2 (a least-maximum fit of
+// the relative error, 3e-8): 7 operations for two scores instead of 25. A chunk of 32 columns takes it when all of the
+// warp's scores there are that small, as scores that a cap only guards are; a NaN is not.
+struct NearCap {
+    float c[6], limit;
+    __device__ __forceinline__ NearCap(float scale, float cap) {
+        constexpr float kFit[6] = {1.f, -0.333330684f, 0.133265212f, -0.0533902585f, 0.0196649133f, -0.00476949004f};
+        const float z = cap > 0.f ? scale / cap : 0.f;  // of a score of 1
+        float power = scale * kLog2e;
+#pragma unroll
+        for (int i = 0; i < 6; ++i, power *= z * z) c[i] = kFit[i] * power;
+        limit = z != 0.f ? 0.5625f / (z * z) : 0.f;
+    }
+    __device__ __forceinline__ void cap(float &x, float &y) const {
+        const float2 v = make_float2(x, y), u = mul2(v, v);
+        float2 r = fma2(u, make_float2(c[5], c[5]), make_float2(c[4], c[4]));
+#pragma unroll
+        for (int i = 3; i >= 0; --i) r = fma2(r, u, make_float2(c[i], c[i]));
+        r = mul2(r, v);
+        x = r.x;
+        y = r.y;
+    }
+};
+
 __device__ __forceinline__ float max_of(float top, const float (&x)[32]) {
     float a = top, b = x[0];
 #pragma unroll
@@ -419,6 +443,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tiles(const __grid_cons
         const uint32_t stage = ring + S::kSlots * S::kTileBytes + warp * S::kStageBytes;
         const float scale_log2 = p.scale * kLog2e;
         const float cap_in = p.softcap > 0.f ? scale_log2 * 2.f / p.softcap : 0.f, cap_out = p.softcap * kLog2e;
+        const NearCap near(MODS ? p.scale : 0.f, MODS ? p.softcap : 0.f);
         uint32_t score_phase = 0, output_phase = 0;
         int ring_at = 0;  // tiles of keys walked before this item
         Item item;
@@ -490,8 +515,17 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tiles(const __grid_cons
                                     for (int e = 0; e < 32; ++e)
                                         if (!((e >= from && e < to) || e < below)) y[e] = 0.f;
                                 }
+                                float most = 0.f;
 #pragma unroll
-                                for (int e = 0; e < 32; e += 2) capped(y[e], y[e + 1], cap_in, cap_out);
+                                for (int e = 0; e < 32; e += 2)
+                                    asm("max.f32 %0, %0, %1, %2;" : "+f"(most) : "f"(y[e] * y[e]), "f"(y[e + 1] * y[e + 1]));
+                                if (__all_sync(~0u, most <= near.limit)) {
+#pragma unroll
+                                    for (int e = 0; e < 32; e += 2) near.cap(y[e], y[e + 1]);
+                                } else {
+#pragma unroll
+                                    for (int e = 0; e < 32; e += 2) capped(y[e], y[e + 1], cap_in, cap_out);
+                                }
                             } else {
 #pragma unroll
                                 for (int e = 0; e < 32; ++e) y[e] *= scale_log2;
