@@ -3,9 +3,11 @@ step can bear."""
 
 from __future__ import annotations
 
+import ctypes
+
 import torch
 
-from lean_vllm_b200._native import check
+from lean_vllm_b200._native import check, lib
 
 
 def raw_stream(device: int) -> int:
@@ -21,3 +23,26 @@ def call(device: int, function, *args) -> None:
     else:
         with torch.cuda.device(device):
             check(function(*args))
+
+
+def _bind():
+    """The C++ marshalling of the plain calls (csrc/calls.cpp), bound to the library; None where it is not built: the
+    Python wrappers then do the same, slower."""
+    try:
+        from lean_vllm_b200 import _calls
+    except ModuleNotFoundError:
+        return None
+    handle = lib()
+    _calls.bind(ctypes.cast(handle.kvx_attention, ctypes.c_void_p).value,
+                ctypes.cast(handle.kvx_rotate_store, ctypes.c_void_p).value)
+    return _calls
+
+
+_bound: list = []
+
+
+def calls():
+    """The bound module, or None."""
+    if not _bound:
+        _bound.append(_bind())
+    return _bound[0]

@@ -11,8 +11,8 @@ from __future__ import annotations
 import torch
 
 from lean_vllm_b200 import _native
-from lean_vllm_b200._native import lib
-from lean_vllm_b200.attention.device import call, raw_stream
+from lean_vllm_b200._native import check, lib
+from lean_vllm_b200.attention.device import call, calls, raw_stream
 
 _INT32_MAX = 2**31 - 1
 _DTYPES = {torch.bfloat16: _native.BF16, torch.float16: _native.FP16}
@@ -44,6 +44,14 @@ def _int32(name: str, t: torch.Tensor, shape: tuple, device: int) -> int:
 
 def _attention(query, k_cache, v_cache, block_tables, kv_lens, scale, q_starts, max_q_len, max_kv_len, softcap, window,
                slopes, prefix_lens, shared_table, shared_len, out, workspace, stream, flags, status):
+    if out is None and stream is None and workspace is not None and (native := calls()) is not None:
+        done = native.attention(query, k_cache, v_cache, block_tables, kv_lens, scale, q_starts, max_q_len, max_kv_len,
+                                softcap, window, slopes, prefix_lens, shared_table, shared_len, workspace.address,
+                                workspace.index, flags, status)
+        if type(done) is int:
+            check(done)
+        elif done is not None:
+            return done
     shape, cache_shape = query.shape, k_cache.shape
     if len(shape) != 3 or len(cache_shape) != 4 or cache_shape != v_cache.shape:
         raise ValueError(f"queries {tuple(query.shape)} [num_tokens, heads, dim] over caches {tuple(k_cache.shape)} / "

@@ -16,8 +16,8 @@ from dataclasses import dataclass
 import torch
 
 from lean_vllm_b200 import _native
-from lean_vllm_b200._native import lib
-from lean_vllm_b200.attention.device import call, raw_stream
+from lean_vllm_b200._native import check, lib
+from lean_vllm_b200.attention.device import call, calls, raw_stream
 from lean_vllm_b200.attention.kvx_cache import PushTarget, _dest, _slots, _target_slots
 
 _DTYPES = {torch.bfloat16: _native.BF16, torch.float16: _native.FP16}
@@ -160,6 +160,13 @@ def rotate_store_kvcache(query: torch.Tensor, key: torch.Tensor, value: torch.Te
     `status` too) and returns the queries, in `out` when given (which may be `query` itself). Rows may be strided over
     tokens and heads (views into a fused qkv product). A position outside the table takes its nearest row and sets bit
     8 of `status`."""
+    if out is None and stream is None and not push_to and (native := calls()) is not None:
+        done = native.rotate_store(query, key, value, k_cache, v_cache, slot_mapping, positions, rotary.table,
+                                   rotary.interleaved, q_weight, k_weight, eps, flags, status)
+        if type(done) is int:
+            check(done)
+        elif done is not None:
+            return done
     if query.dim() != 3 or key.dim() != 3:
         raise ValueError("queries, keys and values are [num_tokens, heads, dim]")
     num_tokens, num_heads, head_dim = key.shape
@@ -211,6 +218,13 @@ def rotate_store_latents(latent: torch.Tensor, latent_cache: torch.Tensor, slot_
     `slot_mapping` (as store_latents), the leading `rank` elements normed with `weight` (where given) and the last
     rotary_dim rotated, and returns the queries' rotated part `query_pe` [num_tokens, heads, rotary_dim] rotated, in
     `out` when given (None without queries)."""
+    if out is None and stream is None and not push_to and (native := calls()) is not None:
+        done = native.rotate_latents(latent, latent_cache, slot_mapping, positions, rotary.table, rotary.interleaved,
+                                     query_pe, weight, eps, flags, status)
+        if type(done) is int:
+            check(done)
+        elif done is not None:
+            return done if query_pe is not None else None
     if latent.dim() != 2 or latent_cache.dim() != 3 or latent_cache.size(2) != latent.size(1):
         raise ValueError(f"latents {tuple(latent.shape)} into a cache {tuple(latent_cache.shape)}")
     num_tokens, dim = latent.shape

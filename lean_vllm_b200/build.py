@@ -1,4 +1,5 @@
-"""Builds libkvx.so in-tree for sm_100a (B200) with nvcc: `python -m lean_vllm_b200.build`."""
+"""Builds libkvx.so in-tree for sm_100a (B200) with nvcc, and the module that calls it from torch tensors:
+`python -m lean_vllm_b200.build`."""
 
 from __future__ import annotations
 
@@ -6,6 +7,7 @@ import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 import tempfile
 
 HERE = os.path.dirname(os.path.abspath(__file__))
@@ -15,6 +17,8 @@ SOURCES = [os.path.join(CSRC, name) for name in ("kvx.cu", "rotary.cu", "attenti
 HEADERS = [os.path.join(ROOT, "include", "kvx.h"),
            *(os.path.join(CSRC, name) for name in sorted(os.listdir(CSRC)) if name.endswith(".cuh"))]
 OUTPUT = os.path.join(HERE, "libkvx.so")
+CALLS_SOURCE = os.path.join(CSRC, "calls.cpp")
+CALLS = os.path.join(HERE, "_calls" + sysconfig.get_config_var("EXT_SUFFIX"))
 
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",
@@ -31,14 +35,34 @@ def nvcc() -> str:
     return path
 
 
-def stale() -> bool:
-    if not os.path.exists(OUTPUT):
+def stale(output: str = OUTPUT, sources: list[str] | None = None) -> bool:
+    if not os.path.exists(output):
         return True
-    built = os.path.getmtime(OUTPUT)
-    return any(os.path.getmtime(f) > built for f in SOURCES + HEADERS)
+    built = os.path.getmtime(output)
+    return any(os.path.getmtime(f) > built for f in (sources or SOURCES + HEADERS))
+
+
+def build_calls(force: bool = False) -> str:
+    """The binding of the calls a decode step makes per layer (csrc/calls.cpp), with g++ against torch's headers."""
+    if not force and not stale(CALLS, [CALLS_SOURCE, HEADERS[0]]):
+        return CALLS
+    from torch.utils import cpp_extension
+    import torch
+
+    cuda = os.path.dirname(os.path.dirname(nvcc()))
+    includes = [*cpp_extension.include_paths(), sysconfig.get_paths()["include"], os.path.join(cuda, "include"),
+                os.path.join(ROOT, "include")]
+    libraries = cpp_extension.library_paths()
+    cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}",
+           *(f"-I{i}" for i in includes), "-o", CALLS + ".tmp", CALLS_SOURCE, *(f"-L{d}" for d in libraries),
+           "-lc10", "-ltorch_cpu", "-lc10_cuda", "-ltorch_python"]
+    subprocess.run(cmd, check=True)
+    os.replace(CALLS + ".tmp", CALLS)
+    return CALLS
 
 
 def build(force: bool = False, verbose: bool = False) -> str:
+    build_calls(force)
     if not force and not stale():
         return OUTPUT
     # One object per source, compiled side by side, then linked; objects are rebuilt together with the library.

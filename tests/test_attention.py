@@ -4,6 +4,7 @@ the rotary table's angles."""
 import ctypes
 import math
 import os
+from concurrent.futures import ThreadPoolExecutor
 
 import pytest
 import torch
@@ -129,6 +130,12 @@ def test_shared_prefix_attention_refuses():
                                 args["block_tables"], args["kv_lens"])
 
 
+def in_a_thread(fn):
+    """fn(), in a thread of its own: the library's last error is per thread, and other tests look at this one's."""
+    with ThreadPoolExecutor(1) as pool:
+        return pool.submit(fn).result()
+
+
 def attention_struct(**change):
     fields = dict(query=16, q_token_stride=512, q_head_stride=128, out=16, out_token_stride=512, out_head_stride=128,
                   k_cache=16, v_cache=16, block_stride=4096, token_stride=256, head_stride=128, block_tables=16,
@@ -163,7 +170,8 @@ def test_the_abi_refuses_attention_arguments(change, message):
     if not os.path.exists(_native.LIB_PATH):
         pytest.skip("libkvx.so is not built here")
     with pytest.raises(_native.KvxError, match=message):
-        _native.check(_native.lib().kvx_attention(ctypes.addressof(struct := attention_struct(**change)), 0, None))
+        struct = attention_struct(**change)
+        in_a_thread(lambda: _native.check(_native.lib().kvx_attention(ctypes.addressof(struct), 0, None)))
 
 
 def test_the_abi_refuses_rotate_arguments():
@@ -180,7 +188,8 @@ def test_the_abi_refuses_rotate_arguments():
                       rotary_dim=64, position_bytes=8, num_tokens=4, eps=1e-6)
         fields.update(change)
         args = _native.RotateArgs(**fields)
-        _native.check(lib.kvx_rotate_store(ctypes.addressof(args), ctypes.addressof(dests), n, None, 0, None))
+        in_a_thread(lambda: _native.check(lib.kvx_rotate_store(ctypes.addressof(args), ctypes.addressof(dests), n, None, 0,
+                                                               None)))
 
     for change, message in [
         (dict(dtype=9), "element type 9"), (dict(num_tokens=-1), "-1 tokens"), (dict(rotary_dim=7), "not an even"),
@@ -260,3 +269,26 @@ def test_rotary_angles():
             RotaryTable.build(4, 8, scaling=bad, device="cpu")
     with pytest.raises(ValueError, match="rotary_dim 7"):
         RotaryTable.build(4, 7, device="cpu")
+
+
+def test_the_native_marshalling_loads_and_leaves_the_rest_to_the_wrappers():
+    """Where it is built, the C++ module imports, binds, and answers None to what is not a plain call (CPU tensors)."""
+    from lean_vllm_b200 import build
+
+    if not os.path.exists(build.CALLS) or not os.path.exists(_native.LIB_PATH):
+        pytest.skip("not built here")
+    from lean_vllm_b200.attention.device import calls
+
+    native = calls()
+    a = attention_args()
+    plain = (a["query"], a["k_cache"], a["v_cache"], a["block_tables"], a["kv_lens"], None, None, 1, 32, 0.0, 0, None,
+             None, None, 0, 4096, 0, 0, 0)
+    assert native.attention(*plain) is None
+    for wrong in ((), plain[:-1], (None,) * 19, (*plain[:5], "x", *plain[6:]), (*plain[:7], 2**70, *plain[8:])):
+        assert native.attention(*wrong) is None
+    s = store_args()
+    assert native.rotate_store(s["query"], s["key"], s["value"], s["k_cache"], s["v_cache"], s["slot_mapping"],
+                               s["positions"], s["rotary"].table, False, None, None, 1e-6, 0, 0) is None
+    assert native.rotate_store(*[None] * 14) is None and native.rotate_latents(*[3] * 11) is None
+    with pytest.raises(TypeError):
+        native.bind(1)
