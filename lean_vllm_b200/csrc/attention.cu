@@ -92,6 +92,12 @@ __device__ __forceinline__ uint32_t transpose8(uint32_t x) {
     return y;
 }
 
+// a / b for what nearly always fits 32 bits: a 64-bit division takes 400 cycles of a walk's 3000.
+__device__ __forceinline__ int64_t quotient(int64_t a, int64_t b) {
+    if (((uint64_t)a | (uint64_t)b) >> 32 == 0) return (int64_t)((uint32_t)a / (uint32_t)b);
+    return a / b;
+}
+
 // A sequence's share of the launch's tiles.
 struct RowWork {
     int32_t lo, row_tiles, tiles;  // first key, tiles of rows, tiles of keys per group
@@ -118,13 +124,6 @@ __device__ __forceinline__ int64_t row_units(const AttnParams &p, int s) {
     return w.groups(p) * w.tiles;
 }
 
-// The address of query row `row` (query token row / group, head row % group of KV head h) in a [token][head] tensor.
-__device__ __forceinline__ uint64_t row_address(const AttnParams &p, uint64_t base, int64_t token_stride,
-                                                int64_t head_stride, const Sequence &q, int h, int row) {
-    const int token = row / p.group;
-    return base + (int64_t)(q.q0 + token) * token_stride + (int64_t)(h * p.group + row - token * p.group) * head_stride;
-}
-
 template <class T, int D, int ROWS, bool MODS>
 __global__ void __launch_bounds__(kRowThreads, RowShape<ROWS>::kCtas)
 attention_rows(const __grid_constant__ AttnParams p) {
@@ -144,15 +143,16 @@ attention_rows(const __grid_constant__ AttnParams p) {
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
 
     // ---- this CTA's run of tiles
-    int64_t mine = 0;
-    for (int s = tid; s < p.batch; s += kRowThreads) mine += row_units<ROWS>(p, s);
+    const int64_t own_units = tid < p.batch ? row_units<ROWS>(p, tid) : 0;  // of the first sequences, all there are often
+    int64_t mine = own_units;
+    for (int s = tid + kRowThreads; s < p.batch; s += kRowThreads) mine += row_units<ROWS>(p, s);
 #pragma unroll
     for (int o = 16; o; o >>= 1) mine += __shfl_xor_sync(~0u, mine, o);
     if (lane == 0) scan[warp] = mine;
     __syncthreads();
     int64_t total = 0;
     for (int w = 0; w < kRowWarps; ++w) total += scan[w];
-    const int64_t per_cta = max((int64_t)1, (total + gridDim.x - 1) / gridDim.x);
+    const int64_t per_cta = max((int64_t)1, quotient(total + gridDim.x - 1, gridDim.x));
     int64_t unit = (int64_t)blockIdx.x * per_cta;
     const int64_t unit_end = min(total, unit + per_cta);
     if (unit >= unit_end) {
@@ -162,7 +162,8 @@ attention_rows(const __grid_constant__ AttnParams p) {
     int64_t before = 0;  // tiles of the sequences looked at so far
     for (int s0 = 0;; s0 += kRowThreads) {
         const int s = s0 + tid;
-        int64_t n = s < p.batch ? row_units<ROWS>(p, s) : 0, sum = n;
+        const int64_t n = s0 == 0 ? own_units : s < p.batch ? row_units<ROWS>(p, s) : 0;
+        int64_t sum = n;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
             const int64_t up = __shfl_up_sync(~0u, sum, o);
@@ -205,20 +206,27 @@ attention_rows(const __grid_constant__ AttnParams p) {
     while (unit < unit_end) {
         const Sequence q = sequence_of(p, s);
         const RowWork work = row_work<ROWS>(p, q);
-        const int64_t s_end = s_start + row_units<ROWS>(p, s);
+        const bool taken = (int64_t)q.q_len * p.group <= p.rows_limit;
+        const int64_t s_end = taken ? s_start + work.groups(p) * work.tiles : s_start;
         if (unit >= s_end) {
             s_start = s_end;
             ++s;
             continue;
         }
         const int64_t in_sequence = unit - s_start;
-        const int64_t group_index = in_sequence / work.tiles;
+        const int64_t group_index = quotient(in_sequence, work.tiles);
         const int tile0 = (int)(in_sequence - group_index * work.tiles);
-        const int h = (int)(group_index / work.row_tiles);
+        const int h = (int)(work.row_tiles == 1 ? group_index : quotient(group_index, work.row_tiles));
         const int row0 = (int)(group_index - (int64_t)h * work.row_tiles) * ROWS;
         const int64_t group_start = s_start + group_index * work.tiles, group_end = group_start + work.tiles;
         const int n_tiles = (int)(min(unit_end, group_end) - unit);
         const int rows = min(ROWS, q.q_len * p.group - row0);
+        auto token_of = [&](int row) { return q.q_len == 1 ? 0 : (row0 + row) / p.group; };  // of the tile's rows
+        auto head_of = [&](int row) { return h * p.group + row0 + row - token_of(row) * p.group; };
+        auto query_of = [&](int row) -> uint64_t {
+            if (row >= rows) return 0;
+            return p.query + (int64_t)(q.q0 + token_of(row)) * p.q_token_stride + (int64_t)head_of(row) * p.q_head_stride;
+        };
         const int first_token = work.lo / kTileTokens * kTileTokens + tile0 * kTileTokens + warp * kWarpTokens;
         const int64_t lane_from = (int64_t)h * p.head_stride +
                                   (stage_in_block ? (lane / kChunks) * p.token_stride + (lane % kChunks) * 16 : 0);
@@ -270,7 +278,7 @@ attention_rows(const __grid_constant__ AttnParams p) {
         uint32_t qf[D / 16][kQueryRegs];
         if (ROWS == 8) {  // row lane / 4 as a column
             const int row = lane / 4;
-            const uint64_t at = row < rows ? row_address(p, p.query, p.q_token_stride, p.q_head_stride, q, h, row0 + row) : 0;
+            const uint64_t at = query_of(row);
 #pragma unroll
             for (int k = 0; k < D / 16; ++k)
 #pragma unroll
@@ -280,8 +288,7 @@ attention_rows(const __grid_constant__ AttnParams p) {
 #pragma unroll
             for (int r = 0; r < 2; ++r) {
                 const int row = lane / 4 + 8 * r;
-                const uint64_t at =
-                    row < rows ? row_address(p, p.query, p.q_token_stride, p.q_head_stride, q, h, row0 + row) : 0;
+                const uint64_t at = query_of(row);
 #pragma unroll
                 for (int k = 0; k < D / 16; ++k)
 #pragma unroll
@@ -296,13 +303,13 @@ attention_rows(const __grid_constant__ AttnParams p) {
         for (int r = 0; r < 2; ++r) {
             const int row = ROWS == 8 ? 2 * (lane & 3) + r : lane / 4 + 8 * r;
             const bool valid = row < rows;
-            position[r] = valid ? q.kv_len - q.q_len + (row0 + row) / p.group : -1;
+            position[r] = valid ? q.kv_len - q.q_len + token_of(row) : -1;
             prefix[r] = valid ? q.prefix : 0;
-            slope[r] = MODS && valid && p.slopes ? p.slopes[h * p.group + (row0 + row) % p.group] * kLog2e : 0.f;
+            slope[r] = MODS && valid && p.slopes ? p.slopes[head_of(row)] * kLog2e : 0.f;
         }
         // Every row of the tile sees the keys from see_lo up to see_hi: whole stages in there need no mask.
-        const int first_position = q.kv_len - q.q_len + row0 / p.group;
-        const int last_position = q.kv_len - q.q_len + (row0 + rows - 1) / p.group;
+        const int first_position = q.kv_len - q.q_len + token_of(0);
+        const int last_position = q.kv_len - q.q_len + token_of(rows - 1);
         const int see_lo = p.window > 0 ? max(work.lo, last_position - p.window + 1) : 0;
         const int see_hi = min(q.kv_len, first_position + 1);
 
@@ -461,7 +468,6 @@ attention_rows(const __grid_constant__ AttnParams p) {
         }
         __syncthreads();
         const bool whole = unit == group_start && n_tiles == work.tiles;
-        const int c0 = (int)(group_start / per_cta), c1 = (int)((group_end - 1) / per_cta);
         const int slot = 2 * blockIdx.x + (unit == group_start ? 1 : 0);
         constexpr int kQuads = D / 4;
         constexpr int kWarpFloats = kStages * 2 * kStageBytes / 4;
@@ -469,7 +475,7 @@ attention_rows(const __grid_constant__ AttnParams p) {
 
         // A row's four elements, done but for a shared prefix: into the output, or as one more part for attention_join.
         auto finish = [&](int row, int quad, const Joined &j) {
-            const int token = q.q0 + (row0 + row) / p.group, head = h * p.group + (row0 + row) % p.group;
+            const int token = q.q0 + token_of(row), head = head_of(row);
             if (p.prefix_splits > 0) {
                 const int64_t at = ((int64_t)p.prefix_splits * p.num_tokens + token) * p.q_heads + head;
                 reinterpret_cast<float4 *>(p.split_o)[at * kQuads + quad] = j.o;
@@ -499,9 +505,10 @@ attention_rows(const __grid_constant__ AttnParams p) {
         }
         if (!whole) {
             // ---- the group's last part to arrive joins all of them
-            __threadfence();
+            const int c0 = (int)quotient(group_start, per_cta), c1 = (int)quotient(group_end - 1, per_cta);
             __syncthreads();
             if (tid == 0) {
+                __threadfence();  // orders what the barrier made this thread's to know, the other threads' writes
                 is_last = atomicAdd(&p.counters[c0], 1) == c1 - c0;
                 if (is_last) p.counters[c0] = 0;  // for the next launch
             }
