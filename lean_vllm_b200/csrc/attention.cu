@@ -611,13 +611,13 @@ int launch_join(const AttnParams &p, int parts, bool mixed, cudaStream_t stream)
 // of a row is written and read once more. By what both take on B200 (us): a pair of tiles 1.85, an item's ends 1.2, the
 // join 3 and its traffic at 4 TB/s. 200 tokens of 32 heads behind 4k take 67 us in one part, 32 in four; 512 new tokens
 // 16.5 in one, 18.8 in two.
-int choose_splits(int64_t items, int64_t keys, int64_t rows, int head_dim, int sms) {
+int choose_splits(int64_t items, int64_t keys, int64_t rows, int head_dim, int ctas) {
     const int64_t tiles = std::max<int64_t>(1, (keys + kTileKeys - 1) / kTileKeys);
     const double part_bytes = 2.0 * rows * (4 * head_dim + 8);
     int best = 1;
     double least = 0;
-    for (int splits = 1; splits <= sms && splits * rows <= kSplitRows && (splits == 1 || 2 * splits <= tiles + 1); ++splits) {
-        const double rounds = (double)((items * splits + sms - 1) / sms);
+    for (int splits = 1; splits <= ctas && splits * rows <= kSplitRows && (splits == 1 || 2 * splits <= tiles + 1); ++splits) {
+        const double rounds = (double)((items * splits + ctas - 1) / ctas);
         double us = rounds * (1.85 * (double)((tiles + splits - 1) / splits) + 1.2);
         if (splits > 1) us += 3 + splits * part_bytes / 4e6;
         if (splits == 1 || us < least) best = splits, least = us;
@@ -732,15 +732,18 @@ int kvx_attention(const kvx_attention_args *args, int flags, void *stream) {
     // ---- which kernel takes what
     if (tile_box(p) == 0) return rows_kernel(q_rows);
     const int64_t rows = (int64_t)a.num_tokens * a.q_heads;
-    const int64_t item_tokens = 2 * (128 / p.group);  // of attention_tiles' items
+    // attention_tiles' items: two tiles of rows on one CTA per SM or, where one tile holds all rows there are, one on two.
+    const int64_t tile_tokens = 128 / p.group;
     if (a.shared_len > 0 && q_rows <= kTileKeys && 2 * rows <= kSplitRows) {
         // A prefix shared by short sequences: all their rows together against it, each against its own keys, both joined.
-        // One item per SM: its parts are a part more of every row either way.
+        // One item per CTA: its parts are a part more of every row either way.
+        const int groups = a.num_tokens <= tile_tokens ? 1 : 2;
+        const int64_t item_tokens = groups * tile_tokens, ctas = (int64_t)device.sms * (3 - groups);
         const int64_t items = (a.num_tokens + item_tokens - 1) / item_tokens * p.kv_heads;
         const int64_t tiles = (a.shared_len + kTileKeys - 1) / kTileKeys;
         const int splits =
-            (int)std::max<int64_t>(1, std::min({device.sms / items, (tiles + 1) / 2, kSplitRows / rows - 1}));
-        if (int rc = launch_tiles(p, a.head_dim, a.dtype, mods, true, splits, device, s)) return rc;
+            (int)std::max<int64_t>(1, std::min({ctas / items, (tiles + 1) / 2, kSplitRows / rows - 1}));
+        if (int rc = launch_tiles(p, a.head_dim, a.dtype, mods, true, groups, splits, device, s)) return rc;
         p.prefix_splits = splits;
         p.shared_len = 0;
         if (int rc = rows_kernel(q_rows)) return rc;
@@ -750,12 +753,14 @@ int kvx_attention(const kvx_attention_args *args, int flags, void *stream) {
     // Prompt chunks, and beside them (unless every sequence may be one) the sequences of few rows.
     const bool mixed = a.batch > 1 && a.num_tokens < (int64_t)a.batch * a.max_q_len;
     p.rows_limit = !mixed ? 0 : p.group <= 8 ? 8 : kRowTile;
+    const int groups = a.max_q_len <= tile_tokens ? 1 : 2;
+    const int64_t item_tokens = groups * tile_tokens;
     int64_t keys = (int64_t)a.max_kv_len + a.shared_len;
     if (a.window > 0 && !a.prefix_lens) keys = std::min<int64_t>(keys, a.window + item_tokens);
     const int64_t items = std::min<int64_t>(a.batch * (((int64_t)a.max_q_len + item_tokens - 1) / item_tokens),
                                             (a.num_tokens + item_tokens - 1) / item_tokens + (a.batch - 1) / 2);
-    const int splits = choose_splits(std::max<int64_t>(1, items) * p.kv_heads, keys, rows, a.head_dim, device.sms);
-    if (int rc = launch_tiles(p, a.head_dim, a.dtype, mods, false, splits, device, s)) return rc;
+    const int splits = choose_splits(std::max<int64_t>(1, items) * p.kv_heads, keys, rows, a.head_dim, device.sms * (3 - groups));
+    if (int rc = launch_tiles(p, a.head_dim, a.dtype, mods, false, groups, splits, device, s)) return rc;
     if (splits > 1)
         if (int rc = join(splits, mixed)) return rc;
     return mixed ? rows_kernel(p.rows_limit) : KVX_OK;

@@ -53,9 +53,9 @@ struct AllowedSmem {
 };
 
 // attention_tiles (attention_tiles.cu). `prefix_only`: all query rows against the shared prefix alone; else each
-// sequence's rows above rows_limit. It leaves `splits` parts to join, and finished rows when there is one split and it is
+// sequence's rows above rows_limit. `groups`: tiles of rows per CTA, 1 or 2. It leaves `splits` parts to join, and finished rows when there is one split and it is
 // not prefix_only.
-int launch_tiles(const AttnParams &p, int head_dim, int dtype, bool mods, bool prefix_only, int splits,
+int launch_tiles(const AttnParams &p, int head_dim, int dtype, bool mods, bool prefix_only, int groups, int splits,
                  const Device &device, cudaStream_t stream);
 // The tokens of this cache that one of attention_tiles' copies brings; 0 if it cannot take the call (blocks that are no
 // multiple of 8 tokens, strides that no tensor map holds, groups beyond a tile's rows).

@@ -8,6 +8,10 @@
 // pair of tiles, S = Q K^T and O += P V are one chain of tcgen05.mma each, 128 x 128 x D and 128 x D x 128, with Q, K and
 // V in shared memory and S, P and O in TMEM (S, then P in its place, 128 columns a tile; O, D columns a tile).
 //
+// Where an item has no more rows than one tile (a small batch behind a shared prefix, drafted tokens), a CTA has one tile
+// of them and an SM two CTAs: one tile's chain of products and softmax takes 2900 cycles a tile of keys, and would read 22
+// bytes a cycle, what an SM's share of HBM brings at best.
+//
 // Roles. One warp copies K and V tiles by TMA into a ring, one copies the queries, one issues the products, one looks up
 // what to do next; two groups of 4 warps run the softmax of a tile each, one row per thread. While one tile's scores are
 // in the softmax the other's products run, and a CTA takes item after item: the next one's keys and queries arrive and
@@ -28,34 +32,40 @@ namespace {
 
 using namespace kvx;
 
-constexpr int kSoftmaxWarps = 8;
-constexpr int kIssueWarp = 8;
-constexpr int kLoadWarp = 9;
-constexpr int kQueryWarp = 10;
-constexpr int kPlanWarp = 11;
-constexpr int kItemReaders = kSoftmaxWarps + 3;  // warps that read an item
-constexpr int kThreads = 384;
-// The launch gives each thread 168 registers; a row's 128 scores want more, the other warps less:
-// 256 x 224 + 128 x 56 = 64512, the launch's 384 x 168.
-constexpr int kSoftmaxRegisters = 224, kOtherRegisters = 56;
+// Warps of a CTA with GROUPS tiles of rows (two, or one where an item has no more rows): the softmax's, then one each that
+// issues products, copies keys and values, copies queries and looks up items.
+//
+// Registers. A row's 128 scores want more than the launch gives each thread, the other warps less. Two tiles, one CTA per
+// SM: 256 x 224 + 128 x 56 = 64512, the launch's 384 x 168. One tile, two CTAs: 128 x 200 + 128 x 56 = 32768, 256 x 128.
+template <int GROUPS>
+struct Warps {
+    static constexpr int kSoftmax = 4 * GROUPS, kIssue = kSoftmax, kLoad = kSoftmax + 1, kQuery = kSoftmax + 2,
+                         kPlan = kSoftmax + 3, kThreads = 32 * (kSoftmax + 4), kCtas = GROUPS == 2 ? 1 : 2;
+    static constexpr int kItemReaders = kSoftmax + 3;  // warps that read an item
+    static constexpr int kSoftmaxRegisters = GROUPS == 2 ? 224 : 200, kOtherRegisters = 56;
+    static constexpr int kColumns = 256 * GROUPS;      // of TMEM
+};
 constexpr float kLazy = 8.f;
 constexpr uint64_t kWaitNs = 2000000000ull;  // a wait that has not ended after 2 s is an error
 
-template <int D>
+template <int D, int GROUPS>
 struct Shape {
     static constexpr int kHalves = D / 64;                      // 128-byte columns of a row
     static constexpr int kTileBytes = kTileKeys * D * 2;        // of 128 rows: queries, keys or values
     static constexpr int kHalfBytes = kTileKeys * 128;
-    static constexpr int kSlots = D == 128 ? 4 : 8;             // ring of K and V tiles: 128 KB
+    static constexpr int kSlots = (D == 128 ? 2 : 4) * GROUPS;  // ring of K and V tiles: 64 KB a group
     static constexpr int kStageBytes = 32 * 128;                // of a softmax warp: its rows' output on its way out
-    static constexpr int kBytes = (2 + kSlots) * kTileBytes + kSoftmaxWarps * kStageBytes + 1024;
-    static constexpr int kOutColumn = 256;                      // TMEM: S and P of both tiles, then O of both
+    static constexpr int kControlBytes = 1024;                  // barriers and items; the tiles start on 1024 bytes
+    static constexpr int kBytes =
+        kControlBytes + (GROUPS + kSlots) * kTileBytes + Warps<GROUPS>::kSoftmax * kStageBytes;
+    static constexpr int kOutColumn = 128 * GROUPS;             // TMEM: S and P of each tile, then O of each
 };
 
 struct TileParams {
     AttnParams a;
     CUtensorMap keys, values, queries;
     int32_t tile_tokens;  // query tokens of a tile of up to 128 rows
+    int32_t item_tokens;  // and of an item: as many tiles as the CTA has
     int32_t box;          // tokens per copy
     int32_t splits;
     int32_t prefix_only;
@@ -303,14 +313,14 @@ __device__ bool find_item(const TileParams &t, int id, Item &item, int &count) {
         if (id >= count) return false;
         item.sequence = 0;
         item.q = Sequence{0, p.num_tokens, p.shared_len, 0};
-        item.token0 = r * 2 * t.tile_tokens;
-        item.tokens = min(2 * t.tile_tokens, p.num_tokens - item.token0);
+        item.token0 = r * t.item_tokens;
+        item.tokens = min(t.item_tokens, p.num_tokens - item.token0);
         item.lo = item.hi = item.lo_tile = 0;
         item.shared_tiles = (p.shared_len + kTileKeys - 1) / kTileKeys;
         item.tiles = item.shared_tiles;
     } else {
         auto tiles_of = [&](const Sequence &q) {
-            return (int64_t)q.q_len * p.group > p.rows_limit ? (q.q_len + 2 * t.tile_tokens - 1) / (2 * t.tile_tokens) : 0;
+            return (int64_t)q.q_len * p.group > p.rows_limit ? (q.q_len + t.item_tokens - 1) / t.item_tokens : 0;
         };
         auto at = [&](int s) { return s < p.batch ? sequence_of(p, s) : Sequence{0, 0, 0, 0}; };
         Sequence mine = at(lane);  // of the 32 sequences looked at now: all there are, often
@@ -332,7 +342,7 @@ __device__ bool find_item(const TileParams &t, int id, Item &item, int &count) {
             if (here) {
                 const int who = __ffs(here) - 1;
                 item.sequence = s0 + who;
-                item.token0 = (wanted - before - __shfl_sync(~0u, sum - n, who)) * 2 * t.tile_tokens;
+                item.token0 = (wanted - before - __shfl_sync(~0u, sum - n, who)) * t.item_tokens;
                 item.q = Sequence{__shfl_sync(~0u, mine.q0, who), __shfl_sync(~0u, mine.q_len, who),
                                   __shfl_sync(~0u, mine.kv_len, who), __shfl_sync(~0u, mine.prefix, who)};
                 break;
@@ -344,7 +354,7 @@ __device__ bool find_item(const TileParams &t, int id, Item &item, int &count) {
         }
         if (lane == 0 && (int64_t)p.kv_lens[item.sequence] > (int64_t)p.max_blocks * p.block_size)
             flag_error(p.error_word, p.status, kErrPastCache);
-        item.tokens = min(2 * t.tile_tokens, item.q.q_len - item.token0);
+        item.tokens = min(t.item_tokens, item.q.q_len - item.token0);
         // Own keys, counted without the shared prefix, whose rows all see it.
         const int own = item.q.kv_len - p.shared_len;
         const int first = own - item.q.q_len + item.token0, last = first + item.tokens - 1;
@@ -381,21 +391,37 @@ __device__ __forceinline__ TileAt tile_at(const AttnParams &p, const Item &item,
     return at;
 }
 
-template <class T, int D, bool MODS>
-__global__ void __launch_bounds__(kThreads, 1) attention_tiles(const __grid_constant__ TileParams t) {
-    using S = Shape<D>;
-    extern __shared__ unsigned char raw[];
-    __shared__ __align__(8) uint64_t full[S::kSlots], empty[S::kSlots];  // ring: filled by copies, read by products
-    __shared__ __align__(8) uint64_t queries_in, queries_read;
-    __shared__ __align__(8) uint64_t scores[2], weights[2][2], outputs[2];  // by tile of 128 rows (and half of its keys)
-    __shared__ __align__(8) uint64_t item_in[2], item_read[2], drain;
-    __shared__ uint32_t tmem_base;
-    __shared__ int gave_up;
-    __shared__ Item items[2];
+template <int SLOTS>
+struct Control {
+    uint64_t full[SLOTS], empty[SLOTS];  // ring: filled by copies, read by products
+    uint64_t queries_in, queries_read;
+    uint64_t scores[2], weights[2][2], outputs[2];  // by tile of 128 rows (and half of its keys)
+    uint64_t item_in[2], item_read[2], drain;
+    uint32_t tmem_base;
+    int gave_up;
+    Item items[2];
+};
+
+template <class T, int D, int GROUPS, bool MODS>
+__global__ void __launch_bounds__(Warps<GROUPS>::kThreads, Warps<GROUPS>::kCtas)
+attention_tiles(const __grid_constant__ TileParams t) {
+    using S = Shape<D, GROUPS>;
+    using W = Warps<GROUPS>;
+    extern __shared__ __align__(1024) unsigned char raw[];
+    static_assert(sizeof(Control<S::kSlots>) <= S::kControlBytes, "the control block's room");
+    Control<S::kSlots> &control = *reinterpret_cast<Control<S::kSlots> *>(raw);
+    auto &full = control.full, &empty = control.empty;
+    auto &queries_in = control.queries_in, &queries_read = control.queries_read, &drain = control.drain;
+    auto &scores = control.scores, &outputs = control.outputs;
+    auto &weights = control.weights;
+    auto &item_in = control.item_in, &item_read = control.item_read;
+    auto &tmem_base = control.tmem_base;
+    int &gave_up = control.gave_up;
+    auto &items = control.items;
     const AttnParams &p = t.a;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    const uint32_t base = (smem_u32(raw) + 1023) & ~1023u;  // swizzled tiles start on 1024 bytes
-    const uint32_t ring = base + 2 * S::kTileBytes;
+    const uint32_t base = smem_u32(raw) + S::kControlBytes;
+    const uint32_t ring = base + GROUPS * S::kTileBytes;
 
     if (tid == 0) {
         gave_up = 0;
@@ -405,13 +431,14 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tiles(const __grid_cons
         for (int i = 0; i < S::kSlots; ++i) init(&full[i], 1), init(&empty[i], 1);
         for (int i = 0; i < 2; ++i) {
             init(&scores[i], 1), init(&outputs[i], 1), init(&weights[i][0], 128), init(&weights[i][1], 128);
-            init(&item_in[i], 1), init(&item_read[i], kItemReaders);
+            init(&item_in[i], 1), init(&item_read[i], W::kItemReaders);
         }
         init(&queries_in, 1), init(&queries_read, 1), init(&drain, 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    if (warp == kIssueWarp) {
-        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(&tmem_base))
+    if (warp == W::kIssue) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_base)),
+                     "n"(W::kColumns)
                      : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
         fence_before();
@@ -420,8 +447,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tiles(const __grid_cons
     fence_after();
     wait_prerequisites();
     launch_dependents();  // after the wait: what starts now may read all that came before this kernel
-    // All 512 columns there are, so the allocation starts at column 0; the issuing warp counts on it (constants stay out
-    // of its way to the tensor cores).
+    // All 512 columns there are start at column 0, a constant that stays out of the products' way.
     const uint32_t tmem = tmem_base;
 
     // Item n of the CTA, in turn for every warp that reads items; false: there are no more (or a wait ran out).
@@ -432,11 +458,11 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tiles(const __grid_cons
         if (lane == 0) arrive(smem_u32(&item_read[n & 1]));
         return item.valid != 0;
     };
-    auto active_of = [&](const Item &item) { return item.tokens > t.tile_tokens ? 2 : 1; };  // tiles of rows in use
+    auto active_of = [&](const Item &item) { return GROUPS == 2 && item.tokens > t.tile_tokens ? 2 : 1; };  // tiles in use
 
-    if (warp < kSoftmaxWarps) {
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegisters));
-        const int g = warp >> 2, row = tid & 127;
+    if (warp < W::kSoftmax) {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(W::kSoftmaxRegisters));
+        const int g = GROUPS == 2 ? warp >> 2 : 0, row = tid & 127;
         const int row_token = row / p.group, row_head = row - row_token * p.group;
         const uint32_t s_tmem = tmem + ((uint32_t)(warp & 3) << 21) + g * 128;
         const uint32_t o_tmem = tmem + ((uint32_t)(warp & 3) << 21) + S::kOutColumn + g * D;
@@ -681,9 +707,9 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tiles(const __grid_cons
             fence_before();  // the next item's first product overwrites what was read
         }
     } else {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegisters));
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(W::kOtherRegisters));
     }
-    if (warp == kIssueWarp) {
+    if (warp == W::kIssue) {
         // The whole warp walks the loop, one elected lane issues: operands then stay in uniform registers. Issued from
         // a divergent branch, a tile's 16 products took 700 cycles longer.
         constexpr uint32_t score_inst = instruction<T>(kTileKeys, false), output_inst = instruction<T>(D, true);
@@ -692,6 +718,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tiles(const __grid_cons
             if (ok) ok = warp_waits(smem_u32(bar), parity, &gave_up);
             return ok;
         };
+        const uint32_t columns = GROUPS == 2 ? 0 : tmem;
         const uint64_t q_operand = operand(base, 16), k_operand = operand(ring, 16),
                        v_operand = operand(ring, S::kHalfBytes);
         auto score = [&](int g, int slot) {
@@ -702,7 +729,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tiles(const __grid_cons
                 for (int c = 0; c < D / 16; ++c) {
                     constexpr int kHalf = S::kHalfBytes >> 4;
                     const uint32_t step = (c >> 2) * kHalf + (c & 3) * 2;
-                    mma_shared(g * 128, q + step, k + step, score_inst, c > 0);
+                    mma_shared(columns + g * 128, q + step, k + step, score_inst, c > 0);
                 }
                 commit(smem_u32(&scores[g]));
             }
@@ -713,8 +740,8 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tiles(const __grid_cons
             if (elect_one()) {
 #pragma unroll
                 for (int c = 0; c < kTileKeys / 32; ++c)
-                    mma_tensor(S::kOutColumn + g * D, g * 128 + half * 32 + c * 8, v + (uint32_t)(c * (16 * 128 >> 4)),
-                               output_inst, accumulate || c > 0);
+                    mma_tensor(columns + S::kOutColumn + g * D, columns + g * 128 + half * 32 + c * 8,
+                               v + (uint32_t)(c * (16 * 128 >> 4)), output_inst, accumulate || c > 0);
             }
             __syncwarp();
         };
@@ -774,7 +801,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tiles(const __grid_cons
             }
         }
         __syncwarp();
-    } else if (warp == kLoadWarp) {
+    } else if (warp == W::kLoad) {
         // ---- K 0, V 0, K 1, V 1, ... into the ring, one copy of `box` tokens x 64 elements per lane
         const int boxes = kTileKeys / t.box, copies = boxes * S::kHalves;  // at most 32: 8-token boxes, 128-wide heads
         const int half = lane / boxes, box = lane - half * boxes;
@@ -825,7 +852,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tiles(const __grid_cons
                 }
         }
         __syncwarp();
-    } else if (warp == kQueryWarp) {
+    } else if (warp == W::kQuery) {
         // ---- query rows: one copy per tile and 64 columns. Rows past the tokens there are come as zeros or as the next
         // sequence's, those past a tile's whole tokens as whatever was there: each row's scores are its own.
         const int bytes = t.tile_tokens * p.group * 128;  // of a copy
@@ -859,7 +886,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tiles(const __grid_cons
             }
         }
         __syncwarp();
-    } else if (warp == kPlanWarp) {
+    } else if (warp == W::kPlan) {
         // ---- what to do: the CTA's first item by its number, then whichever is next
         int id = blockIdx.x;
         for (int n = 0;; ++n) {
@@ -886,8 +913,8 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tiles(const __grid_cons
     fence_before();
     __syncthreads();
     fence_after();
-    if (warp == kIssueWarp)
-        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
+    if (warp == W::kIssue)
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "n"(W::kColumns) : "memory");
     if (tid == 0 && gave_up) flag_error(p.error_word, p.status, kErrAttentionWait);
 }
 
@@ -957,14 +984,22 @@ int launch(Kernel kernel, const TileParams &t, int64_t grid, int threads, int sm
     return KVX_OK;
 }
 
+template <class T, int D, int GROUPS, bool MODS>
+int launch_typed(const TileParams &t, const Device &device, cudaStream_t stream) {
+    static AllowedSmem allowed;
+    auto kernel = attention_tiles<T, D, GROUPS, MODS>;
+    if (int rc = allowed.allow(kernel, Shape<D, GROUPS>::kBytes, device.index)) return rc;
+    // One wave of CTAs, each taking item after item.
+    const int64_t items = (int64_t)t.row_tiles * t.a.kv_heads * t.splits;
+    const int64_t grid = std::min<int64_t>(items, (int64_t)device.sms * Warps<GROUPS>::kCtas);
+    return launch(kernel, t, grid, Warps<GROUPS>::kThreads, Shape<D, GROUPS>::kBytes, stream);
+}
+
 template <class T, int D>
-int launch_typed(const TileParams &t, bool mods, const Device &device, cudaStream_t stream) {
-    static AllowedSmem allowed[2];
-    auto kernel = mods ? attention_tiles<T, D, true> : attention_tiles<T, D, false>;
-    if (int rc = allowed[mods].allow(kernel, Shape<D>::kBytes, device.index)) return rc;
-    const int64_t items = (int64_t)t.row_tiles * t.a.kv_heads;
-    const int64_t grid = std::min<int64_t>(items * t.splits, device.sms);  // one CTA per SM, item after item
-    return launch(kernel, t, grid, kThreads, Shape<D>::kBytes, stream);
+int launch_typed(const TileParams &t, int groups, bool mods, const Device &device, cudaStream_t stream) {
+    if (groups == 1)
+        return mods ? launch_typed<T, D, 1, true>(t, device, stream) : launch_typed<T, D, 1, false>(t, device, stream);
+    return mods ? launch_typed<T, D, 2, true>(t, device, stream) : launch_typed<T, D, 2, false>(t, device, stream);
 }
 
 }  // namespace
@@ -978,8 +1013,8 @@ int kvx::tile_box(const AttnParams &p) {
     return box >= 8 && strides && p.num_blocks > 0 ? box : 0;
 }
 
-int kvx::launch_tiles(const AttnParams &p, int head_dim, int dtype, bool mods, bool prefix_only, int splits,
-                      const Device &device, cudaStream_t stream) {
+int kvx::launch_tiles(const AttnParams &p, int head_dim, int dtype, bool mods, bool prefix_only, int groups,
+                      int splits, const Device &device, cudaStream_t stream) {
     TileParams t;
     t.a = p;
     t.box = tile_box(p);
@@ -987,14 +1022,14 @@ int kvx::launch_tiles(const AttnParams &p, int head_dim, int dtype, bool mods, b
     t.prefix_only = prefix_only;
     t.next = p.counters + kTileCounter;
     t.tile_tokens = 128 / p.group;
-    const int tokens = 2 * t.tile_tokens;
-    t.row_tiles = (p.num_tokens + tokens - 1) / tokens + (prefix_only ? 0 : p.batch - 1);
+    t.item_tokens = groups * t.tile_tokens;
+    t.row_tiles = (p.num_tokens + t.item_tokens - 1) / t.item_tokens + (prefix_only ? 0 : p.batch - 1);
     if (int rc = cache_map(&t.keys, p, p.k_cache, head_dim, dtype, t.box)) return rc;
     if (int rc = cache_map(&t.values, p, p.v_cache, head_dim, dtype, t.box)) return rc;
     if (int rc = query_map(&t.queries, p, head_dim, dtype, t.tile_tokens)) return rc;
     if (head_dim == 128)
-        return dtype == KVX_BF16 ? launch_typed<__nv_bfloat16, 128>(t, mods, device, stream)
-                                 : launch_typed<__half, 128>(t, mods, device, stream);
-    return dtype == KVX_BF16 ? launch_typed<__nv_bfloat16, 64>(t, mods, device, stream)
-                             : launch_typed<__half, 64>(t, mods, device, stream);
+        return dtype == KVX_BF16 ? launch_typed<__nv_bfloat16, 128>(t, groups, mods, device, stream)
+                                 : launch_typed<__half, 128>(t, groups, mods, device, stream);
+    return dtype == KVX_BF16 ? launch_typed<__nv_bfloat16, 64>(t, groups, mods, device, stream)
+                             : launch_typed<__half, 64>(t, groups, mods, device, stream);
 }
