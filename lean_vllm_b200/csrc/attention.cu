@@ -532,32 +532,48 @@ attention_rows(const __grid_constant__ AttnParams p) {
 
 // Joins each row's parts, four elements a thread: attention_tiles' splits, or its splits of a shared prefix and
 // attention_rows' part over the sequence's own keys. Rows of sequences that attention_rows took whole have none.
+// SPREAD threads share the parts of the same elements, so that many parts of few rows are still read at once (4 requests
+// of 30k tokens and 32 heads over one KV head, 74 parts of 128 rows: 47 us for the call with one thread, 29 with four).
 constexpr int kJoinThreads = 128;
 
-template <class T, int D>
+template <class T, int D, int SPREAD>
 __global__ void __launch_bounds__(kJoinThreads) attention_join(const __grid_constant__ AttnParams p, int parts, bool mixed) {
-    constexpr uint32_t kQuads = D / 4;
+    constexpr uint32_t kQuads = D / 4, kRows = kJoinThreads / (kQuads * SPREAD);
+    __shared__ Joined shares[SPREAD == 1 ? 1 : kJoinThreads];
     const uint32_t rows = (uint32_t)p.num_tokens * p.q_heads;  // at most kSplitRows
-    const uint32_t item = blockIdx.x * kJoinThreads + threadIdx.x, row = item / kQuads, quad = item % kQuads;
+    const uint32_t quad = threadIdx.x % kQuads, share = threadIdx.x / kQuads % SPREAD;
+    const uint32_t row = blockIdx.x * kRows + threadIdx.x / (kQuads * SPREAD);
     const int token = (int)(row / (uint32_t)p.q_heads);
     wait_prerequisites();
     launch_dependents();
-    if (row >= rows) return;
-    if (mixed) {
+    bool wanted = row < rows;
+    if (wanted && mixed) {
         int low = 0, high = p.batch;  // the last sequence that starts at or before the token
         while (high - low > 1) {
             const int mid = (low + high) / 2;
             if (p.q_starts[mid] <= token) low = mid;
             else high = mid;
         }
-        if ((int64_t)sequence_of(p, low).q_len * p.group <= p.rows_limit) return;
+        wanted = (int64_t)sequence_of(p, low).q_len * p.group > p.rows_limit;
     }
     Joined j;
-    if (parts <= 2)
-        join_parts<2>(j, parts, p.split_ml, p.split_o, kQuads, quad, [&](int i) { return row + i * rows; });
-    else
-        join_parts<8>(j, parts, p.split_ml, p.split_o, kQuads, quad, [&](int i) { return row + i * rows; });
-    write_row<T>(p, token, (int)(row - token * p.q_heads), quad, j);
+    if (wanted)
+        join_parts<SPREAD == 1 ? 4 : 8>(j, (parts - (int)share + SPREAD - 1) / SPREAD, p.split_ml, p.split_o, kQuads, quad,
+                                        [&](int i) { return (int64_t)row + (int64_t)(share + i * SPREAD) * rows; });
+    if (SPREAD > 1) {
+        shares[threadIdx.x % (SPREAD == 1 ? 1 : kJoinThreads)] = j;
+        __syncthreads();
+        if (share != 0) return;
+        for (int other = 1; other < SPREAD; ++other) {
+            const Joined &with = shares[(threadIdx.x + other * kQuads) % (SPREAD == 1 ? 1 : kJoinThreads)];
+            const float top = fmaxf(j.top, with.top), mine = weight_of(j.top, top), theirs = weight_of(with.top, top);
+            j.top = top;
+            j.sum = j.sum * mine + with.sum * theirs;
+            j.o.x = j.o.x * mine + with.o.x * theirs, j.o.y = j.o.y * mine + with.o.y * theirs;
+            j.o.z = j.o.z * mine + with.o.z * theirs, j.o.w = j.o.w * mine + with.o.w * theirs;
+        }
+    }
+    if (wanted) write_row<T>(p, token, (int)(row - token * p.q_heads), quad, j);
 }
 
 // ------------------------------------------------------------------------------------------------ host side
@@ -603,8 +619,13 @@ int launch_rows(const AttnParams &p, int rows, bool mods, const Device &device, 
 
 template <class T, int D>
 int launch_join(const AttnParams &p, int parts, bool mixed, cudaStream_t stream) {
-    const int64_t items = (int64_t)p.num_tokens * p.q_heads * (D / 4);
-    return launch(attention_join<T, D>, (items + kJoinThreads - 1) / kJoinThreads, kJoinThreads, 0, stream, p, parts, mixed);
+    const int64_t rows = (int64_t)p.num_tokens * p.q_heads;
+    if (parts > 4) {
+        constexpr int kRows = kJoinThreads / D;  // 4 x D / 4 threads a row
+        return launch(attention_join<T, D, 4>, (rows + kRows - 1) / kRows, kJoinThreads, 0, stream, p, parts, mixed);
+    }
+    constexpr int kRows = 4 * kJoinThreads / D;
+    return launch(attention_join<T, D, 1>, (rows + kRows - 1) / kRows, kJoinThreads, 0, stream, p, parts, mixed);
 }
 
 // How many parts attention_tiles' items are cut into along the keys: more items fill SMs that would idle, but every part
