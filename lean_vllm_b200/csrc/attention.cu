@@ -539,7 +539,8 @@ constexpr int kJoinThreads = 128;
 template <class T, int D, int SPREAD>
 __global__ void __launch_bounds__(kJoinThreads) attention_join(const __grid_constant__ AttnParams p, int parts, bool mixed) {
     constexpr uint32_t kQuads = D / 4, kRows = kJoinThreads / (kQuads * SPREAD);
-    __shared__ Joined shares[SPREAD == 1 ? 1 : kJoinThreads];
+    __shared__ float4 share_o[SPREAD == 1 ? 1 : kJoinThreads];
+    __shared__ float2 share_ml[SPREAD == 1 ? 1 : kJoinThreads];
     const uint32_t rows = (uint32_t)p.num_tokens * p.q_heads;  // at most kSplitRows
     const uint32_t quad = threadIdx.x % kQuads, share = threadIdx.x / kQuads % SPREAD;
     const uint32_t row = blockIdx.x * kRows + threadIdx.x / (kQuads * SPREAD);
@@ -561,16 +562,20 @@ __global__ void __launch_bounds__(kJoinThreads) attention_join(const __grid_cons
         join_parts<SPREAD == 1 ? 4 : 8>(j, (parts - (int)share + SPREAD - 1) / SPREAD, p.split_ml, p.split_o, kQuads, quad,
                                         [&](int i) { return (int64_t)row + (int64_t)(share + i * SPREAD) * rows; });
     if (SPREAD > 1) {
-        shares[threadIdx.x % (SPREAD == 1 ? 1 : kJoinThreads)] = j;
+        const uint32_t place = threadIdx.x % (SPREAD == 1 ? 1 : kJoinThreads);
+        share_o[place] = j.o;
+        share_ml[place] = make_float2(j.top, j.sum);
         __syncthreads();
         if (share != 0) return;
         for (int other = 1; other < SPREAD; ++other) {
-            const Joined &with = shares[(threadIdx.x + other * kQuads) % (SPREAD == 1 ? 1 : kJoinThreads)];
-            const float top = fmaxf(j.top, with.top), mine = weight_of(j.top, top), theirs = weight_of(with.top, top);
+            const uint32_t at = (threadIdx.x + other * kQuads) % (SPREAD == 1 ? 1 : kJoinThreads);
+            const float2 ml = share_ml[at];
+            const float4 o = share_o[at];
+            const float top = fmaxf(j.top, ml.x), mine = weight_of(j.top, top), theirs = weight_of(ml.x, top);
             j.top = top;
-            j.sum = j.sum * mine + with.sum * theirs;
-            j.o.x = j.o.x * mine + with.o.x * theirs, j.o.y = j.o.y * mine + with.o.y * theirs;
-            j.o.z = j.o.z * mine + with.o.z * theirs, j.o.w = j.o.w * mine + with.o.w * theirs;
+            j.sum = j.sum * mine + ml.y * theirs;
+            j.o.x = j.o.x * mine + o.x * theirs, j.o.y = j.o.y * mine + o.y * theirs;
+            j.o.z = j.o.z * mine + o.z * theirs, j.o.w = j.o.w * mine + o.w * theirs;
         }
     }
     if (wanted) write_row<T>(p, token, (int)(row - token * p.q_heads), quad, j);
@@ -620,7 +625,7 @@ int launch_rows(const AttnParams &p, int rows, bool mods, const Device &device, 
 template <class T, int D>
 int launch_join(const AttnParams &p, int parts, bool mixed, cudaStream_t stream) {
     const int64_t rows = (int64_t)p.num_tokens * p.q_heads;
-    if (parts > 4) {
+    if (parts > 4 && rows <= 4096) {  // more rows fill the device with a thread each: 16,384 rows of 5 parts 33 and 65 us
         constexpr int kRows = kJoinThreads / D;  // 4 x D / 4 threads a row
         return launch(attention_join<T, D, 4>, (rows + kRows - 1) / kRows, kJoinThreads, 0, stream, p, parts, mixed);
     }
@@ -778,8 +783,8 @@ int kvx_attention(const kvx_attention_args *args, int flags, void *stream) {
     const int64_t item_tokens = groups * tile_tokens;
     int64_t keys = (int64_t)a.max_kv_len + a.shared_len;
     if (a.window > 0 && !a.prefix_lens) keys = std::min<int64_t>(keys, a.window + item_tokens);
-    const int64_t items = std::min<int64_t>(a.batch * (((int64_t)a.max_q_len + item_tokens - 1) / item_tokens),
-                                            (a.num_tokens + item_tokens - 1) / item_tokens + (a.batch - 1) / 2);
+    int64_t items = a.batch * (((int64_t)a.max_q_len + item_tokens - 1) / item_tokens);
+    if (mixed) items = std::min<int64_t>(items, (a.num_tokens + item_tokens - 1) / item_tokens + (a.batch - 1) / 2);
     const int splits = choose_splits(std::max<int64_t>(1, items) * p.kv_heads, keys, rows, a.head_dim, device.sms * (3 - groups));
     if (int rc = launch_tiles(p, a.head_dim, a.dtype, mods, false, groups, splits, device, s)) return rc;
     if (splits > 1)
