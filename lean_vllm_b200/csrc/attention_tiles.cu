@@ -269,6 +269,9 @@ struct NearCap {
     }
 };
 
+// The lowest n bits, for any n.
+__device__ __forceinline__ uint32_t lowest(int n) { return n >= 32 ? ~0u : n <= 0 ? 0u : (1u << n) - 1; }
+
 __device__ __forceinline__ float max_of(float top, const float (&x)[32]) {
     float a = top, b = x[0];
 #pragma unroll
@@ -533,13 +536,14 @@ attention_tiles(const __grid_constant__ TileParams t) {
                     for (int c = 0; c < 4; ++c, from -= 32, to -= 32, below -= 32, offset += 32.f) {
                         float y[32];
                         load32(s_tmem + c * 32, y);
+                        const uint32_t seen = (lowest(to) & ~lowest(from)) | lowest(below);  // by column
                         wait_loads();
                         if (MODS) {  // scores times log2(e)
                             if (p.softcap > 0.f) {
                                 if (masked) {  // what is not seen may be NaN, and pairs share a reciprocal
 #pragma unroll
                                     for (int e = 0; e < 32; ++e)
-                                        if (!((e >= from && e < to) || e < below)) y[e] = 0.f;
+                                        if (!(seen >> e & 1)) y[e] = 0.f;
                                 }
                                 float most = 0.f;
 #pragma unroll
@@ -564,7 +568,7 @@ attention_tiles(const __grid_constant__ TileParams t) {
                         if (masked) {
 #pragma unroll
                             for (int e = 0; e < 32; ++e)
-                                if (!((e >= from && e < to) || e < below)) y[e] = -INFINITY;
+                                if (!(seen >> e & 1)) y[e] = -INFINITY;
                         }
                         store32(s_tmem + c * 32, y);
                     }
@@ -672,16 +676,20 @@ attention_tiles(const __grid_constant__ TileParams t) {
             if (valid)
                 to = partial ? reinterpret_cast<uint64_t>(p.split_o + split_row * D)
                              : p.out + (int64_t)out_token * p.out_token_stride + (int64_t)head * p.out_head_stride;
+            float all[D / 32][32];
 #pragma unroll
             for (int c = 0; c < D / 32; ++c) {
-                float o[32];
                 if (item.tiles > 0) {
-                    load32(o_tmem + c * 32, o);
-                    wait_loads();
+                    load32(o_tmem + c * 32, all[c]);
                 } else {
 #pragma unroll
-                    for (int e = 0; e < 32; ++e) o[e] = 0.f;
+                    for (int e = 0; e < 32; ++e) all[c][e] = 0.f;
                 }
+            }
+            wait_loads();
+#pragma unroll
+            for (int c = 0; c < D / 32; ++c) {
+                const float(&o)[32] = all[c];
                 if (partial) {
 #pragma unroll
                     for (int e = 0; e < 8; ++e)
