@@ -250,7 +250,8 @@ typedef struct kvx_attention_args {
     void *workspace;            /* kvx_attention_workspace_bytes() of device memory, its first
                                    KVX_ATTENTION_ZEROED bytes zero before its first use; one launch at a time uses it */
     int32_t *status;            /* status word or NULL: bit 2 for a block id past the cache or a length past its table,
-                                   bit 16 for a bounded wait that ran out */
+                                   bit 16 for a bounded wait that ran out: then neither the output nor the workspace
+                                   is to be used any further */
     int32_t shared_len;         /* tokens of the shared prefix */
     int32_t shared_blocks;      /* entries of shared_table */
     int32_t block_size;

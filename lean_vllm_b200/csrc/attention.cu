@@ -3,8 +3,9 @@
 // Mathematics. For a query row at position i, over the keys j that its mask leaves,
 //     s_j = cap(scale q.k_j) + slope (j - i),   o = sum_j 2^(t_j - m) v_j / sum_j 2^(t_j - m),   t_j = s_j log2(e)
 // in one pass with the running maximum m and sum of the softmax. Scores, maxima, sums and the accumulated output are
-// held in 32 bits; the weights 2^(t_j - m) are rounded to the cache's 16-bit type for the tensor cores' second product
-// (each is below 2^0, so the rounding is relative, 2^-9 in bf16, and averages out over the keys).
+// held in 32 bits; the weights 2^(t_j - m) are rounded to the cache's 16-bit type for the tensor cores' second product:
+// a relative rounding of at most 2^-8 in bf16 that averages out over the keys. They are at most 1 (attention_rows) or 2^8
+// (attention_tiles, whose m may lag), far from the type's ends.
 
 #include <algorithm>
 
@@ -27,6 +28,10 @@ using namespace kvx;
 //
 // Inside a CTA each of the 4 warps takes its own 16 tokens of every tile with its own running maximum, sum and output,
 // and loads them itself with cp.async into its own ring: no barrier until the group's end.
+//
+// Bound by HBM: 64 ragged requests of up to 16k tokens (957 MB) take 159 us, 6.0 TB/s; one of 131k 96 us, 5.6 TB/s, of
+// which 10 are the start and the join of 55 parts a head. One request of 317 tokens takes 7.6 us, a chain of waits: the
+// launch, lengths, table, keys (0.5 us each) and the join of 5 parts.
 //
 // Up to 8 rows the products run transposed, S^T = K Q^T and O^T = V^T P^T, with the rows as the tensor cores' 8 columns:
 // half the instructions and registers of a 16-row tile that would be half padding.

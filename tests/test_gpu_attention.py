@@ -241,6 +241,41 @@ def test_strided_queries_and_outputs(workspace):
         assert not wide[:, :3].any() and not wide[:, 9:].any()
 
 
+@pytest.mark.parametrize("q_lens, kv_lens", [([1, 1], [90, 333]), ([40, 200], [90, 333])], ids=["decode", "chunks"])
+def test_block_tables_that_are_views(q_lens, kv_lens, workspace):
+    """A batch's rows of a wider table, as an engine keeps for all its requests."""
+    case = paged_case(q_lens, kv_lens, 8, 2, 128, 16, BF16)
+    wide = torch.full((9, 50), -7, dtype=torch.int32, device="cuda")
+    wide[3:5, : case["tables"].size(1)] = case["tables"]
+    case["tables"] = wide[3:5, : case["tables"].size(1)]
+    check(case, workspace)
+
+
+@pytest.mark.parametrize("q_lens, kv_lens, heads, kv_heads, dim", [
+    ([1, 1], [77, 900], 160, 1, 64),    # more heads on a KV head than a tile has rows
+    ([3, 50], [77, 300], 160, 1, 128),
+    ([2, 100], [20, 130], 72, 1, 64),   # one token a tile of 128 rows
+    ([1, 33], [400, 400], 1, 1, 128),
+])
+def test_large_and_single_groups(q_lens, kv_lens, heads, kv_heads, dim, workspace):
+    check(paged_case(q_lens, kv_lens, heads, kv_heads, dim, 16, BF16), workspace)
+
+
+@pytest.mark.parametrize("scale", [-0.2, 0.0, 2.0])
+def test_any_scale(scale, workspace):
+    for q_lens, kv_lens in (([1, 1], [70, 500]), ([100, 30], [300, 400])):
+        check(paged_case(q_lens, kv_lens, 8, 2, 128, 16, BF16), workspace, scale=scale)
+
+
+def test_a_nan_that_is_seen_shows(workspace):
+    """NaN in a key that every row sees makes every output of its head NaN, and of no other."""
+    for q_lens, options in (([1], {}), ([70], {}), ([70], {"softcap": 5.0}), ([1], {"softcap": 5.0})):
+        case = paged_case(q_lens, [300], 4, 2, 128, 16, BF16)
+        case["k_cache"][int(case["tables"][0, 1]), 5, 1] = math.nan  # position 21, KV head 1
+        out = run(case, workspace, **options)
+        assert torch.isnan(out[:, 2:]).all() and torch.isfinite(out[:, :2]).all()
+
+
 def test_no_tokens_launch_nothing(workspace):
     case = paged_case([1], [5], 4, 2, 64, 16, BF16)
     before = transport.launch_count()
