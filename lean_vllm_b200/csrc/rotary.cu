@@ -175,7 +175,7 @@ __global__ void __launch_bounds__(kAnyThreads) rotate_store_any(const __grid_con
 // reads the token's angles, slot and norm weights once for them. Bound by HBM: a step's rows in and out, once.
 
 constexpr int kFastThreads = 256;
-// One resident wave of 4 CTAs per SM at 64 registers. 8192 tokens of 32 + 8 + 8 heads of 128: 37.5 us (5.48 TB/s); with
+// One resident wave of 4 CTAs per SM at 64 registers. 8192 tokens of 32 + 8 + 8 heads of 128: 37.1 us (5.55 TB/s); with
 // twice as many CTAs 38.5, with a CTA for every 8 units 47; 5 resident CTAs (48 registers) 43.2, 6 with half the loads in
 // flight 54.7.
 constexpr int kFastCtas = 4;
@@ -198,12 +198,12 @@ __device__ __forceinline__ uint32_t pack(float x, float y, __half) {
 template <class T>
 struct Piece {  // four elements
     uint2 bits;
-    __device__ __forceinline__ void get(float (&x)[4]) const {
-        const float2 lo = unpack(bits.x, T()), hi = unpack(bits.y, T());
-        x[0] = lo.x, x[1] = lo.y, x[2] = hi.x, x[3] = hi.y;
+    __device__ __forceinline__ void get(float2 (&x)[2]) const {
+        x[0] = unpack(bits.x, T());
+        x[1] = unpack(bits.y, T());
     }
-    __device__ __forceinline__ void set(const float (&x)[4]) {
-        bits = make_uint2(pack(x[0], x[1], T()), pack(x[2], x[3], T()));
+    __device__ __forceinline__ void set(const float2 (&x)[2]) {
+        bits = make_uint2(pack(x[0].x, x[0].y, T()), pack(x[1].x, x[1].y, T()));
     }
 };
 
@@ -234,17 +234,33 @@ __device__ __forceinline__ Place place_of(int lane_in_row, int rotary_dim) {
     return p;
 }
 
+// Turns the pairs of a and b by the angles whose cos and sin are c and s: two by two in one instruction where they lie in
+// halves.
 template <bool INTERLEAVED>
-__device__ __forceinline__ void rotate(float (&a)[4], float (&b)[4], const float4 &cos4, const float4 &sin4) {
-    const float c[4] = {cos4.x, cos4.y, cos4.z, cos4.w}, s[4] = {sin4.x, sin4.y, sin4.z, sin4.w};
+__device__ __forceinline__ void rotate(float2 (&a)[2], float2 (&b)[2], const float4 &c, const float4 &s) {
+    if (INTERLEAVED) {
+        auto turn = [](float2 &x, float cos, float sin) {
+            x = make_float2(x.x * cos - x.y * sin, x.y * cos + x.x * sin);
+        };
+        turn(a[0], c.x, s.x);
+        turn(a[1], c.y, s.y);
+        turn(b[0], c.z, s.z);
+        turn(b[1], c.w, s.w);
+    } else {
+        const float2 cos[2] = {make_float2(c.x, c.y), make_float2(c.z, c.w)};
+        const float2 sin[2] = {make_float2(s.x, s.y), make_float2(s.z, s.w)};
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        float &x = INTERLEAVED ? (i < 2 ? a[2 * i] : b[2 * i - 4]) : a[i];
-        float &y = INTERLEAVED ? (i < 2 ? a[2 * i + 1] : b[2 * i - 3]) : b[i];
-        const float turned = x * c[i] - y * s[i];
-        y = y * c[i] + x * s[i];
-        x = turned;
+        for (int i = 0; i < 2; ++i) {
+            const float2 minus = make_float2(-sin[i].x, -sin[i].y), x = a[i];
+            a[i] = fma2(b[i], minus, mul2(x, cos[i]));
+            b[i] = fma2(x, sin[i], mul2(b[i], cos[i]));
+        }
     }
+}
+
+__device__ __forceinline__ float squares(const float2 (&a)[2], const float2 (&b)[2]) {
+    const float2 sum = fma2(b[1], b[1], fma2(b[0], b[0], fma2(a[1], a[1], mul2(a[0], a[0]))));
+    return sum.x + sum.y;
 }
 
 // PASSES x (32 / LANES) rows of one token and one kind (0 queries, 1 keys, 2 values) from head `head0` on.
@@ -281,21 +297,20 @@ __device__ __forceinline__ void rotate_rows(const RotateParams &p, const Rows &r
         }
 #pragma unroll
         for (int i = 0; i < PASSES; ++i) {
-            float a[4], b[4];
+            float2 a[2], b[2];
             x[i].get(a);
             y[i].get(b);
             if (normed) {
-                float sum = 0.f;
-#pragma unroll
-                for (int e = 0; e < 4; ++e) sum += a[e] * a[e] + b[e] * b[e];
+                float sum = squares(a, b);
 #pragma unroll
                 for (int o = LANES / 2; o; o >>= 1) sum += __shfl_xor_sync(~0u, sum, o);
                 const float scale = rsqrtf(sum * (1.f / (LANES * 8)) + p.eps);
-                float w[4], v[4];
+                const float2 scales = make_float2(scale, scale);
+                float2 w[2], v[2];
                 weight[0].get(w);
                 weight[1].get(v);
 #pragma unroll
-                for (int e = 0; e < 4; ++e) a[e] = a[e] * scale * w[e], b[e] = b[e] * scale * v[e];
+                for (int e = 0; e < 2; ++e) a[e] = mul2(mul2(a[e], scales), w[e]), b[e] = mul2(mul2(b[e], scales), v[e]);
             }
             if (place.rotated) rotate<INTERLEAVED>(a, b, cos4, sin4);
             x[i].set(a);
@@ -380,10 +395,10 @@ __global__ void __launch_bounds__(kFastThreads) rotate_latents_fast(const __grid
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
                     weight[k][h] = load_piece<T>((uint64_t)p.key.weight + ((k * 64 + h * 32 + lane) * 4) * sizeof(T));
-                    float v[4];
+                    float2 v[2];
                     c[k][h].get(v);
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) sum += v[e] * v[e];
+                    const float2 two = fma2(v[1], v[1], mul2(v[0], v[0]));
+                    sum += two.x + two.y;
                 }
 #pragma unroll
             for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(~0u, sum, o);
@@ -392,16 +407,16 @@ __global__ void __launch_bounds__(kFastThreads) rotate_latents_fast(const __grid
             for (int k = 0; k < CHUNKS; ++k)
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
-                    float v[4], m[4];
+                    float2 v[2], m[2];
                     c[k][h].get(v);
                     weight[k][h].get(m);
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) v[e] = v[e] * scale * m[e];
+                    for (int e = 0; e < 2; ++e) v[e] = mul2(mul2(v[e], make_float2(scale, scale)), m[e]);
                     c[k][h].set(v);
                 }
         }
         if (lane < kLanes) {
-            float a[4], b[4];
+            float2 a[2], b[2];
             x.get(a);
             y.get(b);
             rotate<INTERLEAVED>(a, b, __ldg(reinterpret_cast<const float4 *>(angle) + lane),
