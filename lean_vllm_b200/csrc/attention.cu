@@ -763,18 +763,16 @@ int kvx_attention(const kvx_attention_args *args, int flags, void *stream) {
     // ---- which kernel takes what
     if (tile_box(p) == 0) return rows_kernel(q_rows);
     const int64_t rows = (int64_t)a.num_tokens * a.q_heads;
-    // attention_tiles' items: two tiles of rows on one CTA per SM or, where one tile holds all rows there are, one on two.
     const int64_t tile_tokens = 128 / p.group;
     if (a.shared_len > 0 && q_rows <= kTileKeys && 2 * rows <= kSplitRows) {
         // A prefix shared by short sequences: all their rows together against it, each against its own keys, both joined.
-        // One item per CTA: its parts are a part more of every row either way.
-        const int groups = a.num_tokens <= tile_tokens ? 1 : 2;
-        const int64_t item_tokens = groups * tile_tokens, ctas = (int64_t)device.sms * (3 - groups);
-        const int64_t items = (a.num_tokens + item_tokens - 1) / item_tokens * p.kv_heads;
+        // One item per CTA: its parts are a part more of every row either way. Items of one tile of rows: 64 requests
+        // behind 8192 tokens take 35.9 us, 36.3 with two tiles (64-wide heads: 27.6 and 28.8).
+        const int64_t items = (a.num_tokens + tile_tokens - 1) / tile_tokens * p.kv_heads;
         const int64_t tiles = (a.shared_len + kTileKeys - 1) / kTileKeys;
         const int splits =
-            (int)std::max<int64_t>(1, std::min({ctas / items, (tiles + 1) / 2, kSplitRows / rows - 1}));
-        if (int rc = launch_tiles(p, a.head_dim, a.dtype, mods, true, groups, splits, device, s)) return rc;
+            (int)std::max<int64_t>(1, std::min({2 * device.sms / items, (tiles + 1) / 2, kSplitRows / rows - 1}));
+        if (int rc = launch_tiles(p, a.head_dim, a.dtype, mods, true, 1, splits, device, s)) return rc;
         p.prefix_splits = splits;
         p.shared_len = 0;
         if (int rc = rows_kernel(q_rows)) return rc;
@@ -784,13 +782,27 @@ int kvx_attention(const kvx_attention_args *args, int flags, void *stream) {
     // Prompt chunks, and beside them (unless every sequence may be one) the sequences of few rows.
     const bool mixed = a.batch > 1 && a.num_tokens < (int64_t)a.batch * a.max_q_len;
     p.rows_limit = !mixed ? 0 : p.group <= 8 ? 8 : kRowTile;
-    const int groups = a.max_q_len <= tile_tokens ? 1 : 2;
-    const int64_t item_tokens = groups * tile_tokens;
-    int64_t keys = (int64_t)a.max_kv_len + a.shared_len;
-    if (a.window > 0 && !a.prefix_lens) keys = std::min<int64_t>(keys, a.window + item_tokens);
-    int64_t items = a.batch * (((int64_t)a.max_q_len + item_tokens - 1) / item_tokens);
-    if (mixed) items = std::min<int64_t>(items, (a.num_tokens + item_tokens - 1) / item_tokens + (a.batch - 1) / 2);
-    const int splits = choose_splits(std::max<int64_t>(1, items) * p.kv_heads, keys, rows, a.head_dim, device.sms * (3 - groups));
+    auto items_of = [&](int groups) {  // about how many
+        const int64_t tokens = groups * tile_tokens;
+        int64_t items = a.batch * (((int64_t)a.max_q_len + tokens - 1) / tokens);
+        if (mixed) items = std::min<int64_t>(items, (a.num_tokens + tokens - 1) / tokens + (a.batch - 1) / 2);
+        return std::max<int64_t>(1, items) * p.kv_heads;
+    };
+    auto splits_of = [&](int groups) {
+        int64_t keys = (int64_t)a.max_kv_len + a.shared_len;
+        if (a.window > 0 && !a.prefix_lens) keys = std::min<int64_t>(keys, a.window + groups * tile_tokens);
+        return choose_splits(items_of(groups), keys, rows, a.head_dim, device.sms * (3 - groups));
+    };
+    // Two tiles of rows on one CTA per SM bring the same keys for both; one tile on each of two CTAs lets a few items
+    // spread over more SMs, and the two fall less into step. 128 wide, 32 heads over 8: a prompt of 512 tokens (64 pairs
+    // for 148 SMs) takes 15.8 us in pairs and 14.3 in single tiles, 768 tokens 19.7 and 19.3, 1024 24.1 and 24.6, 2048
+    // 53.2 and 57.0. 64 wide, the single tile is ahead at every size: 13.4 and 11.1, 45.4 and 42.1, 8192 tokens 418 and 389.
+    int groups = 1, splits = 0;
+    if (a.head_dim == 128 && a.max_q_len > tile_tokens) {
+        splits = splits_of(2);
+        if (items_of(2) * splits * 8 > (int64_t)device.sms * 5) groups = 2;
+    }
+    if (groups == 1) splits = splits_of(1);
     if (int rc = launch_tiles(p, a.head_dim, a.dtype, mods, false, groups, splits, device, s)) return rc;
     if (splits > 1)
         if (int rc = join(splits, mixed)) return rc;

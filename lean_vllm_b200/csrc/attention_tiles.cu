@@ -8,9 +8,9 @@
 // pair of tiles, S = Q K^T and O += P V are one chain of tcgen05.mma each, 128 x 128 x D and 128 x D x 128, with Q, K and
 // V in shared memory and S, P and O in TMEM (S, then P in its place, 128 columns a tile; O, D columns a tile).
 //
-// Where an item has no more rows than one tile (a small batch behind a shared prefix, drafted tokens), a CTA has one tile
-// of them and an SM two CTAs: one tile's chain of products and softmax takes 2900 cycles a tile of keys, and would read 22
-// bytes a cycle, what an SM's share of HBM brings at best.
+// Where few items would leave SMs idle, for 64-wide heads and behind a shared prefix (kvx_attention's rule), a CTA has one
+// tile of rows and an SM two CTAs: one tile's chain of products and softmax alone takes 2900 cycles a tile of keys, and
+// would read 22 bytes a cycle, what an SM's share of HBM brings at best.
 //
 // Roles. One warp copies K and V tiles by TMA into a ring, one copies the queries, one issues the products, one looks up
 // what to do next; two groups of 4 warps run the softmax of a tile each, one row per thread. While one tile's scores are
@@ -38,8 +38,7 @@ namespace {
 
 using namespace kvx;
 
-// Warps of a CTA with GROUPS tiles of rows (two, or one where an item has no more rows): the softmax's, then one each that
-// issues products, copies keys and values, copies queries and looks up items.
+// Warps of a CTA with GROUPS tiles of rows (two, or one): the softmax's, then one each that issues products, copies keys and values, copies queries and looks up items.
 //
 // Registers. A row's 128 scores want more than the launch gives each thread, the other warps less. Two tiles, one CTA per
 // SM: 256 x 224 + 128 x 56 = 64512, the launch's 384 x 168. One tile, two CTAs: 128 x 200 + 128 x 56 = 32768, 256 x 128.
@@ -1012,9 +1011,10 @@ int launch_typed(const TileParams &t, const Device &device, cudaStream_t stream)
 
 template <class T, int D>
 int launch_typed(const TileParams &t, int groups, bool mods, const Device &device, cudaStream_t stream) {
-    if (groups == 1)
-        return mods ? launch_typed<T, D, 1, true>(t, device, stream) : launch_typed<T, D, 1, false>(t, device, stream);
-    return mods ? launch_typed<T, D, 2, true>(t, device, stream) : launch_typed<T, D, 2, false>(t, device, stream);
+    if constexpr (D == 128)  // pairs of tiles: kvx_attention takes them there alone
+        if (groups == 2)
+            return mods ? launch_typed<T, D, 2, true>(t, device, stream) : launch_typed<T, D, 2, false>(t, device, stream);
+    return mods ? launch_typed<T, D, 1, true>(t, device, stream) : launch_typed<T, D, 1, false>(t, device, stream);
 }
 
 }  // namespace
