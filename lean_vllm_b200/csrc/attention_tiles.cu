@@ -38,31 +38,33 @@ namespace {
 
 using namespace kvx;
 
-// Warps of a CTA with GROUPS tiles of rows (two, or one): the softmax's, then one each that issues products, copies keys and values, copies queries and looks up items.
+// Warps of a CTA with GROUPS tiles of rows (two, or one) and CTAS CTAs per SM: the softmax's, then one each that issues
+// products, copies keys and values, copies queries and looks up items.
 //
 // Registers. A row's 128 scores want more than the launch gives each thread, the other warps less. Two tiles, one CTA per
-// SM: 256 x 224 + 128 x 56 = 64512, the launch's 384 x 168. One tile, two CTAs: 128 x 200 + 128 x 56 = 32768, 256 x 128.
-template <int GROUPS>
+// SM: 256 x 224 + 128 x 56 = 64512, the launch's 384 x 168. One tile, two CTAs: 128 x 200 + 128 x 56 = 32768, 256 x 128;
+// one CTA: 128 x 224 + 128 x 56, of the launch's 256 x 224.
+template <int GROUPS, int CTAS>
 struct Warps {
     static constexpr int kSoftmax = 4 * GROUPS, kIssue = kSoftmax, kLoad = kSoftmax + 1, kQuery = kSoftmax + 2,
-                         kPlan = kSoftmax + 3, kThreads = 32 * (kSoftmax + 4), kCtas = GROUPS == 2 ? 1 : 2;
+                         kPlan = kSoftmax + 3, kThreads = 32 * (kSoftmax + 4);
     static constexpr int kItemReaders = kSoftmax + 3;  // warps that read an item
-    static constexpr int kSoftmaxRegisters = GROUPS == 2 ? 224 : 200, kOtherRegisters = 56;
+    static constexpr int kSoftmaxRegisters = CTAS == 1 ? 224 : 200, kOtherRegisters = 56;
     static constexpr int kColumns = 256 * GROUPS;      // of TMEM
 };
 constexpr float kLazy = 8.f;
 constexpr uint64_t kWaitNs = 2000000000ull;  // a wait that has not ended after 2 s is an error
 
-template <int D, int GROUPS>
+template <int D, int GROUPS, int CTAS>
 struct Shape {
     static constexpr int kHalves = D / 64;                      // 128-byte columns of a row
     static constexpr int kTileBytes = kTileKeys * D * 2;        // of 128 rows: queries, keys or values
     static constexpr int kHalfBytes = kTileKeys * 128;
-    static constexpr int kSlots = (D == 128 ? 2 : 4) * GROUPS;  // ring of K and V tiles: 64 KB a group
+    static constexpr int kSlots = (D == 128 ? 4 : 8) / CTAS;    // ring of K and V tiles: 128 KB an SM
     static constexpr int kStageBytes = 32 * 128;                // of a softmax warp: its rows' output on its way out
     static constexpr int kControlBytes = 1024;                  // barriers and items; the tiles start on 1024 bytes
     static constexpr int kBytes =
-        kControlBytes + (GROUPS + kSlots) * kTileBytes + Warps<GROUPS>::kSoftmax * kStageBytes;
+        kControlBytes + (GROUPS + kSlots) * kTileBytes + Warps<GROUPS, CTAS>::kSoftmax * kStageBytes;
     static constexpr int kOutColumn = 128 * GROUPS;             // TMEM: S and P of each tile, then O of each
 };
 
@@ -394,11 +396,11 @@ struct Control {
     Item items[2];
 };
 
-template <class T, int D, int GROUPS, bool MODS>
-__global__ void __launch_bounds__(Warps<GROUPS>::kThreads, Warps<GROUPS>::kCtas)
+template <class T, int D, int GROUPS, int CTAS, bool MODS>
+__global__ void __launch_bounds__(Warps<GROUPS, CTAS>::kThreads, CTAS)
 attention_tiles(const __grid_constant__ TileParams t) {
-    using S = Shape<D, GROUPS>;
-    using W = Warps<GROUPS>;
+    using S = Shape<D, GROUPS, CTAS>;
+    using W = Warps<GROUPS, CTAS>;
     extern __shared__ __align__(1024) unsigned char raw[];
     static_assert(sizeof(Control<S::kSlots>) <= S::kControlBytes, "the control block's room");
     Control<S::kSlots> &control = *reinterpret_cast<Control<S::kSlots> *>(raw);
@@ -998,23 +1000,30 @@ int launch(Kernel kernel, const TileParams &t, int64_t grid, int threads, int sm
     return KVX_OK;
 }
 
-template <class T, int D, int GROUPS, bool MODS>
+template <class T, int D, int GROUPS, int CTAS, bool MODS>
 int launch_typed(const TileParams &t, const Device &device, cudaStream_t stream) {
     static AllowedSmem allowed;
-    auto kernel = attention_tiles<T, D, GROUPS, MODS>;
-    if (int rc = allowed.allow(kernel, Shape<D, GROUPS>::kBytes, device.index)) return rc;
+    auto kernel = attention_tiles<T, D, GROUPS, CTAS, MODS>;
+    using S = Shape<D, GROUPS, CTAS>;
+    if (int rc = allowed.allow(kernel, S::kBytes, device.index)) return rc;
     // One wave of CTAs, each taking item after item.
     const int64_t items = (int64_t)t.row_tiles * t.a.kv_heads * t.splits;
-    const int64_t grid = std::min<int64_t>(items, (int64_t)device.sms * Warps<GROUPS>::kCtas);
-    return launch(kernel, t, grid, Warps<GROUPS>::kThreads, Shape<D, GROUPS>::kBytes, stream);
+    const int64_t grid = std::min<int64_t>(items, (int64_t)device.sms * CTAS);
+    return launch(kernel, t, grid, Warps<GROUPS, CTAS>::kThreads, S::kBytes, stream);
 }
 
 template <class T, int D>
 int launch_typed(const TileParams &t, int groups, bool mods, const Device &device, cudaStream_t stream) {
-    if constexpr (D == 128)  // pairs of tiles: kvx_attention takes them there alone
+    if constexpr (D == 128) {
         if (groups == 2)
-            return mods ? launch_typed<T, D, 2, true>(t, device, stream) : launch_typed<T, D, 2, false>(t, device, stream);
-    return mods ? launch_typed<T, D, 1, true>(t, device, stream) : launch_typed<T, D, 1, false>(t, device, stream);
+            return mods ? launch_typed<T, D, 2, 1, true>(t, device, stream) : launch_typed<T, D, 2, 1, false>(t, device, stream);
+        // No more items than SMs: a CTA has an SM, and twice the ring, to itself. A prompt of 256 tokens of 32 heads over 8
+        // takes 9.5 us so and 10.3 in the other shape, one of 512 12.9 and 14.2 (64 wide: 8.2 and 8.2, 10.7 and 11.1).
+        // Behind a shared prefix attention_rows' CTAs start in the room that the smaller ring leaves.
+        if (!t.prefix_only && (int64_t)t.row_tiles * t.a.kv_heads * t.splits <= device.sms)
+            return mods ? launch_typed<T, D, 1, 1, true>(t, device, stream) : launch_typed<T, D, 1, 1, false>(t, device, stream);
+    }
+    return mods ? launch_typed<T, D, 1, 2, true>(t, device, stream) : launch_typed<T, D, 1, 2, false>(t, device, stream);
 }
 
 }  // namespace
