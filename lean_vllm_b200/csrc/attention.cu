@@ -29,8 +29,8 @@ using namespace kvx;
 // Inside a CTA each of the 4 warps takes its own 16 tokens of every tile with its own running maximum, sum and output,
 // and loads them itself with cp.async into its own ring: no barrier until the group's end.
 //
-// Bound by HBM: 64 ragged requests of up to 16k tokens (957 MB) take 159 us, 6.0 TB/s; one of 131k 96 us, 5.6 TB/s, of
-// which 10 are the start and the join of 55 parts a head. One request of 317 tokens takes 7.6 us, a chain of waits: the
+// Bound by HBM: 64 ragged requests of up to 16k tokens (957 MB) take 160 us, 6.0 TB/s; one of 131k 94 us, 5.7 TB/s: the
+// walks end after 70 us on half of the SMs and 80 to 87 on the others, and 7 are the join of 55 parts a head. One request of 317 tokens takes 7.6 us, a chain of waits: the
 // launch, lengths, table, keys (0.5 us each) and the join of 5 parts.
 //
 // Up to 8 rows the products run transposed, S^T = K Q^T and O^T = V^T P^T, with the rows as the tensor cores' 8 columns:
@@ -50,9 +50,7 @@ struct RowShape {
 };
 
 template <int D, int ROWS>
-constexpr int row_smem() {
-    return kRowWarps * RowShape<ROWS>::kStages * kWarpTokens * D * 2 * 2;
-}
+constexpr int kRowSmem = kRowWarps * RowShape<ROWS>::kStages * kWarpTokens * D * 2 * 2;
 
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void *src, bool valid) {
     const int bytes = valid ? 16 : 0;  // the rest is filled with zeros
@@ -127,6 +125,70 @@ __device__ __forceinline__ int64_t row_units(const AttnParams &p, int s) {
     if ((int64_t)q.q_len * p.group > p.rows_limit) return 0;  // attention_tiles takes it
     const RowWork w = row_work<ROWS>(p, q);
     return w.groups(p) * w.tiles;
+}
+
+// Joins many parts of a group by way of shared memory, the ring's, half of it full of parts on their way while the other
+// half is joined: registers hold 8 parts a thread, one wait for the L2 cache (1.1 us) after another, and 55 parts of 4 rows
+// take 8 us so, 5 this way. (Up to 8 parts registers are as fast.)
+template <int D, int ROWS, class FirstRow, class Finish>
+__device__ __forceinline__ void join_many(const AttnParams &p, unsigned char *room, int parts, int rows,
+                                          const FirstRow &first_row, const Finish &finish) {
+    constexpr int kQuads = D / 4, kItems = ROWS * kQuads / kRowThreads, kHalf = kRowSmem<D, ROWS> / 2;
+    static_assert(kHalf / (D * 4 + 8) <= kRowThreads, "a row of a part per thread");
+    const int tid = threadIdx.x, values = rows * kQuads;  // float4 of a part
+    const int at_once = kHalf / (rows * (D * 4 + 8));
+    const int ml_part = tid / rows, ml_row = tid - ml_part * rows;  // the maximum and sum that this thread fetches
+    Joined j[kItems];
+    float2 ml_next = make_float2(0.f, 0.f);
+    auto fetch = [&](int i0) {
+        const int n = min(at_once, parts - i0);
+        const uint32_t to = smem_u32(room) + (i0 / at_once & 1) * kHalf + tid * 16;
+        if (ml_part < n) ml_next = __ldcg(&p.partial_ml[first_row(i0 + ml_part) + ml_row]);
+#pragma unroll 4
+        for (int i = 0; i < n; ++i) {
+            const float4 *from = reinterpret_cast<const float4 *>(p.partial_o) + first_row(i0 + i) * kQuads + tid;
+#pragma unroll
+            for (int k = 0; k < kItems; ++k)
+                if (tid + k * kRowThreads < values)
+                    cp_async16(to + i * values * 16 + k * kRowThreads * 16, from + k * kRowThreads, true);
+        }
+    };
+    fetch(0);
+    asm volatile("cp.async.commit_group;" ::: "memory");
+    for (int i0 = 0; i0 < parts; i0 += at_once) {
+        const int n = min(at_once, parts - i0);
+        unsigned char *half = room + (i0 / at_once & 1) * kHalf;
+        float2 *ml = reinterpret_cast<float2 *>(half + at_once * values * 16);  // [part][row]
+        if (ml_part < n) ml[tid] = ml_next;
+        if (i0 + at_once < parts) fetch(i0 + at_once);
+        asm volatile("cp.async.commit_group;\n\tcp.async.wait_group 1;" ::: "memory");
+        __syncthreads();
+#pragma unroll
+        for (int k = 0; k < kItems; ++k) {
+            const int item = tid + k * kRowThreads, row = item / kQuads;
+            if (item >= values) break;
+            float top = j[k].top;
+#pragma unroll 8
+            for (int i = 0; i < n; ++i) top = fmaxf(top, ml[i * rows + row].x);
+            const float reference = top == -INFINITY ? 0.f : top, own = exp2_fast(j[k].top - reference);
+            j[k].top = top;
+            j[k].sum *= own, j[k].o.x *= own, j[k].o.y *= own, j[k].o.z *= own, j[k].o.w *= own;
+#pragma unroll 8
+            for (int i = 0; i < n; ++i) {
+                const float2 part = ml[i * rows + row];
+                const float4 x = reinterpret_cast<const float4 *>(half)[i * values + item];
+                const float f = exp2_fast(part.x - reference);
+                j[k].sum += f * part.y;
+                j[k].o.x += f * x.x, j[k].o.y += f * x.y, j[k].o.z += f * x.z, j[k].o.w += f * x.w;
+            }
+        }
+        __syncthreads();  // this half is free again
+    }
+#pragma unroll
+    for (int k = 0; k < kItems; ++k) {
+        const int item = tid + k * kRowThreads;
+        if (item < values) finish(item / kQuads, item % kQuads, j[k]);
+    }
 }
 
 template <class T, int D, int ROWS, bool MODS>
@@ -520,12 +582,18 @@ attention_rows(const __grid_constant__ AttnParams p) {
             __syncthreads();
             if (is_last) {
                 __threadfence();
-                for (int item = tid; item < rows * kQuads; item += kRowThreads) {
-                    const int row = item / kQuads, quad = item % kQuads;
-                    Joined j;
-                    join_parts<8>(j, c1 - c0 + 1, p.partial_ml, p.partial_o, kQuads, quad,
-                               [&](int i) { return (int64_t)(2 * (c0 + i) + (i == 0)) * kRowTile + row; });
-                    finish(row, quad, j);
+                const int parts = c1 - c0 + 1;
+                auto first_row = [&](int i) { return (int64_t)(2 * (c0 + i) + (i == 0)) * kRowTile; };  // of part i
+                if (parts <= 8) {
+                    for (int item = tid; item < rows * kQuads; item += kRowThreads) {
+                        const int row = item / kQuads, quad = item % kQuads;
+                        Joined j;
+                        join_parts<8>(j, parts, p.partial_ml, p.partial_o, kQuads, quad,
+                                      [&](int i) { return first_row(i) + row; });
+                        finish(row, quad, j);
+                    }
+                } else {
+                    join_many<D, ROWS>(p, smem, parts, rows, first_row, finish);
                 }
             }
         }
@@ -616,8 +684,8 @@ template <class T, int D, int ROWS, bool MODS>
 int launch_rows(const AttnParams &p, const Device &device, cudaStream_t stream) {
     static AllowedSmem allowed;
     auto kernel = attention_rows<T, D, ROWS, MODS>;
-    if (int rc = allowed.allow(kernel, row_smem<D, ROWS>(), device.index)) return rc;
-    return launch(kernel, std::min(RowShape<ROWS>::kCtas * device.sms, kMaxRowCtas), kRowThreads, row_smem<D, ROWS>(),
+    if (int rc = allowed.allow(kernel, kRowSmem<D, ROWS>, device.index)) return rc;
+    return launch(kernel, std::min(RowShape<ROWS>::kCtas * device.sms, kMaxRowCtas), kRowThreads, kRowSmem<D, ROWS>,
                   stream, p);
 }
 
