@@ -603,55 +603,72 @@ attention_rows(const __grid_constant__ AttnParams p) {
     wait_prerequisites();
 }
 
-// Joins each row's parts, four elements a thread: attention_tiles' splits, or its splits of a shared prefix and
-// attention_rows' part over the sequence's own keys. Rows of sequences that attention_rows took whole have none.
-// SPREAD threads share the parts of the same elements, so that many parts of few rows are still read at once (4 requests
-// of 30k tokens and 32 heads over one KV head, 74 parts of 128 rows: 47 us for the call with one thread, 29 with four).
+// Joins each row's parts: attention_tiles' splits, or its splits of a shared prefix and attention_rows' part over the
+// sequence's own keys. Rows of sequences that attention_rows took whole have none.
+//
+// A thread has four elements of a row, and at_once parts of them on their way into its own places in shared memory at a
+// time; the threads of a row fetch the parts' maxima and sums, up to two each. Bound by the L2 cache's latency, so
+// everything is asked for at once: 64 requests of 32 heads behind 8192 tokens (2048 rows of 19 parts) take 36 us, 40 with
+// 8 parts at a time in registers; 500 of them (5 parts) 133 and 135.
 constexpr int kJoinThreads = 128;
+template <int D>
+constexpr int kJoinAtOnce = D == 128 ? 48 : 32;  // two for each of a row's threads, 96 KB of shared memory at most
 
-template <class T, int D, int SPREAD>
-__global__ void __launch_bounds__(kJoinThreads) attention_join(const __grid_constant__ AttnParams p, int parts, bool mixed) {
-    constexpr uint32_t kQuads = D / 4, kRows = kJoinThreads / (kQuads * SPREAD);
-    __shared__ float4 share_o[SPREAD == 1 ? 1 : kJoinThreads];
-    __shared__ float2 share_ml[SPREAD == 1 ? 1 : kJoinThreads];
+template <class T, int D>
+__global__ void __launch_bounds__(kJoinThreads)
+attention_join(const __grid_constant__ AttnParams p, int parts, int at_once, bool mixed) {
+    constexpr uint32_t kQuads = D / 4, kRows = kJoinThreads / kQuads;
+    extern __shared__ __align__(128) unsigned char smem[];  // [part][thread]
     const uint32_t rows = (uint32_t)p.num_tokens * p.q_heads;  // at most kSplitRows
-    const uint32_t quad = threadIdx.x % kQuads, share = threadIdx.x / kQuads % SPREAD;
-    const uint32_t row = blockIdx.x * kRows + threadIdx.x / (kQuads * SPREAD);
+    const uint32_t quad = threadIdx.x % kQuads, row = blockIdx.x * kRows + threadIdx.x / kQuads;
     const int token = (int)(row / (uint32_t)p.q_heads);
     wait_prerequisites();
     launch_dependents();
-    bool wanted = row < rows;
-    if (wanted && mixed) {
+    if (row >= rows) return;
+    if (mixed) {
         int low = 0, high = p.batch;  // the last sequence that starts at or before the token
         while (high - low > 1) {
             const int mid = (low + high) / 2;
             if (p.q_starts[mid] <= token) low = mid;
             else high = mid;
         }
-        wanted = (int64_t)sequence_of(p, low).q_len * p.group > p.rows_limit;
+        if ((int64_t)sequence_of(p, low).q_len * p.group <= p.rows_limit) return;
     }
+    const uint32_t mask = kQuads == 32 ? ~0u : 0xffffu << (threadIdx.x & 16);  // the row's threads
+    const float4 *mine = reinterpret_cast<const float4 *>(smem) + threadIdx.x;
     Joined j;
-    if (wanted)
-        join_parts<SPREAD == 1 ? 4 : 8>(j, (parts - (int)share + SPREAD - 1) / SPREAD, p.split_ml, p.split_o, kQuads, quad,
-                                        [&](int i) { return (int64_t)row + (int64_t)(share + i * SPREAD) * rows; });
-    if (SPREAD > 1) {
-        const uint32_t place = threadIdx.x % (SPREAD == 1 ? 1 : kJoinThreads);
-        share_o[place] = j.o;
-        share_ml[place] = make_float2(j.top, j.sum);
-        __syncthreads();
-        if (share != 0) return;
-        for (int other = 1; other < SPREAD; ++other) {
-            const uint32_t at = (threadIdx.x + other * kQuads) % (SPREAD == 1 ? 1 : kJoinThreads);
-            const float2 ml = share_ml[at];
-            const float4 o = share_o[at];
-            const float top = fmaxf(j.top, ml.x), mine = weight_of(j.top, top), theirs = weight_of(ml.x, top);
-            j.top = top;
-            j.sum = j.sum * mine + ml.y * theirs;
-            j.o.x = j.o.x * mine + o.x * theirs, j.o.y = j.o.y * mine + o.y * theirs;
-            j.o.z = j.o.z * mine + o.z * theirs, j.o.w = j.o.w * mine + o.w * theirs;
+    for (int i0 = 0; i0 < parts; i0 += at_once) {
+        const int n = min(at_once, parts - i0);
+        float2 ml[2];
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+            const int i = quad + k * kQuads;
+            ml[k] = i < n ? __ldcg(&p.split_ml[row + (int64_t)(i0 + i) * rows]) : make_float2(-INFINITY, 0.f);
+        }
+        const float4 *from = reinterpret_cast<const float4 *>(p.split_o) + (row + (int64_t)i0 * rows) * kQuads + quad;
+        for (int i = 0; i < n; ++i, from += (int64_t)rows * kQuads)
+            cp_async16(smem_u32(mine + i * kJoinThreads), from, true);
+        asm volatile("cp.async.commit_group;" ::: "memory");
+        float top = fmaxf(j.top, fmaxf(ml[0].x, ml[1].x));
+#pragma unroll
+        for (int o = kQuads / 2; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(mask, top, o));
+        const float reference = top == -INFINITY ? 0.f : top, own = exp2_fast(j.top - reference);
+        const float f[2] = {exp2_fast(ml[0].x - reference), exp2_fast(ml[1].x - reference)};
+        float sum = f[0] * ml[0].y + f[1] * ml[1].y;
+#pragma unroll
+        for (int o = kQuads / 2; o; o >>= 1) sum += __shfl_xor_sync(mask, sum, o);
+        j.top = top;
+        j.sum = j.sum * own + sum;
+        j.o.x *= own, j.o.y *= own, j.o.z *= own, j.o.w *= own;
+        asm volatile("cp.async.wait_group 0;" ::: "memory");
+#pragma unroll 4
+        for (int i = 0; i < n; ++i) {
+            const float factor = __shfl_sync(mask, i < (int)kQuads ? f[0] : f[1], i % kQuads, kQuads);
+            const float4 x = mine[i * kJoinThreads];
+            j.o.x += factor * x.x, j.o.y += factor * x.y, j.o.z += factor * x.z, j.o.w += factor * x.w;
         }
     }
-    if (wanted) write_row<T>(p, token, (int)(row - token * p.q_heads), quad, j);
+    write_row<T>(p, token, (int)(row - token * p.q_heads), quad, j);
 }
 
 // ------------------------------------------------------------------------------------------------ host side
@@ -696,20 +713,21 @@ int launch_rows(const AttnParams &p, int rows, bool mods, const Device &device, 
 }
 
 template <class T, int D>
-int launch_join(const AttnParams &p, int parts, bool mixed, cudaStream_t stream) {
+int launch_join(const AttnParams &p, int parts, bool mixed, const Device &device, cudaStream_t stream) {
     const int64_t rows = (int64_t)p.num_tokens * p.q_heads;
-    if (parts > 4 && rows <= 4096) {  // more rows fill the device with a thread each: 16,384 rows of 5 parts 33 and 65 us
-        constexpr int kRows = kJoinThreads / D;  // 4 x D / 4 threads a row
-        return launch(attention_join<T, D, 4>, (rows + kRows - 1) / kRows, kJoinThreads, 0, stream, p, parts, mixed);
-    }
-    constexpr int kRows = 4 * kJoinThreads / D;
-    return launch(attention_join<T, D, 1>, (rows + kRows - 1) / kRows, kJoinThreads, 0, stream, p, parts, mixed);
+    constexpr int kRows = 4 * kJoinThreads / D, kAtOnce = kJoinAtOnce<D>;
+    const int rounds = (parts + kAtOnce - 1) / kAtOnce, at_once = (parts + rounds - 1) / rounds;
+    static AllowedSmem allowed;
+    auto kernel = attention_join<T, D>;
+    if (int rc = allowed.allow(kernel, kAtOnce * kJoinThreads * 16, device.index)) return rc;
+    return launch(kernel, (rows + kRows - 1) / kRows, kJoinThreads, at_once * kJoinThreads * 16, stream, p,
+                  parts, at_once, mixed);
 }
 
 // How many parts attention_tiles' items are cut into along the keys: more items fill SMs that would idle, but every part
 // of a row is written and read once more. By what both take on B200 (us): a pair of tiles 1.85, an item's ends 1.2, the
-// join 3 and its traffic at 4 TB/s. 200 tokens of 32 heads behind 4k take 67 us in one part, 32 in four; 512 new tokens
-// 16.5 in one, 18.8 in two.
+// join 3 and its traffic at 4 TB/s. 200 tokens of 32 heads behind 4k take 60 us in one part, 29 in four; 512 new tokens
+// 14 in one, 18 in two.
 int choose_splits(int64_t items, int64_t keys, int64_t rows, int head_dim, int ctas) {
     const int64_t tiles = std::max<int64_t>(1, (keys + kTileKeys - 1) / kTileKeys);
     const double part_bytes = 2.0 * rows * (4 * head_dim + 8);
@@ -822,10 +840,10 @@ int kvx_attention(const kvx_attention_args *args, int flags, void *stream) {
 
     auto join = [&](int parts, bool mixed) {
         if (a.head_dim == 128)
-            return a.dtype == KVX_BF16 ? launch_join<__nv_bfloat16, 128>(p, parts, mixed, s)
-                                       : launch_join<__half, 128>(p, parts, mixed, s);
-        return a.dtype == KVX_BF16 ? launch_join<__nv_bfloat16, 64>(p, parts, mixed, s)
-                                   : launch_join<__half, 64>(p, parts, mixed, s);
+            return a.dtype == KVX_BF16 ? launch_join<__nv_bfloat16, 128>(p, parts, mixed, device, s)
+                                       : launch_join<__half, 128>(p, parts, mixed, device, s);
+        return a.dtype == KVX_BF16 ? launch_join<__nv_bfloat16, 64>(p, parts, mixed, device, s)
+                                   : launch_join<__half, 64>(p, parts, mixed, device, s);
     };
 
     // ---- which kernel takes what
