@@ -19,7 +19,7 @@
 // items (lookup, queries, first keys, output), a quarter of a prompt of 8192 tokens.
 //
 // Bound by the tensor cores as the power limit lets them run: a prompt of 8192 tokens of 32 heads over 8, 128 wide, takes
-// 478 us, 1150 TFLOP/s, 70% of a large cuBLAS product's rate. A pair of tiles takes 3300 cycles where its products alone
+// 470 us, 1170 TFLOP/s, 71% of a large cuBLAS product's rate. A pair of tiles takes 3300 cycles where its products alone
 // take 2048: each waits 1250 for the other's (768 of them its own last half and next scores) and spends 2000 in the
 // softmax, half of that on the special-function unit. A third of the exponentials on the multiply-add pipe instead made
 // that shorter and the whole no faster (498 us); an issuing warp for each tile let both fall into step and contend (499).
