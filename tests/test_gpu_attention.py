@@ -102,6 +102,51 @@ def test_masks_caps_and_biases(q_lens, kv_lens, heads, kv_heads, dim, block, dty
     check(case, workspace, **options)
 
 
+@pytest.mark.parametrize("q_lens, kv_lens, heads, kv_heads, dim, dtype, shared", [
+    ([300], [900], 8, 2, 128, BF16, 0),
+    ([300], [900], 8, 2, 64, FP16, 0),
+    ([40, 1, 90], [2000, 400, 90], 4, 1, 64, BF16, 0),
+    ([700, 300], [1500, 300], 16, 8, 128, BF16, 0),
+    ([1] * 40, [300] * 40, 8, 2, 128, FP16, 700),
+], ids=["prompt128", "prompt64", "chunks64", "prompts128", "shared"])
+@pytest.mark.parametrize("window", [0, 350])
+def test_caps_near_and_far(q_lens, kv_lens, heads, kv_heads, dim, dtype, shared, window, workspace):
+    """Scores well below the cap; scores of which some tiles of keys are near it and beyond, others not; scores beyond it
+    everywhere."""
+    if shared and window:
+        pytest.skip("a shared prefix takes no window")
+    for softcap, factor in ((40.0, 1.0), (20.0, 8.0), (0.5, 1.0)):
+        case = paged_case(q_lens, kv_lens, heads, kv_heads, dim, 16, dtype, shared=shared)
+        if factor != 1.0:  # some stretches of 160 keys
+            for s, keys in enumerate(case["keys"]):
+                if not shared:
+                    i = torch.arange(0, keys.size(0), device="cuda")
+                    chosen = i[i // 160 % 3 == 1]
+                    keys[chosen] *= factor
+                    case["k_cache"][case["tables"][s][chosen // 16].long(), chosen % 16] = keys[chosen]
+        check(case, workspace, softcap=softcap, **(dict(window=window) if window else {}))
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("q_lens, kv_lens, heads, shared", [
+    ([1], [20000], 4, 0), ([4], [20000], 4, 0), ([3, 1], [9000, 17], 1, 0),  # one walk of the cache in hundreds of parts
+    ([40], [20000], 4, 0), ([20, 1], [30000, 5], 8, 0),
+    ([1, 2], [50, 0], 4, 20000),
+], ids=["rows4", "rows16", "rows3", "tiles", "mixed", "shared"])
+def test_many_parts(q_lens, kv_lens, heads, shared, dim, workspace):
+    """One KV head and a long cache: parts in numbers that are joined in several rounds, the same each time."""
+    case = paged_case(q_lens, kv_lens, heads, 1, dim, 16, BF16, shared=shared)
+    first = check(case, workspace)
+    for _ in range(3):
+        assert torch.equal(run(case, workspace), first)
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+def test_more_items_than_a_wave(dim, workspace):
+    """Tiles of rows that CTAs take one after another."""
+    check(paged_case([900, 3, 400], [900, 600, 1000], 32, 8, dim, 16, BF16), workspace)
+
+
 def test_a_window_never_reads_what_lies_before_it(workspace):
     """Blocks ahead of every row's window may be gone: their table entries are stale and their rows NaN."""
     case = paged_case([1, 20], [1000, 700], 8, 2, 128, 16, BF16)
