@@ -30,8 +30,8 @@ using namespace kvx;
 // and loads them itself with cp.async into its own ring: no barrier until the group's end.
 //
 // Bound by HBM: 64 ragged requests of up to 16k tokens (957 MB) take 160 us, 6.0 TB/s; one of 131k 94 us, 5.7 TB/s: the
-// walks end after 70 us on half of the SMs and 80 to 87 on the others, and 7 are the join of 55 parts a head. One request of 317 tokens takes 7.6 us, a chain of waits: the
-// launch, lengths, table, keys (0.5 us each) and the join of 5 parts.
+// walks end after 70 to 75 us on most SMs and 80 to 87 on the others, and 7 are the join of 55 parts a head. One request
+// of 317 tokens takes 7.6 us, a chain of waits: the launch, lengths, table, keys (0.5 us each) and the join of 5 parts.
 //
 // Up to 8 rows the products run transposed, S^T = K Q^T and O^T = V^T P^T, with the rows as the tensor cores' 8 columns:
 // half the instructions and registers of a 16-row tile that would be half padding.
@@ -588,8 +588,8 @@ attention_rows(const __grid_constant__ AttnParams p) {
                     for (int item = tid; item < rows * kQuads; item += kRowThreads) {
                         const int row = item / kQuads, quad = item % kQuads;
                         Joined j;
-                        join_parts<8>(j, parts, p.partial_ml, p.partial_o, kQuads, quad,
-                                      [&](int i) { return first_row(i) + row; });
+                        join_parts(j, parts, p.partial_ml, p.partial_o, kQuads, quad,
+                                   [&](int i) { return first_row(i) + row; });
                         finish(row, quad, j);
                     }
                 } else {

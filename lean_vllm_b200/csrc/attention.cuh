@@ -53,8 +53,8 @@ struct AllowedSmem {
 };
 
 // attention_tiles (attention_tiles.cu). `prefix_only`: all query rows against the shared prefix alone; else each
-// sequence's rows above rows_limit. `groups`: tiles of rows per CTA, 1 or 2. It leaves `splits` parts to join, and finished rows when there is one split and it is
-// not prefix_only.
+// sequence's rows above rows_limit. `groups`: tiles of rows per CTA, 1 or 2. It leaves `splits` parts to join, and finished
+// rows when there is one split and it is not prefix_only.
 int launch_tiles(const AttnParams &p, int head_dim, int dtype, bool mods, bool prefix_only, int groups, int splits,
                  const Device &device, cudaStream_t stream);
 // The tokens of this cache that one of attention_tiles' copies brings; 0 if it cannot take the call (blocks that are no
@@ -64,7 +64,6 @@ int tile_box(const AttnParams &p);
 constexpr int kMaxRowCtas = 1024;       // of attention_rows: a counter and two slots of partial results each
 constexpr int kTileCounter = 8192;      // attention_tiles' counter, on a line of its own
 constexpr int kRowTile = 16;            // rows of attention_rows' widest tile
-constexpr int kTileRows = 256;
 constexpr int kTileKeys = 128;
 constexpr int64_t kSplitRows = 131072;  // rows of partial results the workspace holds
 
@@ -119,11 +118,11 @@ struct Joined {
     float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
 };
 
-// Joins n more parts in order; at(i) is part i's row index into `ml`, of [row][quads] float4 in `o`. AT_ONCE parts' loads
-// are in flight together: one after another, each would wait for the L2 cache (0.5 us), 18 of them for 10 us.
-template <int AT_ONCE, class At>
+// Joins n more parts in order; at(i) is part i's row index into `ml`, of [row][quads] float4 in `o`. Eight parts' loads are
+// in flight together: one after another, each would wait for the L2 cache (0.5 us).
+template <class At>
 __device__ __forceinline__ void join_parts(Joined &j, int n, const float2 *ml, const float *o, int quads, int quad, At at) {
-    constexpr int kAtOnce = AT_ONCE;
+    constexpr int kAtOnce = 8;
     for (int i0 = 0; i0 < n; i0 += kAtOnce) {
         float2 part[kAtOnce];
         float4 x[kAtOnce];
