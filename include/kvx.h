@@ -264,7 +264,8 @@ typedef struct kvx_attention_args {
     int32_t head_dim;           /* 64 or 128 */
     int32_t dtype;              /* KVX_BF16 or KVX_FP16 */
     int32_t max_q_len;          /* the most query tokens of a sequence and the most cached ones, for the choice of */
-    int32_t max_kv_len;         /* launch shape: a wrong bound costs time, not correctness */
+    int32_t max_kv_len;         /* launch shape: a wrong bound costs time, not correctness; without q_starts the
+                                   first is 1, whatever it says */
     int32_t window;             /* a row sees its own position and the window - 1 before it; 0: all */
     float scale;                /* scores are scale * q.k ... */
     float softcap;              /* ... capped to softcap * tanh(score / softcap); 0: as they are */

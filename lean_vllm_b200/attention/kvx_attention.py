@@ -135,7 +135,8 @@ def paged_attention(query: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.T
     used, whatever they hold. Inside it, a value that one row sees must be finite for the rows beside it too (they
     multiply it by zero).
 
-    `max_q_len` and `max_kv_len` bound the lengths (the device holds them): they choose the launch's shape only.
+    `max_q_len` and `max_kv_len` bound the lengths (the device holds them): they choose the launch's shape only. Without
+    q_starts `max_q_len` means nothing.
     `status` (a StatusWord's address) gets bit 2 for a block id outside the cache, which reads as zeros, or a length past
     its table, which is cut to it."""
     return _attention(query, k_cache, v_cache, block_tables, kv_lens, scale, q_starts, max_q_len, max_kv_len, softcap,

@@ -625,15 +625,7 @@ attention_join(const __grid_constant__ AttnParams p, int parts, int at_once, boo
     wait_prerequisites();
     launch_dependents();
     if (row >= rows) return;
-    if (mixed) {
-        int low = 0, high = p.batch;  // the last sequence that starts at or before the token
-        while (high - low > 1) {
-            const int mid = (low + high) / 2;
-            if (p.q_starts[mid] <= token) low = mid;
-            else high = mid;
-        }
-        if ((int64_t)sequence_of(p, low).q_len * p.group <= p.rows_limit) return;
-    }
+    if (mixed && (int64_t)sequence_of(p, sequence_at(p, token)).q_len * p.group <= p.rows_limit) return;
     const uint32_t mask = kQuads == 32 ? ~0u : 0xffffu << (threadIdx.x & 16);  // the row's threads
     const float4 *mine = reinterpret_cast<const float4 *>(smem) + threadIdx.x;
     Joined j;
@@ -828,7 +820,9 @@ int kvx_attention(const kvx_attention_args *args, int flags, void *stream) {
     p.rows_limit = INT32_MAX;
     const bool mods = a.softcap > 0.f || a.slopes || !(a.scale > 0.f);
     cudaStream_t s = static_cast<cudaStream_t>(stream);
-    const int64_t q_rows = (int64_t)std::max(a.max_q_len, 1) * p.group;  // of the longest sequence and one KV head
+    // Without q_starts every sequence has one query token, whatever bound came with the call.
+    const int64_t max_q_len = a.q_starts ? std::max(a.max_q_len, 1) : 1;
+    const int64_t q_rows = max_q_len * p.group;  // of the longest sequence and one KV head
     auto rows_kernel = [&](int64_t rows) {
         const int n = rows <= 8 ? 8 : 16;
         if (a.head_dim == 128)
@@ -866,11 +860,11 @@ int kvx_attention(const kvx_attention_args *args, int flags, void *stream) {
     }
     if (q_rows <= kRowTile) return rows_kernel(q_rows);
     // Prompt chunks, and beside them (unless every sequence may be one) the sequences of few rows.
-    const bool mixed = a.batch > 1 && a.num_tokens < (int64_t)a.batch * a.max_q_len;
+    const bool mixed = a.batch > 1 && a.num_tokens < a.batch * max_q_len;
     p.rows_limit = !mixed ? 0 : p.group <= 8 ? 8 : kRowTile;
     auto items_of = [&](int groups) {  // about how many
         const int64_t tokens = groups * tile_tokens;
-        int64_t items = a.batch * (((int64_t)a.max_q_len + tokens - 1) / tokens);
+        int64_t items = a.batch * ((max_q_len + tokens - 1) / tokens);
         if (mixed) items = std::min<int64_t>(items, (a.num_tokens + tokens - 1) / tokens + (a.batch - 1) / 2);
         return std::max<int64_t>(1, items) * p.kv_heads;
     };
@@ -884,7 +878,7 @@ int kvx_attention(const kvx_attention_args *args, int flags, void *stream) {
     // for 148 SMs) takes 15.8 us in pairs and 14.3 in single tiles, 768 tokens 19.7 and 19.3, 1024 24.1 and 24.6, 2048
     // 53.2 and 57.0. 64 wide, the single tile is ahead at every size: 13.4 and 11.1, 45.4 and 42.1, 8192 tokens 418 and 389.
     int groups = 1, splits = 0;
-    if (a.head_dim == 128 && a.max_q_len > tile_tokens) {
+    if (a.head_dim == 128 && max_q_len > tile_tokens) {
         splits = splits_of(2);
         if (items_of(2) * splits * 8 > (int64_t)device.sms * 5) groups = 2;
     }

@@ -84,6 +84,18 @@ __device__ __forceinline__ Sequence sequence_of(const AttnParams &p, int s) {
     return q;
 }
 
+// Whose query token `token` is: the last sequence that starts at or before it.
+__device__ __forceinline__ int sequence_at(const AttnParams &p, int token) {
+    if (!p.q_starts) return token;
+    int low = 0, high = p.batch;
+    while (high - low > 1) {
+        const int mid = (low + high) / 2;
+        if (p.q_starts[mid] <= token) low = mid;
+        else high = mid;
+    }
+    return low;
+}
+
 // Where sequence s keeps token t: a byte offset from the caches' first block and head, or -1 for a block id outside
 // the cache, which is flagged.
 __device__ __forceinline__ int64_t token_at(const AttnParams &p, int s, int32_t t) {

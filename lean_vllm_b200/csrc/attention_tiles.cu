@@ -480,17 +480,7 @@ attention_tiles(const __grid_constant__ TileParams t) {
             float slope = 0.f;
             if (t.prefix_only) {
                 if (MODS && p.slopes && valid) {  // where the row stands behind the prefix
-                    int s = token;
-                    if (p.q_starts) {
-                        int low = 0, high = p.batch;  // the last sequence that starts at or before the token
-                        while (high - low > 1) {
-                            const int mid = (low + high) / 2;
-                            if (p.q_starts[mid] <= token) low = mid;
-                            else high = mid;
-                        }
-                        s = low;
-                    }
-                    const Sequence q = sequence_of(p, s);
+                    const Sequence q = sequence_of(p, sequence_at(p, token));
                     position = q.kv_len - q.q_len + token - q.q0;
                 }
             } else if (valid) {

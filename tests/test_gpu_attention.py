@@ -276,6 +276,17 @@ def test_wrong_bounds_on_the_query_lengths_are_harmless(workspace):
         check_attention(got, case)
 
 
+@pytest.mark.parametrize("kv_lens, heads, kv_heads, dim, shared", [
+    ([4096, 77], 32, 8, 128, 0), ([600, 1, 0, 300], 32, 8, 128, 0), ([5000, 9], 14, 2, 64, 0), ([3, 40, 2], 32, 4, 128, 3000),
+], ids=["long", "short", "dim64", "shared"])
+@pytest.mark.parametrize("bound", [5, 16, 10000])
+def test_single_tokens_are_single_whatever_the_bound(kv_lens, heads, kv_heads, dim, shared, bound, workspace):
+    """Without q_starts a bound on the query lengths, a captured maximum say, means nothing: the same bits."""
+    case = paged_case([1] * len(kv_lens), kv_lens, heads, kv_heads, dim, 16, BF16, shared=shared)
+    want = check(case, workspace)
+    assert torch.equal(run(case, workspace, max_q_len=bound), want)
+
+
 def test_strided_queries_and_outputs(workspace):
     for q_lens in ([1, 1], [90, 5]):
         case = paged_case(q_lens, [200, 300], 6, 2, 128, 16, BF16, fused=True)
