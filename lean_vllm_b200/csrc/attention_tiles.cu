@@ -495,7 +495,9 @@ attention_tiles(const __grid_constant__ TileParams t) {
 
             float m = -INFINITY;
             float2 sum = make_float2(0.f, 0.f);
-            bool look_near = MODS && p.softcap > 0.f && !p.slopes;  // until a tile is not
+            // Until a tile is not. (Under a negative scale the capped scores fall as the products rise, and a tile's maximum
+            // would be its smallest product: those take the way through TMEM.)
+            bool look_near = MODS && p.softcap > 0.f && p.scale > 0.f && !p.slopes;
             for (int i = 0; i < item.tiles; ++i) {
                 const TileAt at = tile_at(p, item, i);
                 if (!warp_waits(smem_u32(&scores[g]), score_phase, &gave_up)) {

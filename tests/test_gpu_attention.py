@@ -323,6 +323,17 @@ def test_any_scale(scale, workspace):
         check(paged_case(q_lens, kv_lens, 8, 2, 128, 16, BF16), workspace, scale=scale)
 
 
+@pytest.mark.parametrize("softcap", [5.0, 30.0, 50.0])
+@pytest.mark.parametrize("q_lens, kv_lens, heads, kv_heads, dim, dtype, shared", [
+    ([300], [900], 8, 2, 128, FP16, 0), ([300, 40], [900, 700], 4, 2, 64, FP16, 0), ([300], [900], 8, 2, 128, BF16, 0),
+    ([1] * 20, [50] * 20, 8, 2, 128, FP16, 700), ([1, 2], [500, 300], 8, 2, 128, FP16, 0),
+], ids=["prompt128", "chunks64", "bf16", "shared", "decode"])
+def test_a_negative_scale_under_a_cap(q_lens, kv_lens, heads, kv_heads, dim, dtype, shared, softcap, workspace):
+    """Capped scores fall as the products rise: the row's maximum is its smallest product."""
+    check(paged_case(q_lens, kv_lens, heads, kv_heads, dim, 16, dtype, shared=shared), workspace, scale=-0.2,
+          softcap=softcap)
+
+
 def test_a_nan_that_is_seen_shows(workspace):
     """NaN in a key that every row sees makes every output of its head NaN, and of no other."""
     for q_lens, options in (([1], {}), ([70], {}), ([70], {"softcap": 5.0}), ([1], {"softcap": 5.0})):
