@@ -16,6 +16,11 @@ def raw_stream(device: int) -> int:
     return torch._C._cuda_getCurrentRawStream(device)
 
 
+def stream_of(handle: int, device: torch.device) -> torch.cuda.Stream:
+    """The stream object of a cudaStream_t; 0 is the default stream (torch.cuda.ExternalStream(0) would be another)."""
+    return torch.cuda.ExternalStream(handle, device) if handle else torch.cuda.default_stream(device)
+
+
 def call(device: int, function, *args) -> None:
     """Calls a library function that launches on the current device, with `device` as that; raises for an error."""
     if torch.cuda.current_device() == device:

@@ -12,7 +12,7 @@ import torch
 
 from lean_vllm_b200 import _native
 from lean_vllm_b200._native import check, lib
-from lean_vllm_b200.attention.device import call, calls, raw_stream
+from lean_vllm_b200.attention.device import call, calls, raw_stream, stream_of
 
 _INT32_MAX = 2**31 - 1
 _DTYPES = {torch.bfloat16: _native.BF16, torch.float16: _native.FP16}
@@ -26,7 +26,7 @@ class AttentionWorkspace:
     def __init__(self, device: torch.device | str = "cuda", stream: int | None = None):
         size = lib().kvx_attention_workspace_bytes()
         device = torch.device(device)
-        where = torch.cuda.ExternalStream(stream, device) if stream else torch.cuda.current_stream(device)
+        where = torch.cuda.current_stream(device) if stream is None else stream_of(stream, device)
         with torch.cuda.stream(where):
             self.tensor = torch.empty(size, dtype=torch.uint8, device=device)
             self.tensor[: _native.ATTENTION_ZEROED].zero_()
@@ -95,7 +95,7 @@ def _attention(query, k_cache, v_cache, block_tables, kv_lens, scale, q_starts, 
         out = torch.empty_like(query, memory_format=torch.contiguous_format)  # half the cost of torch.empty
         o0, o1 = q_heads * head_dim, head_dim
         if stream is not None:  # the caching allocator has to know who writes it
-            out.record_stream(torch.cuda.ExternalStream(stream, query.device))
+            out.record_stream(stream_of(stream, query.device))
     else:
         o0, o1, o2 = out.stride() if out.dim() == 3 else (0, 0, 0)
         if out.shape != shape or out.dtype != dtype or out.get_device() != device or o2 != 1:
@@ -103,7 +103,7 @@ def _attention(query, k_cache, v_cache, block_tables, kv_lens, scale, q_starts, 
     if workspace is None:
         workspace = AttentionWorkspace(query.device, stream)
         if stream is not None:
-            workspace.tensor.record_stream(torch.cuda.ExternalStream(stream, query.device))
+            workspace.tensor.record_stream(stream_of(stream, query.device))
     elif workspace.index != device:
         raise ValueError("the workspace must be on the queries' device")
     args = _native.ATTENTION_ARGS.pack(

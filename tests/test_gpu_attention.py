@@ -372,6 +372,30 @@ def test_other_streams(workspace):
         assert torch.equal(raw, want)
 
 
+def test_stream_0_is_the_default_stream(workspace):
+    """A workspace made for stream 0, and a call there, while another stream is the current one and busy."""
+    case = paged_case([1, 40], [900, 300], 8, 2, 128, 16, BF16)
+    want = run(case, workspace)
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        dirty = torch.full((workspace.tensor.numel(),), 255, dtype=torch.uint8, device="cuda")
+        torch.cuda.synchronize()
+        del dirty
+        torch.cuda._sleep(50_000_000)
+        made = AttentionWorkspace("cuda", stream=0)
+        with torch.cuda.stream(torch.cuda.default_stream()):
+            head = made.tensor[:65536].clone()
+    torch.cuda.synchronize()
+    assert not head.any()
+    with torch.cuda.stream(side):
+        torch.cuda._sleep(50_000_000)
+        got = run(case, None, stream=0)
+        torch.cuda.default_stream().synchronize()
+        assert not side.query()
+    torch.cuda.synchronize()
+    assert torch.equal(got, want)
+
+
 def test_a_graph_replays_the_call_at_other_lengths(workspace):
     """Lengths live on the device: a captured call follows them."""
     for q_lens, kv_lens, shared in (([1, 1, 1], [800, 300, 50], 0), ([64, 64], [500, 400], 0), ([1, 1], [40, 60], 700)):
