@@ -21,6 +21,18 @@ def stream_of(handle: int, device: torch.device) -> torch.cuda.Stream:
     return torch.cuda.ExternalStream(handle, device) if handle else torch.cuda.default_stream(device)
 
 
+def output_like(query: torch.Tensor, stream: int | None) -> torch.Tensor:
+    """An uninitialised contiguous tensor of the queries' shape that a launch on `stream` (a cudaStream_t; None: the current
+    stream) may write at once. It is that stream's memory: what is still queued on the current stream for memory freed
+    there cannot reach it. The current stream, where the caller goes on, is made known to the allocator."""
+    if stream is None or not query.is_cuda:
+        return torch.empty_like(query, memory_format=torch.contiguous_format)  # half the cost of torch.empty
+    with torch.cuda.stream(stream_of(stream, query.device)):
+        out = torch.empty_like(query, memory_format=torch.contiguous_format)
+    out.record_stream(torch.cuda.current_stream(query.device))
+    return out
+
+
 def call(device: int, function, *args) -> None:
     """Calls a library function that launches on the current device, with `device` as that; raises for an error."""
     if torch.cuda.current_device() == device:

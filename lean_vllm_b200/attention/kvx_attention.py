@@ -12,7 +12,7 @@ import torch
 
 from lean_vllm_b200 import _native
 from lean_vllm_b200._native import check, lib
-from lean_vllm_b200.attention.device import call, calls, raw_stream, stream_of
+from lean_vllm_b200.attention.device import call, calls, output_like, raw_stream, stream_of
 
 _INT32_MAX = 2**31 - 1
 _DTYPES = {torch.bfloat16: _native.BF16, torch.float16: _native.FP16}
@@ -92,18 +92,14 @@ def _attention(query, k_cache, v_cache, block_tables, kv_lens, scale, q_starts, 
         shared_blocks = shared_table.numel()
         shared = _int32("prefix_table", shared_table, (shared_blocks,), device)
     if out is None:
-        out = torch.empty_like(query, memory_format=torch.contiguous_format)  # half the cost of torch.empty
+        out = output_like(query, stream)
         o0, o1 = q_heads * head_dim, head_dim
-        if stream is not None:  # the caching allocator has to know who writes it
-            out.record_stream(stream_of(stream, query.device))
     else:
         o0, o1, o2 = out.stride() if out.dim() == 3 else (0, 0, 0)
         if out.shape != shape or out.dtype != dtype or out.get_device() != device or o2 != 1:
             raise ValueError("`out` must have the queries' shape, dtype and device, a head's elements contiguous")
     if workspace is None:
-        workspace = AttentionWorkspace(query.device, stream)
-        if stream is not None:
-            workspace.tensor.record_stream(stream_of(stream, query.device))
+        workspace = AttentionWorkspace(query.device, stream)  # on the launch's stream, and freed there
     elif workspace.index != device:
         raise ValueError("the workspace must be on the queries' device")
     args = _native.ATTENTION_ARGS.pack(

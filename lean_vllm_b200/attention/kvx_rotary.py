@@ -17,7 +17,7 @@ import torch
 
 from lean_vllm_b200 import _native
 from lean_vllm_b200._native import check, lib
-from lean_vllm_b200.attention.device import call, calls, raw_stream, stream_of
+from lean_vllm_b200.attention.device import call, calls, output_like, raw_stream
 from lean_vllm_b200.attention.kvx_cache import PushTarget, _dest, _slots, _target_slots
 
 _DTYPES = {torch.bfloat16: _native.BF16, torch.float16: _native.FP16}
@@ -142,10 +142,8 @@ def _launch(rows: tuple, out, rotary: RotaryTable, positions: torch.Tensor, posi
 
 def _output(query: torch.Tensor, out: torch.Tensor | None, stream: int | None) -> torch.Tensor:
     if out is None:
-        out = torch.empty_like(query, memory_format=torch.contiguous_format)  # half the cost of torch.empty
-        if stream is not None and query.is_cuda:  # the caching allocator has to know who writes it
-            out.record_stream(stream_of(stream, query.device))
-    elif out.shape != query.shape or out.dtype != query.dtype or out.device != query.device or out.stride(-1) != 1:
+        return output_like(query, stream)
+    if out.shape != query.shape or out.dtype != query.dtype or out.device != query.device or out.stride(-1) != 1:
         raise ValueError("`out` must have the queries' shape, dtype and device, a head's elements contiguous")
     return out
 

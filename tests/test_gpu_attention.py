@@ -372,6 +372,27 @@ def test_other_streams(workspace):
         assert torch.equal(raw, want)
 
 
+def test_an_output_made_for_another_stream_waits_for_nobody(workspace):
+    """Work still queued on the current stream on memory that was freed there does not reach an output (or a workspace)
+    made for a call on another stream."""
+    case = paged_case([200], [900], 32, 8, 128, 16, BF16)
+    want = run(case, workspace)
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        own = AttentionWorkspace("cuda")
+    for mine in (own, None):
+        torch.cuda.synchronize()
+        torch.cuda.empty_cache()
+        taken = [torch.empty_like(case["q"]), torch.empty_like(own.tensor)]
+        torch.cuda._sleep(50_000_000)  # tens of ms
+        for t in taken:
+            t.fill_(1)
+        del taken, t
+        got = run(case, mine, stream=side.cuda_stream)
+        torch.cuda.synchronize()
+        assert torch.equal(got, want)
+
+
 def test_stream_0_is_the_default_stream(workspace):
     """A workspace made for stream 0, and a call there, while another stream is the current one and busy."""
     case = paged_case([1, 40], [900, 300], 8, 2, 128, 16, BF16)

@@ -296,6 +296,26 @@ def test_another_stream_runs_the_call_in_its_own_order():
     assert torch.equal(raw, want)
 
 
+def test_an_output_made_for_another_stream_waits_for_nobody():
+    """Work still queued on the current stream on memory that was freed there does not reach the queries made for a call on
+    another stream (stream 0 among them)."""
+    q, k, v, cache, slots, table, at, weights = rows_case(500, 8, 2, 128, 128, 16, torch.bfloat16)
+    view = cache.transpose(2, 3)
+    want = rotate_store_kvcache(q, k, v, view[0], view[1], slots, at, table)
+    side = torch.cuda.Stream()
+    for current, other in ((torch.cuda.current_stream(), side), (side, torch.cuda.default_stream())):
+        torch.cuda.synchronize()
+        torch.cuda.empty_cache()
+        with torch.cuda.stream(current):
+            taken = torch.empty_like(want)
+            torch.cuda._sleep(50_000_000)  # tens of ms
+            taken.fill_(1)
+            del taken
+            got = rotate_store_kvcache(q, k, v, view[0], view[1], slots, at, table, stream=other.cuda_stream)
+        torch.cuda.synchronize()
+        assert torch.equal(got, want)
+
+
 def test_a_graph_replays_the_call():
     q, k, v, cache, slots, table, at, weights = rows_case(16, 8, 2, 128, 128, 16, torch.bfloat16, fused=False)
     view = cache.transpose(2, 3)
