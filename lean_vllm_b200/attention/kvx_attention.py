@@ -127,9 +127,9 @@ def paged_attention(query: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.T
     A row sees the keys up to its own position; with `window`, only the last `window` of them; with `prefix_lens` (int32
     [batch]), also every key below its sequence's, whatever its position. Scores are `scale` (1/sqrt(dim)) times q.k,
     capped to softcap * tanh(score / softcap) when `softcap` is given, plus slopes[head] * (key - query position) when
-    `slopes` (float32 [heads]) are. A row that sees nothing gets zeros. Cache rows past a sequence's length are never
-    used, whatever they hold. Inside it, a value that one row sees must be finite for the rows beside it too (they
-    multiply it by zero).
+    `slopes` (float32 [heads]) are. A row that sees nothing gets zeros. Cache rows past a sequence's length, ahead of its
+    first row's window and between a prefix and that window are never used, whatever they or the table there hold. A value
+    that one row sees must be finite for the rows beside it too (they multiply it by zero).
 
     `max_q_len` and `max_kv_len` bound the lengths (the device holds them): they choose the launch's shape only. Without
     q_starts `max_q_len` means nothing.

@@ -103,17 +103,21 @@ __device__ __forceinline__ int64_t quotient(int64_t a, int64_t b) {
 
 // A sequence's share of the launch's tiles.
 struct RowWork {
-    int32_t lo, row_tiles, tiles;  // first key, tiles of rows, tiles of keys per group
+    int32_t lo;                // first key of the window, the prefix's lying ahead of it ...
+    int32_t front, skip;       // ... in the first tiles of keys, behind which some are left out
+    int32_t row_tiles, tiles;  // tiles of rows, tiles of keys per group
     __device__ __forceinline__ int64_t groups(const AttnParams &p) const { return (int64_t)row_tiles * p.kv_heads; }
 };
 
 template <int ROWS>
 __device__ __forceinline__ RowWork row_work(const AttnParams &p, const Sequence &q) {
     RowWork w;
-    w.lo = first_seen(p, q, q.kv_len - q.q_len);
+    w.lo = window_start(p, q.kv_len - q.q_len);
+    w.front = (q.prefix + kTileTokens - 1) / kTileTokens;
+    w.skip = max(0, w.lo / kTileTokens - w.front);
     w.row_tiles = (int32_t)(((int64_t)q.q_len * p.group + ROWS - 1) / ROWS);
     // An empty cache still gets one (empty) tile: its rows have to be written.
-    w.tiles = max(1, (q.kv_len + kTileTokens - 1) / kTileTokens - w.lo / kTileTokens);
+    w.tiles = max(1, (q.kv_len + kTileTokens - 1) / kTileTokens - w.skip);
     return w;
 }
 
@@ -294,28 +298,35 @@ attention_rows(const __grid_constant__ AttnParams p) {
             if (row >= rows) return 0;
             return p.query + (int64_t)(q.q0 + token_of(row)) * p.q_token_stride + (int64_t)head_of(row) * p.q_head_stride;
         };
-        const int first_token = work.lo / kTileTokens * kTileTokens + tile0 * kTileTokens + warp * kWarpTokens;
+        auto stage_token = [&](int i) {
+            return (tile0 + i + (tile0 + i >= work.front ? work.skip : 0)) * kTileTokens + warp * kWarpTokens;
+        };
+        const uint32_t gap = max(0, work.lo - q.prefix);  // tokens between the prefix and the window
+        auto readable = [&](int t) { return t < q.kv_len && (uint32_t)(t - q.prefix) >= gap; };
         const int64_t lane_from = (int64_t)h * p.head_stride +
                                   (stage_in_block ? (lane / kChunks) * p.token_stride + (lane % kChunks) * 16 : 0);
 
         // Where stage i's tokens lie: in one block, this lane's first copy; else this lane's token (lanes 0-15). A byte
         // offset, or -1 where nothing is to be read.
         auto stage_offset = [&](int i) -> int64_t {
-            const int t = first_token + i * kTileTokens + (stage_in_block ? 0 : lane);
-            if (i >= n_tiles || t >= q.kv_len) return -1;
-            if (stage_in_block ? t + kWarpTokens <= work.lo : lane >= kWarpTokens || t < work.lo) return -1;
+            if (i >= n_tiles) return -1;
+            const int t = stage_token(i) + (stage_in_block ? 0 : lane);
+            // (Of a stage in one block some token has to be there, so that the block's id is one.)
+            if (stage_in_block ? t >= q.kv_len || (t + kWarpTokens <= work.lo && t >= q.prefix)
+                               : lane >= kWarpTokens || !readable(t))
+                return -1;
             const int64_t at = token_at(p, s, t);
             return at < 0 ? -1 : at + lane_from;
         };
         auto load_stage = [&](int i, int64_t offset) {
             const uint32_t k_stage = ring + (i % kStages) * 2 * kStageBytes + lane_to;
             if (stage_in_block) {
-                const int t = first_token + i * kTileTokens + lane / kChunks;
+                const int t = stage_token(i) + lane / kChunks;
                 uint64_t key = p.k_cache + (offset < 0 ? 0 : offset), value = p.v_cache + (offset < 0 ? 0 : offset);
 #pragma unroll
                 for (int c = 0; c < kCopies; ++c) {
                     const int token = c * kPerCopy + lane / kChunks;
-                    const bool valid = offset >= 0 && t + c * kPerCopy >= work.lo && t + c * kPerCopy < q.kv_len;
+                    const bool valid = offset >= 0 && readable(t + c * kPerCopy);
                     const uint32_t to = k_stage + c * kPerCopy * D * 2 + (((lane % kChunks) ^ (token & 7)) << 4);
                     cp_async16(to, reinterpret_cast<const void *>(key), valid);
                     cp_async16(to + kStageBytes, reinterpret_cast<const void *>(value), valid);
@@ -377,7 +388,7 @@ attention_rows(const __grid_constant__ AttnParams p) {
         // Every row of the tile sees the keys from see_lo up to see_hi: whole stages in there need no mask.
         const int first_position = q.kv_len - q.q_len + token_of(0);
         const int last_position = q.kv_len - q.q_len + token_of(rows - 1);
-        const int see_lo = p.window > 0 ? max(work.lo, last_position - p.window + 1) : 0;
+        const int see_lo = p.window > 0 ? last_position - p.window + 1 : 0;
         const int see_hi = min(q.kv_len, first_position + 1);
 
         // ---- the walk over the keys. c holds a stage's 16 tokens x ROWS scores: c[n][e] belongs to this lane's row
@@ -394,7 +405,7 @@ attention_rows(const __grid_constant__ AttnParams p) {
             asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 1) : "memory");
             __syncwarp();
             const uint32_t k_stage = ring + (i % kStages) * 2 * kStageBytes, v_stage = k_stage + kStageBytes;
-            const int t0 = first_token + i * kTileTokens;
+            const int t0 = stage_token(i);
 
             float c[kScores][4] = {};
             if (ROWS == 8) {
@@ -436,7 +447,7 @@ attention_rows(const __grid_constant__ AttnParams p) {
                         x = c[n][e] * scale_log2;
                     }
                     if (masked) {
-                        const bool seen = t < q.kv_len && t >= work.lo &&
+                        const bool seen = t < q.kv_len &&
                                           ((t <= position[r] && (p.window <= 0 || t > position[r] - p.window)) ||
                                            t < prefix[r]);
                         x = seen ? x : -INFINITY;

@@ -114,9 +114,10 @@ __device__ __forceinline__ int64_t token_at(const AttnParams &p, int s, int32_t 
     return (int64_t)id * p.block_stride + (int64_t)(t - b * p.block_size) * p.token_stride;
 }
 
-// The first key that any row from position `first_position` on can see.
-__device__ __forceinline__ int32_t first_seen(const AttnParams &p, const Sequence &q, int32_t first_position) {
-    return p.window > 0 && q.prefix == 0 ? max(0, first_position - p.window + 1) : 0;
+// The first key that any row from position `first_position` on can see, but for those below the sequence's prefix. What lies
+// between the two is never read: its blocks may be gone.
+__device__ __forceinline__ int32_t window_start(const AttnParams &p, int32_t first_position) {
+    return p.window > 0 ? max(0, first_position - p.window + 1) : 0;
 }
 
 // 2^x for a difference of running maxima: a maximum of -inf (nothing seen yet) contributes nothing.

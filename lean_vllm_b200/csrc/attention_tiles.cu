@@ -84,11 +84,13 @@ struct Item {
     Sequence q;
     int32_t valid;               // 0: no more work
     int32_t sequence, head, token0, tokens, split;  // tokens: of the sequence's (or the batch's) from token0 on
-    int32_t lo, hi;              // own keys that any row sees
-    int32_t shared_tiles, tiles; // tiles of the shared prefix walked first, and all of this split's ...
+    int32_t lo, hi;              // own keys that any row sees, behind ...
+    int32_t front;               // ... those walked first, all rows seeing them: the shared prefix, or the sequence's own one
+                                 // where a window leaves keys out behind it
+    int32_t front_tiles, tiles;  // their tiles, and all of this split's ...
     int32_t first_tile;          // ... from this one of the item's on
-    int32_t lo_tile;             // first tile of own keys
 };
+static_assert(sizeof(Item) == 64, "four 16-byte reads: with one field more a prompt of 8192 tokens took 553 us, not 537");
 
 // ---- tcgen05
 
@@ -309,9 +311,10 @@ __device__ bool find_item(const TileParams &t, int id, Item &item, int &count) {
         item.q = Sequence{0, p.num_tokens, p.shared_len, 0};
         item.token0 = r * t.item_tokens;
         item.tokens = min(t.item_tokens, p.num_tokens - item.token0);
-        item.lo = item.hi = item.lo_tile = 0;
-        item.shared_tiles = (p.shared_len + kTileKeys - 1) / kTileKeys;
-        item.tiles = item.shared_tiles;
+        item.lo = item.hi = 0;
+        item.front = p.shared_len;
+        item.front_tiles = (p.shared_len + kTileKeys - 1) / kTileKeys;
+        item.tiles = item.front_tiles;
     } else {
         auto tiles_of = [&](const Sequence &q) {
             return (int64_t)q.q_len * p.group > p.rows_limit ? (q.q_len + t.item_tokens - 1) / t.item_tokens : 0;
@@ -353,11 +356,12 @@ __device__ bool find_item(const TileParams &t, int id, Item &item, int &count) {
         const int own = item.q.kv_len - p.shared_len;
         const int first = own - item.q.q_len + item.token0, last = first + item.tokens - 1;
         const int prefix = item.q.prefix - p.shared_len;  // beyond a shared prefix there is none
-        item.lo = p.window > 0 && prefix <= 0 ? max(0, first - p.window + 1) : 0;
+        const int window = window_start(p, first);  // behind the prefix: what lies between may be gone, and is left out
+        item.lo = window > prefix ? window : 0;
+        item.front = p.shared_len + (window > prefix ? prefix : 0);
         item.hi = max(max(0, min(own, last + 1)), prefix);
-        item.lo_tile = item.lo / kTileKeys;
-        item.shared_tiles = (p.shared_len + kTileKeys - 1) / kTileKeys;
-        item.tiles = item.shared_tiles + max(0, (item.hi + kTileKeys - 1) / kTileKeys - item.lo_tile);
+        item.front_tiles = (item.front + kTileKeys - 1) / kTileKeys;
+        item.tiles = item.front_tiles + max(0, (item.hi + kTileKeys - 1) / kTileKeys - item.lo / kTileKeys);
     }
     item.valid = 1;
     item.first_tile = 0;
@@ -369,19 +373,19 @@ __device__ bool find_item(const TileParams &t, int id, Item &item, int &count) {
     return true;
 }
 
-// Tile i of the CTA's walk: its first key and the keys of it that are there to read, in the shared prefix's numbering
-// or the sequence's own.
+// Tile i of the CTA's walk: its first key and the keys of it that are there to read, in the front stretch or behind it (in
+// the sequence's own numbering; of a shared prefix, in the prefix's).
 struct TileAt {
-    bool shared;
+    bool front;
     int32_t t0, lo, hi;
 };
-__device__ __forceinline__ TileAt tile_at(const AttnParams &p, const Item &item, int i) {
+__device__ __forceinline__ TileAt tile_at(const Item &item, int i) {
     const int n = item.first_tile + i;
     TileAt at;
-    at.shared = n < item.shared_tiles;
-    at.t0 = (at.shared ? n : n - item.shared_tiles + item.lo_tile) * kTileKeys;
-    at.lo = at.shared ? 0 : item.lo;
-    at.hi = at.shared ? p.shared_len : item.hi;
+    at.front = n < item.front_tiles;
+    at.t0 = (at.front ? n : n - item.front_tiles + item.lo / kTileKeys) * kTileKeys;
+    at.lo = at.front ? 0 : item.lo;
+    at.hi = at.front ? item.front : item.hi;
     return at;
 }
 
@@ -475,7 +479,8 @@ attention_tiles(const __grid_constant__ TileParams t) {
             const bool valid = row_token < t.tile_tokens && in_item < item.tokens;
             const int token = item.token0 + (valid ? in_item : 0);
             const int head = item.head * p.group + row_head;
-            // What the row sees of its sequence's own keys: [see_lo, see_hi) and everything below see_below.
+            // What the row sees of its sequence's own keys, behind the front stretch if there is one: [see_lo, see_hi) and
+            // everything below see_below.
             int position = 0, see_lo = 0, see_hi = 0, see_below = 0;
             float slope = 0.f;
             if (t.prefix_only) {
@@ -488,7 +493,7 @@ attention_tiles(const __grid_constant__ TileParams t) {
                 const int stands = own - item.q.q_len + token;
                 see_hi = min(own, stands + 1);
                 see_lo = p.window > 0 ? max(0, stands - p.window + 1) : 0;
-                see_below = item.q.prefix - p.shared_len;
+                see_below = item.lo > 0 ? 0 : item.q.prefix - p.shared_len;
                 position = stands + p.shared_len;
             }
             if (MODS && p.slopes && valid) slope = p.slopes[head] * kLog2e;
@@ -499,7 +504,7 @@ attention_tiles(const __grid_constant__ TileParams t) {
             // would be its smallest product: those take the way through TMEM.)
             bool look_near = MODS && p.softcap > 0.f && p.scale > 0.f && !p.slopes;
             for (int i = 0; i < item.tiles; ++i) {
-                const TileAt at = tile_at(p, item, i);
+                const TileAt at = tile_at(item, i);
                 if (!warp_waits(smem_u32(&scores[g]), score_phase, &gave_up)) {
                     ok = false;
                     break;
@@ -508,9 +513,9 @@ attention_tiles(const __grid_constant__ TileParams t) {
                 fence_after();
                 // Scores that a mask, cap or bias changes go back to TMEM as they are then, 32 columns at a time.
                 const bool sees_all = !valid ? true
-                                      : at.shared ? at.t0 + kTileKeys <= p.shared_len
-                                                  : (at.t0 >= see_lo && at.t0 + kTileKeys <= see_hi) ||
-                                                        at.t0 + kTileKeys <= see_below;
+                                      : at.front ? at.t0 + kTileKeys <= at.hi
+                                                 : (at.t0 >= see_lo && at.t0 + kTileKeys <= see_hi) ||
+                                                       at.t0 + kTileKeys <= see_below;
                 const bool masked = !__all_sync(~0u, sees_all);
                 float x[4][32];
                 // A cap alone whose scores are near needs no way back through TMEM: the weights' loop below caps them.
@@ -525,9 +530,9 @@ attention_tiles(const __grid_constant__ TileParams t) {
                     near_tile = look_near = __all_sync(~0u, most <= near.reach);
                 }
                 if ((MODS || masked) && !near_tile) {
-                    int from = (at.shared ? 0 : see_lo) - at.t0, to = (at.shared ? p.shared_len : see_hi) - at.t0;
-                    int below = (at.shared ? 0 : see_below) - at.t0;
-                    float offset = MODS ? (float)((at.shared ? 0 : p.shared_len) + at.t0 - position) : 0.f;
+                    int from = (at.front ? 0 : see_lo) - at.t0, to = (at.front ? at.hi : see_hi) - at.t0;
+                    int below = (at.front ? 0 : see_below) - at.t0;
+                    float offset = MODS ? (float)((at.front ? 0 : p.shared_len) + at.t0 - position) : 0.f;
 #pragma unroll 1
                     for (int c = 0; c < 4; ++c, from -= 32, to -= 32, below -= 32, offset += 32.f) {
                         float y[32];
@@ -596,7 +601,8 @@ attention_tiles(const __grid_constant__ TileParams t) {
                         }
                     }
                 }
-                // Values that no row sees (past the length, ahead of the window) may hold anything: 0 times NaN is NaN.
+                // Values that no row sees (past the length, past a front stretch, ahead of the window) may hold anything: 0
+                // times NaN is NaN.
                 if (at.t0 < at.lo || at.t0 + kTileKeys > at.hi) {
                     const int copy = 2 * (ring_at + i) + 1, slot = copy % S::kSlots;
                     if (!warp_waits(smem_u32(&full[slot]), (copy / S::kSlots) & 1, &gave_up)) {
@@ -818,15 +824,16 @@ attention_tiles(const __grid_constant__ TileParams t) {
         Item item;
         for (int n = 0; ok && next_item(n, item); ++n) {
             const int32_t *own_table = p.block_tables + (int64_t)item.sequence * p.table_stride;
+            const int32_t *front_table = p.shared_len > 0 ? p.shared_table : own_table;
             for (int i = 0; ok && i < item.tiles; ++i) {
-                const TileAt at = tile_at(p, item, i);
+                const TileAt at = tile_at(item, i);
                 const int k = at.t0 + box * t.box;
                 const bool wanted = lane < copies && k < at.hi && k + t.box > at.lo;
                 int block = 0, in_block = 0;
                 if (wanted) {
                     const int b = p.block_shift >= 0 ? k >> p.block_shift : k / p.block_size;
                     in_block = k - b * p.block_size;
-                    block = (at.shared ? p.shared_table : own_table)[b];
+                    block = (at.front ? front_table : own_table)[b];
                     if (block < 0 || block >= p.num_blocks) {
                         flag_error(p.error_word, p.status, kErrPastCache);
                         block = p.num_blocks;  // past the tensor: the copy fills in zeros

@@ -161,6 +161,31 @@ def test_a_window_never_reads_what_lies_before_it(workspace):
     check(case, workspace, window=100)
 
 
+@pytest.mark.parametrize("prefix", [1, 5, 64, 70, 200, 640, 899, 10000])
+@pytest.mark.parametrize("q_lens, kv_lens, heads, kv_heads, dim, block, options", [
+    ([1, 1, 1], [1000, 2001, 150], 8, 2, 128, 16, {}),
+    ([4, 2], [1000, 777], 8, 2, 64, 24, {}),
+    ([1, 3], [1000, 650], 4, 2, 128, 7, {}),                           # blocks that lie in no stage of keys
+    ([20, 300], [1000, 900], 8, 2, 128, 16, {}),
+    ([130, 1], [1500, 1300], 4, 1, 64, 64, {}),
+    ([60], [9000], 4, 1, 128, 16, {}),                                 # cut along the keys
+    ([200, 1], [1200, 1200], 8, 2, 128, 16, {"softcap": 20.0}),
+], ids=["decode", "drafts64", "odd", "chunks", "chunks64", "cut", "capped"])
+def test_what_lies_between_a_prefix_and_the_window_is_never_read(q_lens, kv_lens, heads, kv_heads, dim, block, options,
+                                                                 prefix, workspace):
+    """First tokens and a sliding window: keys and values between the two may be gone, NaN rows and stale table entries."""
+    case = paged_case(q_lens, kv_lens, heads, kv_heads, dim, block, BF16)
+    for s, (q_len, n) in enumerate(zip(q_lens, kv_lens)):
+        gap = torch.arange(min(prefix, n), max(n - q_len - 100 + 1, min(prefix, n)), device="cuda")
+        case["k_cache"][case["tables"][s][gap // block].long(), gap % block] = math.nan
+        case["v_cache"][case["tables"][s][gap // block].long(), gap % block] = math.nan
+        blocks = torch.arange(case["tables"].size(1), device="cuda")
+        stale = (blocks * block >= prefix) & ((blocks + 1) * block <= n - q_len - 100 + 1)
+        case["tables"][s][stale] = torch.where(blocks[stale] % 2 == 0, -1, 2**30).to(torch.int32)
+    check(case, workspace, window=100, prefix_lens=torch.full((len(q_lens),), prefix, dtype=torch.int32, device="cuda"),
+          **options)
+
+
 @pytest.mark.parametrize("q_lens, kv_lens, shared, heads, kv_heads, dim, block, dtype, hnd", [
     ([1] * 3, [1, 17, 40], 100, 8, 2, 128, 16, BF16, True),
     ([1] * 64, list(range(1, 65)), 1000, 32, 8, 128, 256, BF16, True),
