@@ -388,7 +388,7 @@ attention_rows(const __grid_constant__ AttnParams p) {
         // Every row of the tile sees the keys from see_lo up to see_hi: whole stages in there need no mask.
         const int first_position = q.kv_len - q.q_len + token_of(0);
         const int last_position = q.kv_len - q.q_len + token_of(rows - 1);
-        const int see_lo = p.window > 0 ? last_position - p.window + 1 : 0;
+        const int see_lo = window_start(p, last_position);
         const int see_hi = min(q.kv_len, first_position + 1);
 
         // ---- the walk over the keys. c holds a stage's 16 tokens x ROWS scores: c[n][e] belongs to this lane's row

@@ -115,9 +115,10 @@ __device__ __forceinline__ int64_t token_at(const AttnParams &p, int s, int32_t 
 }
 
 // The first key that any row from position `first_position` on can see, but for those below the sequence's prefix. What lies
-// between the two is never read: its blocks may be gone.
+// between the two is never read: its blocks may be gone. (Positions ahead of the first key are negative: taken as they are,
+// the subtraction of a window near 2^31 would wrap, and a walk begin outside the table.)
 __device__ __forceinline__ int32_t window_start(const AttnParams &p, int32_t first_position) {
-    return p.window > 0 ? max(0, first_position - p.window + 1) : 0;
+    return p.window > 0 ? max(0, max(0, first_position) - p.window + 1) : 0;
 }
 
 // 2^x for a difference of running maxima: a maximum of -inf (nothing seen yet) contributes nothing.

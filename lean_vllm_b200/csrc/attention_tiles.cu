@@ -492,7 +492,7 @@ attention_tiles(const __grid_constant__ TileParams t) {
                 const int own = item.q.kv_len - p.shared_len;
                 const int stands = own - item.q.q_len + token;
                 see_hi = min(own, stands + 1);
-                see_lo = p.window > 0 ? max(0, stands - p.window + 1) : 0;
+                see_lo = window_start(p, stands);
                 see_below = item.lo > 0 ? 0 : item.q.prefix - p.shared_len;
                 position = stands + p.shared_len;
             }

@@ -161,6 +161,13 @@ def test_a_window_never_reads_what_lies_before_it(workspace):
     check(case, workspace, window=100)
 
 
+@pytest.mark.parametrize("q_len, kv_len", [(4, 2), (10, 3), (300, 260), (5, 0)])
+@pytest.mark.parametrize("window", [2**31 - 1, 2**31 - 200])
+def test_the_widest_windows_see_everything(q_len, kv_len, window, workspace):
+    """Also for queries that stand ahead of the first key."""
+    check(paged_case([q_len], [kv_len], 4, 2, 64, 16, BF16), workspace, window=window)
+
+
 @pytest.mark.parametrize("prefix", [1, 5, 64, 70, 200, 640, 899, 10000])
 @pytest.mark.parametrize("q_lens, kv_lens, heads, kv_heads, dim, block, options", [
     ([1, 1, 1], [1000, 2001, 150], 8, 2, 128, 16, {}),
