@@ -252,7 +252,7 @@ typedef struct kvx_attention_args {
     int32_t *status;            /* status word or NULL: bit 2 for a block id past the cache or a length past its table,
                                    bit 16 for a bounded wait that ran out: then neither the output nor the workspace
                                    is to be used any further */
-    int32_t shared_len;         /* tokens of the shared prefix */
+    int32_t shared_len;         /* tokens of the shared prefix; with max_blocks * block_size 2^31 - 1024 at most */
     int32_t shared_blocks;      /* entries of shared_table */
     int32_t block_size;
     int32_t num_blocks;

@@ -763,8 +763,9 @@ int kvx_attention(const kvx_attention_args *args, int flags, void *stream) {
     if (a.block_size < 1 || a.num_blocks < 0 || a.max_blocks < 0 || a.table_stride < 0 || a.shared_len < 0 ||
         a.shared_blocks < 0)
         return fail(KVX_ERR_INVALID, "bad block size, block count or table");
-    if ((int64_t)a.max_blocks * a.block_size >= (int64_t)1 << 31 || a.shared_len >= 1 << 30)
-        return fail(KVX_ERR_INVALID, "more than 2^31 tokens a sequence");
+    // Positions and the ends of tiles stay below 2^31.
+    if ((int64_t)a.max_blocks * a.block_size + a.shared_len > ((int64_t)1 << 31) - 1024)
+        return fail(KVX_ERR_INVALID, "more than 2^31 - 1024 tokens a sequence");
     if (a.window < 0 || !(a.softcap >= 0.f)) return fail(KVX_ERR_INVALID, "negative window or softcap");
     if ((int64_t)a.shared_blocks * a.block_size < a.shared_len)
         return fail(KVX_ERR_RANGE, "a shared prefix of %d tokens in %d blocks of %d", a.shared_len, a.shared_blocks,

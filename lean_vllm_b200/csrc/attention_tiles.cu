@@ -365,10 +365,11 @@ __device__ bool find_item(const TileParams &t, int id, Item &item, int &count) {
     }
     item.valid = 1;
     item.first_tile = 0;
-    if (t.splits > 1) {  // tiles x splits stays below 2^32: 2^31 tokens in tiles of 128, a split per SM at most
-        const uint32_t tiles = item.tiles, splits = t.splits;
-        item.first_tile = (int)(tiles * (uint32_t)item.split / splits);
-        item.tiles = (int)(tiles * (uint32_t)(item.split + 1) / splits) - item.first_tile;
+    if (t.splits > 1) {  // from tiles * split / splits on, in 32 bits
+        const int each = item.tiles / t.splits, rest = item.tiles - each * t.splits;
+        auto start_of = [&](int split) { return each * split + rest * split / t.splits; };
+        item.first_tile = start_of(item.split);
+        item.tiles = start_of(item.split + 1) - item.first_tile;
     }
     return true;
 }

@@ -174,6 +174,19 @@ def test_the_abi_refuses_attention_arguments(change, message):
         in_a_thread(lambda: _native.check(_native.lib().kvx_attention(ctypes.addressof(struct), 0, None)))
 
 
+@pytest.mark.parametrize("change", [
+    dict(block_size=1, max_blocks=2**31 - 1), dict(block_size=128, max_blocks=2**24 - 1),
+    dict(block_size=1 << 20, max_blocks=2047, shared_len=1 << 29, shared_blocks=1 << 9, shared_table=16),
+    dict(block_size=1 << 20, shared_len=2**31 - 1, shared_blocks=1 << 11, shared_table=16),
+], ids=["table", "last tile", "both", "shared"])
+def test_the_abi_refuses_sequences_whose_positions_pass_31_bits(change):
+    if not os.path.exists(_native.LIB_PATH):
+        pytest.skip("libkvx.so is not built here")
+    with pytest.raises(_native.KvxError, match="tokens a sequence"):
+        struct = attention_struct(**change)
+        in_a_thread(lambda: _native.check(_native.lib().kvx_attention(ctypes.addressof(struct), 0, None)))
+
+
 def test_the_abi_refuses_rotate_arguments():
     if not os.path.exists(_native.LIB_PATH):
         pytest.skip("libkvx.so is not built here")
