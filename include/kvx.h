@@ -221,7 +221,8 @@ typedef struct kvx_rotate_args {
 /* One pass over a step's queries, keys and values: each head's norm, x * rsqrt(mean(x^2) + eps) * weight, the rotation
  * of its pairs by its token's position, (a, b) -> (a cos - b sin, b cos + a sin), and the store of keys and values
  * into every destination, as kvx_store places rows (its flags and status word too; bit 8 for a position outside the
- * table). Computed in 32 bits and rounded once. What the reference's attention layers do ahead of store_kvcache
+ * table). With KVX_STORE_PEERS_ONLY the queries are left alone as destination 0 is: both are the local half's. Computed in
+ * 32 bits and rounded once. What the reference's attention layers do ahead of store_kvcache
  * (attention/triton_cache.py:58-91), in three passes. */
 int kvx_rotate_store(const kvx_rotate_args *args, const kvx_store_dest *dests, int n_dests, int32_t *status, int flags,
                      void *stream);

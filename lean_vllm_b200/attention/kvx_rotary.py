@@ -152,13 +152,16 @@ def rotate_store_kvcache(query: torch.Tensor, key: torch.Tensor, value: torch.Te
                          v_cache: torch.Tensor, slot_mapping: torch.Tensor, positions: torch.Tensor,
                          rotary: RotaryTable, *, q_weight: torch.Tensor | None = None,
                          k_weight: torch.Tensor | None = None, eps: float = 1e-6, out: torch.Tensor | None = None,
-                         push_to=(), stream: int | None = None, flags: int = 0, status: int = 0) -> torch.Tensor:
+                         push_to=(), stream: int | None = None, flags: int = 0,
+                         status: int = 0) -> torch.Tensor | None:
     """Norms (with `q_weight` / `k_weight`) and rotates queries and keys [num_tokens, heads, dim], stores keys and
     values into [num_blocks, block_size, heads, dim] caches by `slot_mapping` (as store_kvcache, `push_to` and
     `status` too) and returns the queries, in `out` when given (which may be `query` itself). Rows may be strided over
     tokens and heads (views into a fused qkv product). A position outside the table takes its nearest row and sets bit
-    8 of `status`."""
-    if out is None and stream is None and not push_to and (native := calls()) is not None:
+    8 of `status`. With STORE_PEERS_ONLY in `flags`, the push half of a store whose local half came before, only the
+    peers are written: the queries are left alone, and `out` is returned as it is (None without one)."""
+    push_half = flags & _native.STORE_PEERS_ONLY
+    if out is None and stream is None and not push_to and not push_half and (native := calls()) is not None:
         done = native.rotate_store(query, key, value, k_cache, v_cache, slot_mapping, positions, rotary.table,
                                    rotary.interleaved, q_weight, k_weight, eps, flags, status)
         if type(done) is int:
@@ -202,7 +205,8 @@ def rotate_store_kvcache(query: torch.Tensor, key: torch.Tensor, value: torch.Te
             value.data_ptr(), 2 * v0, 2 * v1, num_heads, head_dim, 0, 0, 0)
     dests = _dests(k_cache.data_ptr(), v_cache.data_ptr(), (2 * strides[0], 2 * strides[1], 2 * strides[2]), block_size,
                    num_blocks, slots, num_heads, push_to, num_tokens, key.device)
-    out = _output(query, out, stream)
+    if out is not None or not push_half:
+        out = _output(query, out, stream)
     _launch(rows, out, rotary, positions, position_bytes, num_tokens, dtype, eps, dests, stream, flags, status, device)
     return out
 
@@ -215,8 +219,9 @@ def rotate_store_latents(latent: torch.Tensor, latent_cache: torch.Tensor, slot_
     """Stores latents [num_tokens, rank + rotary_dim] into a [num_blocks, block_size, rank + rotary_dim] cache by
     `slot_mapping` (as store_latents), the leading `rank` elements normed with `weight` (where given) and the last
     rotary_dim rotated, and returns the queries' rotated part `query_pe` [num_tokens, heads, rotary_dim] rotated, in
-    `out` when given (None without queries)."""
-    if out is None and stream is None and not push_to and (native := calls()) is not None:
+    `out` when given (None without queries). STORE_PEERS_ONLY in `flags` as for rotate_store_kvcache."""
+    push_half = flags & _native.STORE_PEERS_ONLY
+    if out is None and stream is None and not push_to and not push_half and (native := calls()) is not None:
         done = native.rotate_latents(latent, latent_cache, slot_mapping, positions, rotary.table, rotary.interleaved,
                                      query_pe, weight, eps, flags, status)
         if type(done) is int:
@@ -255,7 +260,8 @@ def rotate_store_latents(latent: torch.Tensor, latent_cache: torch.Tensor, slot_
         if q2 != 1:
             raise ValueError("a head's elements must be contiguous")
         query = (query_pe.data_ptr(), 2 * q0, 2 * q1, query_pe.size(1), rotary_dim, 0, 0, 0)
-        out = _output(query_pe, out, stream)
+        if out is not None or not push_half:
+            out = _output(query_pe, out, stream)
     else:
         query, out = _NO_ROWS, None
     rows = (*query, latent.data_ptr(), 2 * l0, 0, 1, dim, normed, rank, scale, *_NO_ROWS)

@@ -530,7 +530,8 @@ extern "C" int kvx_rotate_store(const kvx_rotate_args *args, const kvx_store_des
     if (a.rotary_dim > 0 && a.num_tokens > 0 &&
         (!a.table || !a.positions || a.num_positions < 1 || (a.position_bytes != 4 && a.position_bytes != 8)))
         return fail(KVX_ERR_INVALID, "a rotation needs a table of one position at least, and 4- or 8-byte positions");
-    const bool has_query = a.query.num_heads > 0, has_value = a.value.num_heads > 0;
+    // The push half of a store leaves the queries to the local half, which may have rotated them in place.
+    const bool has_query = a.query.num_heads > 0 && !(flags & KVX_STORE_PEERS_ONLY), has_value = a.value.num_heads > 0;
     RotateParams p{};
     if (a.num_tokens > 0) {
         if (has_query) {

@@ -4,6 +4,7 @@ for bit, and what it flags."""
 import pytest
 import torch
 
+from lean_vllm_b200._native import STORE_PEERS_ONLY
 from lean_vllm_b200.attention.kvx_cache import PushTarget, store_kvcache, store_latents
 from lean_vllm_b200.attention.kvx_rotary import RotaryTable, rotate_store_kvcache, rotate_store_latents
 from lean_vllm_b200.kv_transfer import transport
@@ -314,6 +315,56 @@ def test_an_output_made_for_another_stream_waits_for_nobody():
             got = rotate_store_kvcache(q, k, v, view[0], view[1], slots, at, table, stream=other.cuda_stream)
         torch.cuda.synchronize()
         assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("dim, rotary", [(128, 128), (80, 80)], ids=["vector", "any"])
+def test_the_push_half_of_a_store_leaves_the_queries_alone(dim, rotary):
+    """STORE_PEERS_ONLY: the peers get the rows that the local half stored, the local cache and the queries, rotated by the
+    local half (in place, here), stay as they are, and without `out` there are none to return."""
+    q, k, v, cache, slots, table, at, weights = rows_case(65, 6, 2, dim, rotary, 16, torch.bfloat16, fused=False)
+    view, peer = cache.transpose(2, 3), torch.zeros_like(cache)
+    target = PushTarget.of(peer.transpose(2, 3)[0], peer.transpose(2, 3)[1], slots)
+
+    def call(**more):
+        return rotate_store_kvcache(q, k, v, view[0], view[1], slots, at, table, q_weight=weights[0],
+                                    k_weight=weights[1], **more)
+
+    call(out=q)
+    rotated, local = q.clone(), cache.clone()
+    assert call(out=q, push_to=[target], flags=STORE_PEERS_ONLY) is q
+    assert call(push_to=[target], flags=STORE_PEERS_ONLY) is None and call(flags=STORE_PEERS_ONLY) is None
+    torch.cuda.synchronize()
+    assert torch.equal(q, rotated) and torch.equal(cache, local)
+    s = slots[slots >= 0]
+    assert torch.equal(peer.transpose(2, 3)[:, s // 16, s % 16], view[:, s // 16, s % 16])
+
+
+@pytest.mark.parametrize("rank, rotary", [(512, 64), (96, 32)], ids=["vector", "any"])
+def test_peers_get_the_latents_too_and_the_push_half_alone(rank, rotary):
+    g = torch.Generator(device="cuda").manual_seed(7)
+    latent = torch.randn(90, rank + rotary, generator=g, device="cuda").to(torch.bfloat16)
+    pe = torch.randn(90, 5, rotary, generator=g, device="cuda").to(torch.bfloat16)
+    weight = (1 + 0.3 * torch.randn(rank, generator=g, device="cuda")).to(torch.bfloat16)
+    table, at = RotaryTable.build(300, rotary), torch.randint(0, 300, (90,), generator=g, device="cuda")
+    slots, other = (torch.randperm(160, generator=g, device="cuda")[:90] for _ in range(2))
+    cache, peers = (torch.zeros(n, 10, 16, rank + rotary, dtype=torch.bfloat16, device="cuda") for n in (1, 2))
+    block_map = torch.randperm(10, generator=g, device="cuda").to(torch.int32)
+    targets = [PushTarget.of(peers[0], None, other), PushTarget.of(peers[1], None, None, block_map=block_map)]
+
+    def call(**more):
+        return rotate_store_latents(latent, cache[0], slots, at, table, query_pe=pe, weight=weight, **more)
+
+    want = call(push_to=targets)
+    rows = cache[0].flatten(0, 1)[slots]
+    assert torch.equal(peers[0].flatten(0, 1)[other], rows)
+    assert torch.equal(peers[1][block_map[slots // 16].long(), slots % 16], rows)
+    peers.zero_()
+    kept = cache.clone()
+    turned = pe.clone()
+    assert call(push_to=targets, out=turned, flags=STORE_PEERS_ONLY) is turned and torch.equal(turned, pe)
+    assert torch.equal(cache, kept) and torch.equal(peers[0].flatten(0, 1)[other], rows)
+    assert call(push_to=targets, flags=STORE_PEERS_ONLY) is None
+    assert torch.equal(call(out=turned), want)
 
 
 def test_a_graph_replays_the_call():
