@@ -281,7 +281,7 @@ uint64_t kvx_attention_workspace_bytes(void);
  * holds it, or when j is below the sequence's prefix; a shared prefix lies in front of every sequence's own tokens,
  * and every row sees all of it. A row that sees nothing gets zeros. Tokens at or past kv_len are never read as numbers;
  * a block id outside the cache reads as zeros and is flagged. No counterpart in the reference's transfer path: it is
- * what its attention layers read the cache with. */
+ * what its attention layers read the cache with. `flags`: 0, or KVX_STORE_SERIAL for plain launches; others are refused. */
 int kvx_attention(const kvx_attention_args *args, int flags, void *stream);
 
 /* ---- transfers with completion (post, poll, release) ---- */

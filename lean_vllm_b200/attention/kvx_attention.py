@@ -133,6 +133,7 @@ def paged_attention(query: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.T
 
     `max_q_len` and `max_kv_len` bound the lengths (the device holds them): they choose the launch's shape only. Without
     q_starts `max_q_len` means nothing.
+    `flags` may be STORE_SERIAL: plain launches, no overlap with the kernel before.
     `status` (a StatusWord's address) gets bit 2 for a block id outside the cache, which reads as zeros, or a length past
     its table, which is cut to it."""
     return _attention(query, k_cache, v_cache, block_tables, kv_lens, scale, q_starts, max_q_len, max_kv_len, softcap,

@@ -682,48 +682,30 @@ constexpr size_t kSplitAt = KVX_ATTENTION_ZEROED + kRowPartials * (kMlBytes + kO
 constexpr size_t kWorkspaceBytes = kSplitAt + kSplitRows * (kMlBytes + kOutBytes);
 static_assert(kMaxRowCtas <= kTileCounter && (kTileCounter + 1) * sizeof(int32_t) <= KVX_ATTENTION_ZEROED, "counters");
 
-template <class Kernel, class... Args>
-int launch(Kernel kernel, int64_t grid, int threads, int smem, cudaStream_t stream, const Args &...args) {
-    if (grid > 0x7fffffff) return fail(KVX_ERR_INVALID, "more rows than a launch holds");
-    cudaLaunchConfig_t cfg = {};
-    cfg.stream = stream;
-    cudaLaunchAttribute attr;
-    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr.val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = &attr;
-    cfg.numAttrs = 1;
-    cfg.gridDim = dim3((unsigned)grid);
-    cfg.blockDim = dim3(threads);
-    cfg.dynamicSmemBytes = smem;
-    KVX_CUDA(cudaLaunchKernelEx(&cfg, kernel, args...));
-    count_launch();
-    return KVX_OK;
-}
-
 template <class T, int D, int ROWS, bool MODS>
-int launch_rows(const AttnParams &p, const Device &device, cudaStream_t stream) {
+int launch_rows(const AttnParams &p, const Device &device, const Queue &queue) {
     static AllowedSmem allowed;
     auto kernel = attention_rows<T, D, ROWS, MODS>;
     if (int rc = allowed.allow(kernel, kRowSmem<D, ROWS>, device.index)) return rc;
     return launch(kernel, std::min(RowShape<ROWS>::kCtas * device.sms, kMaxRowCtas), kRowThreads, kRowSmem<D, ROWS>,
-                  stream, p);
+                  queue, p);
 }
 
 template <class T, int D>
-int launch_rows(const AttnParams &p, int rows, bool mods, const Device &device, cudaStream_t stream) {
-    if (rows <= 8) return mods ? launch_rows<T, D, 8, true>(p, device, stream) : launch_rows<T, D, 8, false>(p, device, stream);
-    return mods ? launch_rows<T, D, 16, true>(p, device, stream) : launch_rows<T, D, 16, false>(p, device, stream);
+int launch_rows(const AttnParams &p, int rows, bool mods, const Device &device, const Queue &queue) {
+    if (rows <= 8) return mods ? launch_rows<T, D, 8, true>(p, device, queue) : launch_rows<T, D, 8, false>(p, device, queue);
+    return mods ? launch_rows<T, D, 16, true>(p, device, queue) : launch_rows<T, D, 16, false>(p, device, queue);
 }
 
 template <class T, int D>
-int launch_join(const AttnParams &p, int parts, bool mixed, const Device &device, cudaStream_t stream) {
+int launch_join(const AttnParams &p, int parts, bool mixed, const Device &device, const Queue &queue) {
     const int64_t rows = (int64_t)p.num_tokens * p.q_heads;
     constexpr int kRows = 4 * kJoinThreads / D, kAtOnce = kJoinAtOnce<D>;
     const int rounds = (parts + kAtOnce - 1) / kAtOnce, at_once = (parts + rounds - 1) / rounds;
     static AllowedSmem allowed;
     auto kernel = attention_join<T, D>;
     if (int rc = allowed.allow(kernel, kAtOnce * kJoinThreads * 16, device.index)) return rc;
-    return launch(kernel, (rows + kRows - 1) / kRows, kJoinThreads, at_once * kJoinThreads * 16, stream, p,
+    return launch(kernel, (rows + kRows - 1) / kRows, kJoinThreads, at_once * kJoinThreads * 16, queue, p,
                   parts, at_once, mixed);
 }
 
@@ -754,6 +736,7 @@ uint64_t kvx_attention_workspace_bytes(void) { return kWorkspaceBytes; }
 int kvx_attention(const kvx_attention_args *args, int flags, void *stream) {
     Range range("kvx_attention");
     if (!args) return fail(KVX_ERR_INVALID, "null arguments");
+    if (flags & ~KVX_STORE_SERIAL) return fail(KVX_ERR_INVALID, "flags %#x; KVX_STORE_SERIAL is the one there is", flags);
     const kvx_attention_args &a = *args;
     if (a.num_tokens < 0 || a.batch < 0) return fail(KVX_ERR_INVALID, "%d tokens of %d sequences", a.num_tokens, a.batch);
     if (a.q_heads < 1 || a.kv_heads < 1 || a.q_heads % a.kv_heads != 0)
@@ -831,25 +814,25 @@ int kvx_attention(const kvx_attention_args *args, int flags, void *stream) {
     p.shared_len = a.shared_len;
     p.rows_limit = INT32_MAX;
     const bool mods = a.softcap > 0.f || a.slopes || !(a.scale > 0.f);
-    cudaStream_t s = static_cast<cudaStream_t>(stream);
+    const Queue queue{static_cast<cudaStream_t>(stream), (flags & KVX_STORE_SERIAL) != 0};
     // Without q_starts every sequence has one query token, whatever bound came with the call.
     const int64_t max_q_len = a.q_starts ? std::max(a.max_q_len, 1) : 1;
     const int64_t q_rows = max_q_len * p.group;  // of the longest sequence and one KV head
     auto rows_kernel = [&](int64_t rows) {
         const int n = rows <= 8 ? 8 : 16;
         if (a.head_dim == 128)
-            return a.dtype == KVX_BF16 ? launch_rows<__nv_bfloat16, 128>(p, n, mods, device, s)
-                                       : launch_rows<__half, 128>(p, n, mods, device, s);
-        return a.dtype == KVX_BF16 ? launch_rows<__nv_bfloat16, 64>(p, n, mods, device, s)
-                                   : launch_rows<__half, 64>(p, n, mods, device, s);
+            return a.dtype == KVX_BF16 ? launch_rows<__nv_bfloat16, 128>(p, n, mods, device, queue)
+                                       : launch_rows<__half, 128>(p, n, mods, device, queue);
+        return a.dtype == KVX_BF16 ? launch_rows<__nv_bfloat16, 64>(p, n, mods, device, queue)
+                                   : launch_rows<__half, 64>(p, n, mods, device, queue);
     };
 
     auto join = [&](int parts, bool mixed) {
         if (a.head_dim == 128)
-            return a.dtype == KVX_BF16 ? launch_join<__nv_bfloat16, 128>(p, parts, mixed, device, s)
-                                       : launch_join<__half, 128>(p, parts, mixed, device, s);
-        return a.dtype == KVX_BF16 ? launch_join<__nv_bfloat16, 64>(p, parts, mixed, device, s)
-                                   : launch_join<__half, 64>(p, parts, mixed, device, s);
+            return a.dtype == KVX_BF16 ? launch_join<__nv_bfloat16, 128>(p, parts, mixed, device, queue)
+                                       : launch_join<__half, 128>(p, parts, mixed, device, queue);
+        return a.dtype == KVX_BF16 ? launch_join<__nv_bfloat16, 64>(p, parts, mixed, device, queue)
+                                   : launch_join<__half, 64>(p, parts, mixed, device, queue);
     };
 
     // ---- which kernel takes what
@@ -864,7 +847,7 @@ int kvx_attention(const kvx_attention_args *args, int flags, void *stream) {
         const int64_t tiles = (a.shared_len + kTileKeys - 1) / kTileKeys;
         const int splits =
             (int)std::max<int64_t>(1, std::min({2 * device.sms / items, (tiles + 1) / 2, kSplitRows / rows - 1}));
-        if (int rc = launch_tiles(p, a.head_dim, a.dtype, mods, true, 1, splits, device, s)) return rc;
+        if (int rc = launch_tiles(p, a.head_dim, a.dtype, mods, true, 1, splits, device, queue)) return rc;
         p.prefix_splits = splits;
         p.shared_len = 0;
         if (int rc = rows_kernel(q_rows)) return rc;
@@ -895,7 +878,7 @@ int kvx_attention(const kvx_attention_args *args, int flags, void *stream) {
         if (items_of(2) * splits * 8 > (int64_t)device.sms * 5) groups = 2;
     }
     if (groups == 1) splits = splits_of(1);
-    if (int rc = launch_tiles(p, a.head_dim, a.dtype, mods, false, groups, splits, device, s)) return rc;
+    if (int rc = launch_tiles(p, a.head_dim, a.dtype, mods, false, groups, splits, device, queue)) return rc;
     if (splits > 1)
         if (int rc = join(splits, mixed)) return rc;
     return mixed ? rows_kernel(p.rows_limit) : KVX_OK;

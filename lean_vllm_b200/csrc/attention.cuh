@@ -52,11 +52,35 @@ struct AllowedSmem {
     }
 };
 
+// Where a call's kernels are launched; serial: each after the one before it, with no overlap.
+struct Queue {
+    cudaStream_t stream;
+    bool serial;
+};
+
+template <class Kernel, class... Args>
+int launch(Kernel kernel, int64_t grid, int threads, int smem, const Queue &queue, const Args &...args) {
+    if (grid > 0x7fffffff) return fail(KVX_ERR_INVALID, "more rows than a launch holds");
+    cudaLaunchConfig_t cfg = {};
+    cfg.stream = queue.stream;
+    cudaLaunchAttribute attr;
+    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr.val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = &attr;
+    cfg.numAttrs = queue.serial ? 0 : 1;
+    cfg.gridDim = dim3((unsigned)grid);
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = smem;
+    KVX_CUDA(cudaLaunchKernelEx(&cfg, kernel, args...));
+    count_launch();
+    return KVX_OK;
+}
+
 // attention_tiles (attention_tiles.cu). `prefix_only`: all query rows against the shared prefix alone; else each
 // sequence's rows above rows_limit. `groups`: tiles of rows per CTA, 1 or 2. It leaves `splits` parts to join, and finished
 // rows when there is one split and it is not prefix_only.
 int launch_tiles(const AttnParams &p, int head_dim, int dtype, bool mods, bool prefix_only, int groups, int splits,
-                 const Device &device, cudaStream_t stream);
+                 const Device &device, const Queue &queue);
 // The tokens of this cache that one of attention_tiles' copies brings; 0 if it cannot take the call (blocks that are no
 // multiple of 8 tokens, strides that no tensor map holds, groups beyond a tile's rows).
 int tile_box(const AttnParams &p);

@@ -982,26 +982,8 @@ int query_map(CUtensorMap *map, const AttnParams &p, int head_dim, int dtype, in
     return encode(map, 3, p.query, dtype, dims, strides, boxes);
 }
 
-template <class Kernel>
-int launch(Kernel kernel, const TileParams &t, int64_t grid, int threads, int smem, cudaStream_t stream) {
-    if (grid > 0x7fffffff) return fail(KVX_ERR_INVALID, "more rows than a launch holds");
-    cudaLaunchConfig_t cfg = {};
-    cfg.stream = stream;
-    cudaLaunchAttribute attr;
-    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr.val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = &attr;
-    cfg.numAttrs = 1;
-    cfg.gridDim = dim3((unsigned)grid);
-    cfg.blockDim = dim3(threads);
-    cfg.dynamicSmemBytes = smem;
-    KVX_CUDA(cudaLaunchKernelEx(&cfg, kernel, t));
-    count_launch();
-    return KVX_OK;
-}
-
 template <class T, int D, int GROUPS, int CTAS, bool MODS>
-int launch_typed(const TileParams &t, const Device &device, cudaStream_t stream) {
+int launch_typed(const TileParams &t, const Device &device, const Queue &queue) {
     static AllowedSmem allowed;
     auto kernel = attention_tiles<T, D, GROUPS, CTAS, MODS>;
     using S = Shape<D, GROUPS, CTAS>;
@@ -1009,21 +991,21 @@ int launch_typed(const TileParams &t, const Device &device, cudaStream_t stream)
     // One wave of CTAs, each taking item after item.
     const int64_t items = (int64_t)t.row_tiles * t.a.kv_heads * t.splits;
     const int64_t grid = std::min<int64_t>(items, (int64_t)device.sms * CTAS);
-    return launch(kernel, t, grid, Warps<GROUPS, CTAS>::kThreads, S::kBytes, stream);
+    return launch(kernel, grid, Warps<GROUPS, CTAS>::kThreads, S::kBytes, queue, t);
 }
 
 template <class T, int D>
-int launch_typed(const TileParams &t, int groups, bool mods, const Device &device, cudaStream_t stream) {
+int launch_typed(const TileParams &t, int groups, bool mods, const Device &device, const Queue &queue) {
     if constexpr (D == 128) {
         if (groups == 2)
-            return mods ? launch_typed<T, D, 2, 1, true>(t, device, stream) : launch_typed<T, D, 2, 1, false>(t, device, stream);
+            return mods ? launch_typed<T, D, 2, 1, true>(t, device, queue) : launch_typed<T, D, 2, 1, false>(t, device, queue);
         // No more items than SMs: a CTA has an SM, and twice the ring, to itself. A prompt of 256 tokens of 32 heads over 8
         // takes 9.5 us so and 10.3 in the other shape, one of 512 12.9 and 14.2 (64 wide: 8.2 and 8.2, 10.7 and 11.1).
         // Behind a shared prefix attention_rows' CTAs start in the room that the smaller ring leaves.
         if (!t.prefix_only && (int64_t)t.row_tiles * t.a.kv_heads * t.splits <= device.sms)
-            return mods ? launch_typed<T, D, 1, 1, true>(t, device, stream) : launch_typed<T, D, 1, 1, false>(t, device, stream);
+            return mods ? launch_typed<T, D, 1, 1, true>(t, device, queue) : launch_typed<T, D, 1, 1, false>(t, device, queue);
     }
-    return mods ? launch_typed<T, D, 1, 2, true>(t, device, stream) : launch_typed<T, D, 1, 2, false>(t, device, stream);
+    return mods ? launch_typed<T, D, 1, 2, true>(t, device, queue) : launch_typed<T, D, 1, 2, false>(t, device, queue);
 }
 
 }  // namespace
@@ -1038,7 +1020,7 @@ int kvx::tile_box(const AttnParams &p) {
 }
 
 int kvx::launch_tiles(const AttnParams &p, int head_dim, int dtype, bool mods, bool prefix_only, int groups,
-                      int splits, const Device &device, cudaStream_t stream) {
+                      int splits, const Device &device, const Queue &queue) {
     TileParams t;
     t.a = p;
     t.box = tile_box(p);
@@ -1052,8 +1034,8 @@ int kvx::launch_tiles(const AttnParams &p, int head_dim, int dtype, bool mods, b
     if (int rc = cache_map(&t.values, p, p.v_cache, head_dim, dtype, t.box)) return rc;
     if (int rc = query_map(&t.queries, p, head_dim, dtype, t.tile_tokens)) return rc;
     if (head_dim == 128)
-        return dtype == KVX_BF16 ? launch_typed<__nv_bfloat16, 128>(t, groups, mods, device, stream)
-                                 : launch_typed<__half, 128>(t, groups, mods, device, stream);
-    return dtype == KVX_BF16 ? launch_typed<__nv_bfloat16, 64>(t, groups, mods, device, stream)
-                             : launch_typed<__half, 64>(t, groups, mods, device, stream);
+        return dtype == KVX_BF16 ? launch_typed<__nv_bfloat16, 128>(t, groups, mods, device, queue)
+                                 : launch_typed<__half, 128>(t, groups, mods, device, queue);
+    return dtype == KVX_BF16 ? launch_typed<__nv_bfloat16, 64>(t, groups, mods, device, queue)
+                             : launch_typed<__half, 64>(t, groups, mods, device, queue);
 }

@@ -6,6 +6,7 @@ import math
 import pytest
 import torch
 
+from lean_vllm_b200._native import STORE_SERIAL
 from lean_vllm_b200.attention.kvx_attention import AttentionWorkspace, paged_attention, shared_prefix_attention
 from lean_vllm_b200.kv_transfer import transport
 from tests.attention_cases import attention64, check_attention, paged_case
@@ -447,6 +448,15 @@ def test_stream_0_is_the_default_stream(workspace):
         assert not side.query()
     torch.cuda.synchronize()
     assert torch.equal(got, want)
+
+
+def test_plain_launches_give_the_same_bits(workspace):
+    for q_lens, kv_lens, shared in (([1, 1], [3000, 50], 0), ([200, 1], [900, 700], 0), ([40], [9000], 0),
+                                    ([1] * 8, [9] * 8, 2000)):
+        case = paged_case(q_lens, kv_lens, 8, 2, 128, 16, BF16, shared=shared)
+        want = run(case, workspace)
+        for _ in range(3):
+            assert torch.equal(run(case, workspace, flags=STORE_SERIAL), want)
 
 
 def test_a_graph_replays_the_call_at_other_lengths(workspace):
