@@ -33,6 +33,13 @@ def output_like(query: torch.Tensor, stream: int | None) -> torch.Tensor:
     return out
 
 
+def no_gradient(*tensors: torch.Tensor | None) -> None:
+    """Refuses tensors whose gradient would be lost: these calls are for serving and have no backward pass."""
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+        raise ValueError("no gradient passes through this call: make it under torch.no_grad() or inference_mode(), or "
+                         "detach its inputs")
+
+
 def call(device: int, function, *args) -> None:
     """Calls a library function that launches on the current device, with `device` as that; raises for an error."""
     if torch.cuda.current_device() == device:

@@ -3,7 +3,8 @@ both, reading the blocks a prefill stored or a transfer brought, in the NHD or H
 
 `paged_attention` is the general call; `shared_prefix_attention` is for a batch whose sequences all begin with the same
 cached prefix, which is read once for all of them. Lengths and block tables stay on the device: no call here waits for
-it. There is no fallback: without libkvx.so the calls raise.
+it. For serving: inputs that require a gradient are refused while gradients are recorded. There is no fallback: without
+libkvx.so the calls raise.
 """
 
 from __future__ import annotations
@@ -12,7 +13,7 @@ import torch
 
 from lean_vllm_b200 import _native
 from lean_vllm_b200._native import check, lib
-from lean_vllm_b200.attention.device import call, calls, output_like, raw_stream, stream_of
+from lean_vllm_b200.attention.device import call, calls, no_gradient, output_like, raw_stream, stream_of
 
 _INT32_MAX = 2**31 - 1
 _DTYPES = {torch.bfloat16: _native.BF16, torch.float16: _native.FP16}
@@ -52,6 +53,7 @@ def _attention(query, k_cache, v_cache, block_tables, kv_lens, scale, q_starts, 
             check(done)
         elif done is not None:
             return done
+    no_gradient(query, k_cache, v_cache, slopes)
     shape, cache_shape = query.shape, k_cache.shape
     if len(shape) != 3 or len(cache_shape) != 4 or cache_shape != v_cache.shape:
         raise ValueError(f"queries {tuple(query.shape)} [num_tokens, heads, dim] over caches {tuple(k_cache.shape)} / "

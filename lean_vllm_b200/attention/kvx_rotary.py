@@ -4,8 +4,8 @@ What an attention layer does to a step's rows between its projections and its at
 norm (where the model has one), the rotation of its pairs by the token's position, and store_kvcache -- here in one
 pass over the rows, with the store's slots, padding, layouts and pushes to decode ranks (PushTarget) unchanged.
 `rotate_store_latents` is the same for a latent-attention model's cached rows, [normed part | rotated part], and the
-rotated part of its queries. Computed in 32 bits and rounded once. There is no fallback: without libkvx.so the calls
-raise.
+rotated part of its queries. Computed in 32 bits and rounded once. For serving: inputs that require a gradient are refused
+while gradients are recorded. There is no fallback: without libkvx.so the calls raise.
 """
 
 from __future__ import annotations
@@ -17,7 +17,7 @@ import torch
 
 from lean_vllm_b200 import _native
 from lean_vllm_b200._native import check, lib
-from lean_vllm_b200.attention.device import call, calls, output_like, raw_stream
+from lean_vllm_b200.attention.device import call, calls, no_gradient, output_like, raw_stream
 from lean_vllm_b200.attention.kvx_cache import PushTarget, _dest, _slots, _target_slots
 
 _DTYPES = {torch.bfloat16: _native.BF16, torch.float16: _native.FP16}
@@ -168,6 +168,7 @@ def rotate_store_kvcache(query: torch.Tensor, key: torch.Tensor, value: torch.Te
             check(done)
         elif done is not None:
             return done
+    no_gradient(query, key, value, q_weight, k_weight, rotary.table)
     if query.dim() != 3 or key.dim() != 3:
         raise ValueError("queries, keys and values are [num_tokens, heads, dim]")
     num_tokens, num_heads, head_dim = key.shape
@@ -228,6 +229,7 @@ def rotate_store_latents(latent: torch.Tensor, latent_cache: torch.Tensor, slot_
             check(done)
         elif done is not None:
             return done if query_pe is not None else None
+    no_gradient(latent, query_pe, weight, rotary.table)
     if latent.dim() != 2 or latent_cache.dim() != 3 or latent_cache.size(2) != latent.size(1):
         raise ValueError(f"latents {tuple(latent.shape)} into a cache {tuple(latent_cache.shape)}")
     num_tokens, dim = latent.shape

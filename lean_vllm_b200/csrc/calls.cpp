@@ -11,12 +11,14 @@
 #include <Python.h>
 
 #include <ATen/ATen.h>
+#include <c10/core/GradMode.h>
 #include <c10/cuda/CUDAFunctions.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <algorithm>
 #include <cmath>
+#include <initializer_list>
 
 #include "kvx.h"
 
@@ -60,6 +62,14 @@ bool number(PyObject *o, double *out) {
     return true;
 }
 
+// Whether a gradient would be lost here, which the wrapper refuses.
+bool loses_gradient(std::initializer_list<const at::Tensor *> tensors) {
+    if (!c10::GradMode::is_enabled()) return false;
+    for (const at::Tensor *t : tensors)
+        if (t && t->requires_grad()) return true;
+    return false;
+}
+
 // A contiguous tensor of `type` on CUDA device `device`.
 bool plain(const at::Tensor &t, at::ScalarType type, int device) {
     return t.is_cuda() && t.get_device() == device && t.scalar_type() == type && t.is_contiguous();
@@ -90,7 +100,8 @@ PyObject *attention(PyObject *, PyObject *const *args, Py_ssize_t n) {
                      *lens = tensor(args[4]), *starts, *slopes, *prefixes, *shared;
     int device;
     if (!q || !k || !v || !tables || !lens || !optional(args[6], &starts) || !optional(args[11], &slopes) ||
-        !optional(args[12], &prefixes) || !optional(args[13], &shared) || !on_current(*q, &device))
+        !optional(args[12], &prefixes) || !optional(args[13], &shared) || !on_current(*q, &device) ||
+        loses_gradient({q, k, v, slopes}))
         Py_RETURN_NONE;
     int64_t max_q, max_kv = 0, window, shared_len, work, work_device, flags, status;
     double scale = 0, softcap;
@@ -218,7 +229,8 @@ PyObject *rotate_store(PyObject *, PyObject *const *args, Py_ssize_t n) {
     int64_t flags, status;
     double eps;
     if (!optional(args[9], &q_weight) || !optional(args[10], &k_weight) || !number(args[11], &eps) ||
-        !integer(args[12], 0, 0xffffffffll, &flags) || !integer(args[13], 0, INT64_MAX, &status) || !on_current(q, &device))
+        !integer(args[12], 0, 0xffffffffll, &flags) || !integer(args[13], 0, INT64_MAX, &status) || !on_current(q, &device) ||
+        loses_gradient({&q, &k, &v, q_weight, k_weight, t[7]}))
         Py_RETURN_NONE;
     const int type = type_of(q);
     if (type < 0 || q.dim() != 3 || k.dim() != 3 || k_cache.dim() != 4 || k.sizes() != v.sizes() ||
@@ -266,7 +278,7 @@ PyObject *rotate_latents(PyObject *, PyObject *const *args, Py_ssize_t n) {
     double eps;
     if (!optional(args[6], &pe) || !optional(args[7], &weight) || !number(args[8], &eps) ||
         !integer(args[9], 0, 0xffffffffll, &flags) || !integer(args[10], 0, INT64_MAX, &status) ||
-        !on_current(latent, &device))
+        !on_current(latent, &device) || loses_gradient({&latent, pe, weight, t[4]}))
         Py_RETURN_NONE;
     const int type = type_of(latent);
     if (type < 0 || latent.dim() != 2 || cache.dim() != 3 || cache.size(2) != latent.size(1) || cache.stride(2) != 1 ||

@@ -130,6 +130,33 @@ def test_shared_prefix_attention_refuses():
                                 args["block_tables"], args["kv_lens"])
 
 
+@pytest.mark.parametrize("call, args, name", [
+    (paged_attention, attention_args, "query"), (paged_attention, attention_args, "k_cache"),
+    (rotate_store_kvcache, store_args, "query"), (rotate_store_kvcache, store_args, "key"),
+    (rotate_store_kvcache, store_args, "value"), (rotate_store_latents, latent_args, "latent"),
+])
+def test_inputs_whose_gradient_would_be_lost_are_refused(call, args, name):
+    given = args()
+    given[name].requires_grad_()
+    with pytest.raises(ValueError, match="no gradient passes"):
+        call(**given)
+    given["out"] = torch.zeros(1)  # with no gradient recorded the checks go on, to this one or the device's
+    with torch.no_grad(), pytest.raises(Exception) as other:
+        call(**given)
+    assert "gradient" not in str(other.value)
+
+
+def test_weights_and_slopes_whose_gradient_would_be_lost_are_refused():
+    weight = torch.ones(64, dtype=BF16, requires_grad=True)
+    for change in (dict(q_weight=weight), dict(k_weight=weight)):
+        with pytest.raises(ValueError, match="no gradient passes"):
+            rotate_store_kvcache(**store_args(**change))
+    with pytest.raises(ValueError, match="no gradient passes"):
+        rotate_store_latents(**latent_args(weight=weight))
+    with pytest.raises(ValueError, match="no gradient passes"):
+        paged_attention(**attention_args(slopes=torch.ones(4, requires_grad=True)))
+
+
 def in_a_thread(fn):
     """fn(), in a thread of its own: the library's last error is per thread, and other tests look at this one's."""
     with ThreadPoolExecutor(1) as pool:

@@ -450,6 +450,18 @@ def test_stream_0_is_the_default_stream(workspace):
     assert torch.equal(got, want)
 
 
+def test_a_gradient_is_refused_not_lost(workspace):
+    case = paged_case([1], [70], 4, 2, 64, 16, BF16)
+    want = run(case, workspace)
+    case["q"].requires_grad_()
+    with pytest.raises(ValueError, match="no gradient passes"):
+        run(case, workspace)
+    with torch.no_grad():
+        assert torch.equal(run(case, workspace), want)
+    with torch.inference_mode():
+        assert torch.equal(run(case, workspace), want)
+
+
 def test_plain_launches_give_the_same_bits(workspace):
     for q_lens, kv_lens, shared in (([1, 1], [3000, 50], 0), ([200, 1], [900, 700], 0), ([40], [9000], 0),
                                     ([1] * 8, [9] * 8, 2000)):

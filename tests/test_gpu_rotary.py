@@ -367,6 +367,19 @@ def test_peers_get_the_latents_too_and_the_push_half_alone(rank, rotary):
     assert torch.equal(call(out=turned), want)
 
 
+def test_a_gradient_is_refused_not_lost():
+    q, k, v, cache, slots, table, at, weights = rows_case(5, 4, 2, 64, 64, 16, torch.bfloat16, fused=False)
+    view = cache.transpose(2, 3)
+    weights[1].requires_grad_()
+    with pytest.raises(ValueError, match="no gradient passes"):
+        rotate_store_kvcache(q, k, v, view[0], view[1], slots, at, table, k_weight=weights[1])
+    with torch.no_grad():
+        rotate_store_kvcache(q, k, v, view[0], view[1], slots, at, table, k_weight=weights[1])
+    latent, rows = torch.zeros(5, 96, dtype=torch.bfloat16, device="cuda", requires_grad=True), view[0].new_zeros(9, 16, 96)
+    with pytest.raises(ValueError, match="no gradient passes"):
+        rotate_store_latents(latent, rows, slots, at, RotaryTable.build(512, 32))
+
+
 def test_a_graph_replays_the_call():
     q, k, v, cache, slots, table, at, weights = rows_case(16, 8, 2, 128, 128, 16, torch.bfloat16, fused=False)
     view = cache.transpose(2, 3)
