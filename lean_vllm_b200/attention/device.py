@@ -50,11 +50,13 @@ def call(device: int, function, *args) -> None:
 
 
 def _bind():
-    """The C++ marshalling of the plain calls (csrc/calls.cpp), bound to the library; None where it is not built: the
-    Python wrappers then do the same, slower."""
+    """The C++ marshalling of the plain calls (csrc/calls.cpp), bound to the library; None where it is not built, or was
+    built against another torch (which may keep it from loading, or not): the Python wrappers then do the same, slower."""
     try:
         from lean_vllm_b200 import _calls
-    except ModuleNotFoundError:
+    except ImportError:
+        return None
+    if getattr(_calls, "torch_version", None) != torch.__version__:
         return None
     handle = lib()
     _calls.bind(ctypes.cast(handle.kvx_attention, ctypes.c_void_p).value,

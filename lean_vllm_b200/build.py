@@ -19,6 +19,7 @@ HEADERS = [os.path.join(ROOT, "include", "kvx.h"),
 OUTPUT = os.path.join(HERE, "libkvx.so")
 CALLS_SOURCE = os.path.join(CSRC, "calls.cpp")
 CALLS = os.path.join(HERE, "_calls" + sysconfig.get_config_var("EXT_SUFFIX"))
+CALLS_TORCH = CALLS + ".torch"  # the torch version it was built against
 
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",
@@ -44,20 +45,24 @@ def stale(output: str = OUTPUT, sources: list[str] | None = None) -> bool:
 
 def build_calls(force: bool = False) -> str:
     """The binding of the calls a decode step makes per layer (csrc/calls.cpp), with g++ against torch's headers."""
-    if not force and not stale(CALLS, [CALLS_SOURCE, HEADERS[0]]):
-        return CALLS
-    from torch.utils import cpp_extension
     import torch
+    from torch.utils import cpp_extension
 
+    if not force and not stale(CALLS, [CALLS_SOURCE, HEADERS[0]]) and os.path.exists(CALLS_TORCH):
+        with open(CALLS_TORCH) as f:
+            if f.read() == torch.__version__:
+                return CALLS
     cuda = os.path.dirname(os.path.dirname(nvcc()))
     includes = [*cpp_extension.include_paths(), sysconfig.get_paths()["include"], os.path.join(cuda, "include"),
                 os.path.join(ROOT, "include")]
     libraries = cpp_extension.library_paths()
     cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}",
-           *(f"-I{i}" for i in includes), "-o", CALLS + ".tmp", CALLS_SOURCE, *(f"-L{d}" for d in libraries),
+           f'-DKVX_TORCH_VERSION="{torch.__version__}"', *(f"-I{i}" for i in includes), "-o", CALLS + ".tmp", CALLS_SOURCE, *(f"-L{d}" for d in libraries),
            "-lc10", "-ltorch_cpu", "-lc10_cuda", "-ltorch_python"]
     subprocess.run(cmd, check=True)
     os.replace(CALLS + ".tmp", CALLS)
+    with open(CALLS_TORCH, "w") as f:
+        f.write(torch.__version__)
     return CALLS
 
 

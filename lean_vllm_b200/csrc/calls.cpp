@@ -350,4 +350,8 @@ PyModuleDef g_module = {PyModuleDef_HEAD_INIT, "_calls", nullptr, -1, g_methods,
 
 }  // namespace
 
-PyMODINIT_FUNC PyInit__calls(void) { return PyModule_Create(&g_module); }
+PyMODINIT_FUNC PyInit__calls(void) {
+    PyObject *module = PyModule_Create(&g_module);
+    if (module && PyModule_AddStringConstant(module, "torch_version", KVX_TORCH_VERSION) != 0) Py_CLEAR(module);
+    return module;
+}

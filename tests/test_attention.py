@@ -320,6 +320,55 @@ def test_rotary_angles():
         RotaryTable.build(4, 7, device="cpu")
 
 
+@pytest.mark.parametrize("kind", ["absent", "does not load", "another torch"])
+def test_a_marshalling_that_is_not_this_torch_s_is_left_alone(kind, monkeypatch):
+    """The wrappers then marshal the calls themselves, and refuse and answer as ever."""
+    import sys
+    import types
+
+    import lean_vllm_b200
+    from lean_vllm_b200.attention import device
+
+    class Broken:  # what the import system meets where a library asks for symbols that another torch had
+        def find_spec(self, name, path=None, target=None):
+            if name == "lean_vllm_b200._calls":
+                raise ModuleNotFoundError(name) if kind == "absent" else ImportError("undefined symbol")
+
+    monkeypatch.delattr(lean_vllm_b200, "_calls", raising=False)
+    if kind == "another torch":
+        other = types.SimpleNamespace(torch_version="1.0", bind=lambda *a: pytest.fail("bound"))
+        monkeypatch.setattr(lean_vllm_b200, "_calls", other, raising=False)
+        monkeypatch.setitem(sys.modules, "lean_vllm_b200._calls", other)
+    else:
+        monkeypatch.delitem(sys.modules, "lean_vllm_b200._calls", raising=False)
+        monkeypatch.setattr(sys, "meta_path", [Broken(), *sys.meta_path])
+    monkeypatch.setattr(device, "_bound", [])
+    assert device.calls() is None
+    with pytest.raises(ValueError, match="kv_lens must be"):
+        paged_attention(**attention_args(kv_lens=torch.ones(4, dtype=torch.int32)))
+
+
+def test_the_binding_is_built_again_for_another_torch(monkeypatch, tmp_path):
+    from lean_vllm_b200 import build
+
+    ran = []
+
+    def compile(cmd, check):
+        ran.append(cmd)
+        open(build.CALLS + ".tmp", "w").close()
+
+    monkeypatch.setattr(build, "CALLS", str(tmp_path / "_calls.so"))
+    monkeypatch.setattr(build, "CALLS_TORCH", str(tmp_path / "_calls.so.torch"))
+    monkeypatch.setattr(build, "nvcc", lambda: "/usr/local/cuda/bin/nvcc")
+    monkeypatch.setattr(build.subprocess, "run", compile)
+    build.build_calls()
+    build.build_calls()
+    assert len(ran) == 1 and f'-DKVX_TORCH_VERSION="{torch.__version__}"' in ran[0]
+    (tmp_path / "_calls.so.torch").write_text("1.0")
+    build.build_calls()
+    assert len(ran) == 2 and (tmp_path / "_calls.so.torch").read_text() == torch.__version__
+
+
 def test_the_native_marshalling_loads_and_leaves_the_rest_to_the_wrappers():
     """Where it is built, the C++ module imports, binds, and answers None to what is not a plain call (CPU tensors)."""
     from lean_vllm_b200 import build
