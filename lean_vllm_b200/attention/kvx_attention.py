@@ -152,7 +152,9 @@ def shared_prefix_attention(query: torch.Tensor, k_cache: torch.Tensor, v_cache:
     """paged_attention for sequences that all begin with the same `prefix_len` cached tokens, in the blocks of
     `prefix_table` (int32): `block_tables` and `kv_lens` hold each sequence's own tokens behind it (the query's
     included), which begin in a block of their own. Every row sees the whole prefix and its sequence's own keys up to
-    its position. The prefix is read once for the batch, not once per sequence."""
+    its position. With up to 128 query rows a sequence and KV head (`max_q_len` times the query heads of one) and blocks of
+    a multiple of 8 tokens, the prefix is read once for the batch (once for every 65,536 rows of it, where it has more),
+    not once per sequence; behind prompts, for each of their tiles of rows."""
     if prefix_len < 0:
         raise ValueError(f"a prefix of {prefix_len} tokens")
     return _attention(query, k_cache, v_cache, block_tables, kv_lens, scale, q_starts, max_q_len, max_kv_len, softcap,

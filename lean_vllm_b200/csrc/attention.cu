@@ -839,19 +839,31 @@ int kvx_attention(const kvx_attention_args *args, int flags, void *stream) {
     if (tile_box(p) == 0) return rows_kernel(q_rows);
     const int64_t rows = (int64_t)a.num_tokens * a.q_heads;
     const int64_t tile_tokens = 128 / p.group;
-    if (a.shared_len > 0 && q_rows <= kTileKeys && 2 * rows <= kSplitRows) {
+    if (a.shared_len > 0 && q_rows <= kTileKeys && 2 * p.q_heads <= kSplitRows) {
         // A prefix shared by short sequences: all their rows together against it, each against its own keys, both joined.
         // One item per CTA: its parts are a part more of every row either way. Items of one tile of rows: 64 requests
-        // behind 8192 tokens take 35.9 us, 36.3 with two tiles (64-wide heads: 27.6 and 28.8).
-        const int64_t items = (a.num_tokens + tile_tokens - 1) / tile_tokens * p.kv_heads;
-        const int64_t tiles = (a.shared_len + kTileKeys - 1) / kTileKeys;
-        const int splits =
-            (int)std::max<int64_t>(1, std::min({2 * device.sms / items, (tiles + 1) / 2, kSplitRows / rows - 1}));
-        if (int rc = launch_tiles(p, a.head_dim, a.dtype, mods, true, 1, splits, device, queue)) return rc;
-        p.prefix_splits = splits;
-        p.shared_len = 0;
-        if (int rc = rows_kernel(q_rows)) return rc;
-        return join(splits + 1, false);
+        // behind 8192 tokens take 35.9 us, 36.3 with two tiles (64-wide heads: 27.6 and 28.8). A batch whose parts pass the
+        // workspace goes in equal runs of tokens, the prefix read once for each.
+        const int64_t runs = (2 * rows + kSplitRows - 1) / kSplitRows;
+        const int run_tokens = (int)((a.num_tokens + runs - 1) / runs);
+        for (int token0 = 0; token0 < a.num_tokens; token0 += run_tokens) {
+            p.token0 = token0;
+            p.num_tokens = std::min(run_tokens, a.num_tokens - token0);
+            p.query = (uint64_t)(uintptr_t)a.query + token0 * a.q_token_stride;
+            p.out = (uint64_t)(uintptr_t)a.out + token0 * a.out_token_stride;
+            const int64_t items = (p.num_tokens + tile_tokens - 1) / tile_tokens * p.kv_heads;
+            const int64_t tiles = (a.shared_len + kTileKeys - 1) / kTileKeys;
+            const int64_t most = kSplitRows / ((int64_t)p.num_tokens * a.q_heads) - 1;
+            const int splits = (int)std::max<int64_t>(1, std::min({2 * device.sms / items, (tiles + 1) / 2, most}));
+            p.prefix_splits = 0;
+            p.shared_len = a.shared_len;
+            if (int rc = launch_tiles(p, a.head_dim, a.dtype, mods, true, 1, splits, device, queue)) return rc;
+            p.prefix_splits = splits;
+            p.shared_len = 0;
+            if (int rc = rows_kernel(q_rows)) return rc;
+            if (int rc = join(splits + 1, false)) return rc;
+        }
+        return KVX_OK;
     }
     if (q_rows <= kRowTile) return rows_kernel(q_rows);
     // Prompt chunks, and beside them (unless every sequence may be one) the sequences of few rows.

@@ -21,6 +21,7 @@ struct AttnParams {
     int64_t table_stride;
     int32_t block_size, block_shift, num_blocks, max_blocks;  // block_shift: log2 of a power-of-two size, else -1
     int32_t batch, num_tokens, q_heads, kv_heads, group;      // group: query heads a KV head
+    int32_t token0;  // of the call's tokens, the launch's first: queries, output and partial results begin there
     int32_t window;
     float scale, softcap;
     // Tokens that every sequence has in front of its own (rows see all of them), in blocks of their own; none when
@@ -91,25 +92,27 @@ constexpr int kRowTile = 16;            // rows of attention_rows' widest tile
 constexpr int kTileKeys = 128;
 constexpr int64_t kSplitRows = 131072;  // rows of partial results the workspace holds
 
-// A sequence's query rows and cached tokens (a shared prefix's first), with its lengths brought into range.
+// A sequence's query rows among the launch's and cached tokens (a shared prefix's first), with its lengths brought into
+// range. Of one whose last query tokens are another launch's, the keys end with those that are here.
 struct Sequence {
     int32_t q0, q_len, kv_len, prefix;
 };
 
 __device__ __forceinline__ Sequence sequence_of(const AttnParams &p, int s) {
     Sequence q;
-    q.q0 = p.q_starts ? p.q_starts[s] : s;
-    q.q_len = p.q_starts ? p.q_starts[s + 1] - q.q0 : 1;
-    q.q0 = max(q.q0, 0);
-    q.q_len = max(0, min(q.q_len, p.num_tokens - q.q0));
+    const int32_t begin = (p.q_starts ? p.q_starts[s] : s) - p.token0;
+    const int32_t end = p.q_starts ? p.q_starts[s + 1] - p.token0 : begin + 1;
+    q.q0 = max(begin, 0);
+    q.q_len = max(0, min(end, p.num_tokens) - q.q0);
     const int64_t room = (int64_t)p.max_blocks * p.block_size;
-    q.kv_len = (int32_t)min((int64_t)max(p.kv_lens[s], 0), room) + p.shared_len;
+    q.kv_len = (int32_t)min((int64_t)max(p.kv_lens[s], 0), room) + p.shared_len - max(0, end - p.num_tokens);
     q.prefix = p.prefix_lens ? min(max(p.prefix_lens[s], 0), q.kv_len) : p.shared_len;
     return q;
 }
 
 // Whose query token `token` is: the last sequence that starts at or before it.
 __device__ __forceinline__ int sequence_at(const AttnParams &p, int token) {
+    token += p.token0;
     if (!p.q_starts) return token;
     int low = 0, high = p.batch;
     while (high - low > 1) {

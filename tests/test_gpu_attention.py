@@ -213,6 +213,33 @@ def test_a_shared_prefix(q_lens, kv_lens, shared, heads, kv_heads, dim, block, d
     check(case, workspace, **options)
 
 
+@pytest.mark.parametrize("q_lens, options", [([1] * 1100, {}), ([3, 1, 2, 4] * 300 + [1], {}),
+                                             ([2, 3] * 250 + [2] * 3, {"slopes": True})],
+                         ids=["single", "drafts", "bias"])
+def test_more_rows_behind_a_prefix_than_parts_fit(q_lens, options, workspace):
+    """A batch that goes in several runs: three launches each, sequences cut between two of them among the checked ones."""
+    heads, options = 64, dict(options)
+    if options:
+        options["slopes"] = 2.0 ** (-8.0 * torch.arange(1, heads + 1, device="cuda") / heads)
+    kv_lens = [n + i % 23 for i, n in enumerate(q_lens)]
+    case = paged_case(q_lens, kv_lens, heads, 4, 64, 16, BF16, shared=300)
+    run(case, workspace, **options)
+    runs = -(-2 * sum(q_lens) * heads // 131072)
+    each = -(-sum(q_lens) // runs)
+    before = transport.launch_count()
+    out = run(case, workspace, **options)
+    assert runs > 1 and transport.launch_count() - before == 3 * runs
+    starts = case["q_starts"].tolist()
+    cut = [s for s in range(len(q_lens)) if starts[s] // each != (starts[s + 1] - 1) // each]
+    assert len(cut) == (0 if max(q_lens) == 1 else runs - 1)
+    chosen = sorted({*range(0, len(q_lens), 97), *cut, len(q_lens) - 1})
+    rows = torch.cat([torch.arange(starts[s], starts[s + 1], device="cuda") for s in chosen])
+    some = dict(case, q=case["q"][rows], q_lens=[q_lens[s] for s in chosen], keys=[case["keys"][s] for s in chosen],
+                values=[case["values"][s] for s in chosen])
+    check_attention(out[rows], some, **options)
+    assert torch.isfinite(out).all()
+
+
 def test_a_shared_prefix_with_nothing_behind_it(workspace):
     """kv_lens of 0: rows that see the prefix alone."""
     case = paged_case([1, 1], [0, 0], 8, 2, 128, 16, BF16, shared=200)
