@@ -710,6 +710,24 @@ class CudaIpcConnectorWorker(KVConnectorWorker):
         self.transport.store(self.kv_caches[layer_index], latent, None, slot_mapping, targets,
                              async_push=envs.LEAN_VLLM_KVX_FUSED_ASYNC, status=word)
 
+    def rotate_store_kv(self, layer_index: int, query, key, value, slot_mapping, positions, rotary, *, q_weight=None,
+                        k_weight=None, eps: float = 1e-6, out=None):
+        """store_kv with the layer's norms and rotation ahead of it in the same pass (rotate_store_kvcache of
+        attention.kvx_rotary, with these decode ranks as its push_to): returns the rotated queries."""
+        targets, word = self._fused_targets(layer_index, latents=False)
+        return self.transport.rotate_store(self.kv_caches[layer_index], query, key, value, slot_mapping, positions, rotary,
+                                           targets, async_push=envs.LEAN_VLLM_KVX_FUSED_ASYNC, status=word,
+                                           q_weight=q_weight, k_weight=k_weight, eps=eps, out=out)
+
+    def rotate_store_latents(self, layer_index: int, latent, slot_mapping, positions, rotary, *, query_pe=None, weight=None,
+                             eps: float = 1e-6, out=None):
+        """store_latents with the latents' norm and rotation ahead of it (rotate_store_latents of attention.kvx_rotary):
+        returns the queries' rotated part, None without queries."""
+        targets, word = self._fused_targets(layer_index, latents=True)
+        return self.transport.rotate_store(self.kv_caches[layer_index], query_pe, latent, None, slot_mapping, positions,
+                                           rotary, targets, async_push=envs.LEAN_VLLM_KVX_FUSED_ASYNC, status=word,
+                                           k_weight=weight, eps=eps, out=out)
+
     def _fused_targets(self, layer_index: int, latents: bool) -> tuple[list, object]:
         """The peer destinations of this layer's store, and the status word the store reports into (None without
         peers): every save whose rows the store writes holds the word until it finishes."""

@@ -235,16 +235,43 @@ class KvxTransport:
                 store_kvcache(key, value, view[0], view[1], slot_mapping, push_to=push_to, stream=stream,
                               flags=flags, status=word)
 
+        self._launch_store(launch, (key, value, slot_mapping), targets, async_push)
+
+    def rotate_store(self, cache: torch.Tensor, query, key: torch.Tensor, value, slot_mapping: torch.Tensor,
+                     positions: torch.Tensor, rotary, targets: list, async_push: bool = False,
+                     status: transport.StatusWord | None = None, q_weight=None, k_weight=None, eps: float = 1e-6,
+                     out=None):
+        """`store`, with the norms and the rotation ahead of it (kvx_rotate_store): returns the rotated queries. Latents
+        when value is None: `query` is then the queries' rotated part, or None, and `k_weight` the latents' norm."""
+        from lean_vllm_b200.attention.kvx_rotary import rotate_store_kvcache, rotate_store_latents
+
+        word = status.address if status is not None else 0
+
+        def launch(push_to, stream=None, flags=0):
+            more = dict(eps=eps, out=None if flags & _native.STORE_PEERS_ONLY else out, push_to=push_to, stream=stream,
+                        flags=flags, status=word)
+            if value is None:
+                return rotate_store_latents(key, cache[0], slot_mapping, positions, rotary, query_pe=query,
+                                            weight=k_weight, **more)
+            view = cache.transpose(2, 3)
+            return rotate_store_kvcache(query, key, value, view[0], view[1], slot_mapping, positions, rotary,
+                                        q_weight=q_weight, k_weight=k_weight, **more)
+
+        return self._launch_store(launch, (key, value, slot_mapping, positions, rotary.table, k_weight),
+                                  targets, async_push)
+
+    def _launch_store(self, launch, inputs: tuple, targets: list, async_push: bool):
+        """launch(push_to, stream, flags) once, or in its two halves."""
         if not targets or not async_push:
-            launch(targets)
-            return
-        launch([])
+            return launch(targets)
+        result = launch([])
         self.save_stream.wait_event(torch.cuda.current_stream(self.device).record_event())
-        for tensor in (key, value, slot_mapping):
+        for tensor in inputs:
             if tensor is not None:
                 tensor.record_stream(self.save_stream)  # the engine may free them once its own store is queued
         budget = min(max(envs.LEAN_VLLM_KVX_SAVE_SMS, 0), 255)
         launch(targets, self.save_stream.cuda_stream, _native.flags(sm_budget=budget) | _native.STORE_PEERS_ONLY)
+        return result
 
     def done(self, xfer: transport.Transfer) -> bool:
         return xfer.done()

@@ -153,6 +153,66 @@ def test_a_fused_store_lands_the_new_rows_in_the_decode_blocks_on_the_gpu(sides,
         assert torch.equal(have[0].transpose(1, 2).reshape(-1, NUM_HEADS, HEAD_DIM)[slots.cpu()], key.cpu())
 
 
+@pytest.mark.parametrize("split", [False, True], ids=["one-launch", "push-on-save-stream"])
+@pytest.mark.parametrize("prefill_tp, decode_tp, mla", [(1, 1, False), (2, 4, False), (1, 2, True)])
+def test_a_rotary_store_lands_the_rotated_rows_in_the_decode_blocks_on_the_gpu(sides, monkeypatch, prefill_tp, decode_tp,
+                                                                               mla, split):
+    """rotate_store_kv and rotate_store_latents: the queries come back, rotated in place, and the local and the decode
+    ranks' blocks hold what the plain call stores elsewhere, bit for bit."""
+    monkeypatch.setenv("LEAN_VLLM_KVX_FUSED_ASYNC", "1" if split else "0")
+    from lean_vllm_b200.attention.kvx_rotary import RotaryTable, rotate_store_kvcache, rotate_store_latents
+    from lean_vllm_b200.kv_transfer import ReqToRecv
+    from lean_vllm_b200.kv_transfer.base import ReqToSave
+    from tests.connector_cases import HEAD_DIM, LATENT_DIM, NUM_HEADS
+
+    prefill, decode = full_cache(0, mla), full_cache(1, mla)
+    producers = sides.make("kv_producer", prefill_tp, prefill)
+    consumers = sides.make("kv_consumer", decode_tp, decode, engine_id="decode", accept_push=True)
+    kv_d, kv_p = consumers[0].kv_transfer, producers[0].kv_transfer
+    local, remote = [7, 2, 9], [0, 5, 3]
+    for c in consumers:
+        c.start_load_kv(KVConnectorMetadata(reqs_to_recv={"d-1": ReqToRecv(
+            remote, local, "p-1", kv_p.engine_id, kv_p.kv_ip, kv_p.kv_port, prefill_tp, pushed=True)}))
+    for p in producers:
+        p.start_load_kv(KVConnectorMetadata(reqs_to_save={"p-1": ReqToSave(
+            local, remote, kv_d.engine_id, kv_d.kv_ip, kv_d.kv_port, decode_tp)}))
+        assert wait_ready(p)
+    g = torch.Generator(device="cuda").manual_seed(3)
+
+    def randn(*shape):
+        return torch.randn(*shape, generator=g, device="cuda").to(torch.bfloat16)
+
+    tokens, per = 3 * BLOCK, NUM_HEADS // prefill_tp
+    slots = torch.tensor([b * BLOCK + o for b in local for o in range(BLOCK)], device="cuda")
+    at = torch.randint(0, 100, (tokens,), generator=g, device="cuda")
+    rotary = RotaryTable.build(100, 4 if mla else HEAD_DIM)
+    for rank, p in enumerate(producers):
+        plain = torch.zeros_like(p.kv_caches[0])
+        if mla:
+            latent, query = randn(tokens, LATENT_DIM), randn(tokens, 3, 4)
+            weight = randn(LATENT_DIM - 4)
+            want = rotate_store_latents(latent, plain[0], slots, at, rotary, query_pe=query, weight=weight)
+            got = p.rotate_store_latents(0, latent, slots, at, rotary, query_pe=query, weight=weight, out=query)
+        else:
+            query, (key, value) = randn(tokens, 2 * per, HEAD_DIM), (randn(tokens, per, HEAD_DIM) for _ in range(2))
+            weights = dict(q_weight=randn(HEAD_DIM), k_weight=randn(HEAD_DIM))
+            view = plain.transpose(2, 3)
+            want = rotate_store_kvcache(query, key, value, view[0], view[1], slots, at, rotary, **weights)
+            got = p.rotate_store_kv(0, query, key, value, slots, at, rotary, out=query, **weights)
+        assert got is query
+        torch.cuda.synchronize()
+        assert torch.equal(got, want) and torch.equal(p.kv_caches[0][:, local], plain[:, local])
+    for p in producers:
+        p.start_load_kv(KVConnectorMetadata(reqs_to_send={"p-1": local}))
+    assert all(wait_for(p).finished_sending == {"p-1"} for p in producers)
+    assert all(wait_for(c).finished_recving == {"d-1"} for c in consumers)
+    have = full_of([p.kv_caches[0].cpu() for p in producers], mla)
+    got = full_of([c.kv_caches[0].cpu() for c in consumers], mla)
+    want = decode.clone()
+    want[:, remote] = have[:, local]
+    assert torch.equal(got, want)
+
+
 def test_a_chunked_prefill_lands_its_final_blocks_on_the_gpu(sides):
     """Three chunks ending inside blocks, each written on the engine's stream behind a long kernel before its layer
     hooks run: every chunk re-pushes the partly filled block on the save stream, in order, so the decode blocks
