@@ -8,6 +8,7 @@
 // (attention_tiles, whose m may lag), far from the type's ends.
 
 #include <algorithm>
+#include <cmath>
 
 #include "attention.cuh"
 
@@ -750,6 +751,7 @@ int kvx_attention(const kvx_attention_args *args, int flags, void *stream) {
     if ((int64_t)a.max_blocks * a.block_size + a.shared_len > ((int64_t)1 << 31) - 1024)
         return fail(KVX_ERR_INVALID, "more than 2^31 - 1024 tokens a sequence");
     if (a.window < 0 || !(a.softcap >= 0.f)) return fail(KVX_ERR_INVALID, "negative window or softcap");
+    if (std::isinf(a.softcap)) return fail(KVX_ERR_INVALID, "an infinite softcap; 0 is none");
     if ((int64_t)a.shared_blocks * a.block_size < a.shared_len)
         return fail(KVX_ERR_RANGE, "a shared prefix of %d tokens in %d blocks of %d", a.shared_len, a.shared_blocks,
                     a.block_size);

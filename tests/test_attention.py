@@ -214,6 +214,15 @@ def test_the_abi_refuses_sequences_whose_positions_pass_31_bits(change):
         in_a_thread(lambda: _native.check(_native.lib().kvx_attention(ctypes.addressof(struct), 0, None)))
 
 
+def test_the_abi_refuses_an_infinite_cap():
+    """inf * tanh(s / inf) is no number."""
+    if not os.path.exists(_native.LIB_PATH):
+        pytest.skip("libkvx.so is not built here")
+    with pytest.raises(_native.KvxError, match="infinite softcap"):
+        struct = attention_struct(softcap=math.inf)
+        in_a_thread(lambda: _native.check(_native.lib().kvx_attention(ctypes.addressof(struct), 0, None)))
+
+
 @pytest.mark.parametrize("flags", [_native.STORE_PEERS_ONLY, 2, 8 << 24, -1])
 def test_the_abi_refuses_flags_that_attention_does_not_have(flags):
     if not os.path.exists(_native.LIB_PATH):
