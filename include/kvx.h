@@ -279,10 +279,11 @@ uint64_t kvx_attention_workspace_bytes(void);
 /* Softmax attention of each sequence's query tokens over its keys and values in the paged cache. Query token i of n,
  * in a sequence of kv_len, stands at position kv_len - n + i and sees position j when j <= its own, when the window
  * holds it, or when j is below the sequence's prefix; a shared prefix lies in front of every sequence's own tokens,
- * and every row sees all of it; up to 128 query rows of a sequence and KV head (max_q_len * q_heads / kv_heads) and blocks
- * of a multiple of 8 tokens, it is read once for every 65,536 rows (num_tokens * q_heads) of the batch. A row that sees nothing gets zeros. Tokens at or past kv_len are never read as numbers;
- * a block id outside the cache reads as zeros and is flagged. No counterpart in the reference's transfer path: it is
- * what its attention layers read the cache with. `flags`: 0, or KVX_STORE_SERIAL for plain launches; others are refused. */
+ * and every row sees all of it; up to 128 query rows of a sequence and KV head (max_q_len * q_heads / kv_heads) and
+ * blocks of a multiple of 8 tokens, it is read once for every 65,536 rows (num_tokens * q_heads) of the batch. A row
+ * that sees nothing gets zeros. Tokens at or past kv_len are never read as numbers; a block id outside the cache reads
+ * as zeros and is flagged. No counterpart in the reference's transfer path: it is what its attention layers read the
+ * cache with. `flags`: 0, or KVX_STORE_SERIAL for plain launches; others are refused. */
 int kvx_attention(const kvx_attention_args *args, int flags, void *stream);
 
 /* ---- transfers with completion (post, poll, release) ---- */

@@ -124,7 +124,7 @@ def paged_attention(query: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.T
     """Attention of queries [num_tokens, heads, dim] over [num_blocks, block_size, kv_heads, dim] caches (HND caches by
     their transposed view), through int32 `block_tables` [batch, blocks] and `kv_lens` [batch] (cached tokens, the
     query's own included). One query token per sequence, or those from q_starts[s] to q_starts[s + 1] (int32,
-    [batch + 1]), of which the last stands at the sequence's last position.
+    [batch + 1]), of which the last stands at the sequence's last position. Query tokens of no sequence get no defined output.
 
     A row sees the keys up to its own position; with `window`, only the last `window` of them; with `prefix_lens` (int32
     [batch]), also every key below its sequence's, whatever its position. Scores are `scale` (1/sqrt(dim)) times q.k,

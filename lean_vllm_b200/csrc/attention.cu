@@ -30,9 +30,13 @@ using namespace kvx;
 // Inside a CTA each of the 4 warps takes its own 16 tokens of every tile with its own running maximum, sum and output,
 // and loads them itself with cp.async into its own ring: no barrier until the group's end.
 //
-// Bound by HBM: 64 ragged requests of up to 16k tokens (957 MB) take 160 us, 6.0 TB/s; one of 131k 94 us, 5.7 TB/s: the
-// walks end after 70 to 75 us on most SMs and 80 to 87 on the others, and 7 are the join of 55 parts a head. One request
-// of 317 tokens takes 7.6 us, a chain of waits: the launch, lengths, table, keys (0.5 us each) and the join of 5 parts.
+// Bound by HBM (graph-replayed times; calls take 0 to 3 us more): 64 ragged requests of up to 16k tokens (957 MB) take 156
+// us, 6.1 TB/s; one of 131k 94 us, 5.7 TB/s: the walks end after 70 to 75 us on most SMs and 80 to 87 on the others, and 7
+// are the join of 55 parts a head. 16 requests of 4 drafts over 8192 tokens (16 rows) take 95 us, 5.6 TB/s. One request of
+// 317 tokens takes 7.2 us, a chain of waits: the launch, lengths, table, keys (0.5 us each) and the join of 5 parts.
+//
+// A window and a prefix mask leave keys between them that no row sees: the walk skips their tiles and fills what remains of
+// them with zeros. A token with a window of 1024 and a prefix of 64 takes 9 us over 8k, 32k and 131k cached tokens alike.
 //
 // Up to 8 rows the products run transposed, S^T = K Q^T and O^T = V^T P^T, with the rows as the tensor cores' 8 columns:
 // half the instructions and registers of a 16-row tile that would be half padding.

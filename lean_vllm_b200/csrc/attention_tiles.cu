@@ -19,7 +19,8 @@
 // items (lookup, queries, first keys, output), a quarter of a prompt of 8192 tokens.
 //
 // Bound by the tensor cores as the power limit lets them run: a prompt of 8192 tokens of 32 heads over 8, 128 wide, takes
-// 470 us, 1170 TFLOP/s, 71% of a large cuBLAS product's rate. A pair of tiles takes 3300 cycles where its products alone
+// 458 to 477 us graph-replayed, 1150 to 1200 TFLOP/s, 70 to 73% of a large cuBLAS product's rate, and 510 to 550 called back
+// to back, with the clock lower still. A pair of tiles takes 3300 cycles where its products alone
 // take 2048: each waits 1250 for the other's (768 of them its own last half and next scores) and spends 2000 in the
 // softmax, half of that on the special-function unit. A third of the exponentials on the multiply-add pipe instead made
 // that shorter and the whole no faster (498 us); an issuing warp for each tile let both fall into step and contend (499).
@@ -43,7 +44,8 @@ using namespace kvx;
 //
 // Registers. A row's 128 scores want more than the launch gives each thread, the other warps less. Two tiles, one CTA per
 // SM: 256 x 224 + 128 x 56 = 64512, the launch's 384 x 168. One tile, two CTAs: 128 x 200 + 128 x 56 = 32768, 256 x 128;
-// one CTA: 128 x 224 + 128 x 56, of the launch's 256 x 224.
+// one CTA: 128 x 224 + 128 x 56, of the launch's 256 x 224. (128 wide, that is less than ptxas wants: it spills 48 to 64 bytes
+// a thread with two tiles, 200 with one tile on each of two CTAs, where an item's end holds all of its output at once.)
 template <int GROUPS, int CTAS>
 struct Warps {
     static constexpr int kSoftmax = 4 * GROUPS, kIssue = kSoftmax, kLoad = kSoftmax + 1, kQuery = kSoftmax + 2,
@@ -1001,7 +1003,8 @@ int launch_typed(const TileParams &t, int groups, bool mods, const Device &devic
             return mods ? launch_typed<T, D, 2, 1, true>(t, device, queue) : launch_typed<T, D, 2, 1, false>(t, device, queue);
         // No more items than SMs: a CTA has an SM, and twice the ring, to itself. A prompt of 256 tokens of 32 heads over 8
         // takes 9.5 us so and 10.3 in the other shape, one of 512 12.9 and 14.2 (64 wide: 8.2 and 8.2, 10.7 and 11.1).
-        // Behind a shared prefix attention_rows' CTAs start in the room that the smaller ring leaves.
+        // Behind a shared prefix two CTAs per SM are ahead: 64 requests behind 8192 tokens take 37.7 us so and 39.9 in this
+        // shape, 5 of 4 drafts behind 30,011 44.4 and 49.0.
         if (!t.prefix_only && (int64_t)t.row_tiles * t.a.kv_heads * t.splits <= device.sms)
             return mods ? launch_typed<T, D, 1, 1, true>(t, device, queue) : launch_typed<T, D, 1, 1, false>(t, device, queue);
     }
