@@ -506,6 +506,8 @@ attention_tiles(const __grid_constant__ TileParams t) {
             // Until a tile is not. (Under a negative scale the capped scores fall as the products rise, and a tile's maximum
             // would be its smallest product: those take the way through TMEM.)
             bool look_near = MODS && p.softcap > 0.f && p.scale > 0.f && !p.slopes;
+            // Rows that are none have no say: what is in them is left from before, and the two ways round differently.
+            const float reach = valid ? near.reach : INFINITY;
             for (int i = 0; i < item.tiles; ++i) {
                 const TileAt at = tile_at(item, i);
                 if (!warp_waits(smem_u32(&scores[g]), score_phase, &gave_up)) {
@@ -530,7 +532,7 @@ attention_tiles(const __grid_constant__ TileParams t) {
                     float most = 0.f;
 #pragma unroll
                     for (int c = 0; c < 4; ++c) most = most_of(most, x[c]);
-                    near_tile = look_near = __all_sync(~0u, most <= near.reach);
+                    near_tile = look_near = __all_sync(~0u, most <= reach);
                 }
                 if ((MODS || masked) && !near_tile) {
                     int from = (at.front ? 0 : see_lo) - at.t0, to = (at.front ? at.hi : see_hi) - at.t0;
@@ -549,7 +551,7 @@ attention_tiles(const __grid_constant__ TileParams t) {
                                     for (int e = 0; e < 32; ++e)
                                         if (!(seen >> e & 1)) y[e] = 0.f;
                                 }
-                                if (__all_sync(~0u, most_of(0.f, y) <= near.reach)) {
+                                if (__all_sync(~0u, most_of(0.f, y) <= reach)) {
 #pragma unroll
                                     for (int e = 0; e < 32; e += 2) {
                                         const float2 v = near.cap(make_float2(y[e], y[e + 1]), make_float2(0.f, 0.f));

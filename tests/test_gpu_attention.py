@@ -128,6 +128,29 @@ def test_caps_near_and_far(q_lens, kv_lens, heads, kv_heads, dim, dtype, shared,
         check(case, workspace, softcap=softcap, **(dict(window=window) if window else {}))
 
 
+@pytest.mark.parametrize("kv_heads, group", [(3, 7), (2, 20), (4, 3), (2, 5)])
+@pytest.mark.parametrize("q_lens, kv_lens, dim, shared, window", [
+    ([300], [900], 128, 0, 0), ([90], [971], 128, 0, 0), ([300, 40], [900, 500], 64, 0, 0), ([300], [900], 128, 0, 120),
+    ([3] * 20, [30] * 20, 128, 700, 0), ([3] * 20, [30] * 20, 64, 700, 0),
+], ids=["prompt", "short", "chunks64", "window", "shared", "shared64"])
+def test_what_ran_before_a_capped_call_changes_no_bit(kv_heads, group, q_lens, kv_lens, dim, shared, window, workspace):
+    """Tiles of 128 rows that groups of 3, 5, 7 or 20 heads do not fill: what is left in their last rows from a call before,
+    queries near the cap or far beyond it, is no row's business."""
+    options = dict(softcap=50.0, **(dict(window=window) if window else {}))
+    case = paged_case(q_lens, kv_lens, kv_heads * group, kv_heads, dim, 16, BF16, shared=shared)
+    filler = paged_case([400] * 8, [400] * 8, 8 * kv_heads, kv_heads, dim, 16, BF16)
+    seen = []
+    for factor in (0.0, 1000.0, 0.0, 1000.0):
+        filler["q"].fill_(factor)
+        run(filler, workspace)
+        fill = paged_case([16] * 20, [16] * 20, 8 * kv_heads, kv_heads, dim, 16, BF16, shared=300)
+        fill["q"].fill_(factor)
+        run(fill, workspace)
+        seen.append(run(case, workspace, **options))
+    check_attention(seen[0], case, **options)
+    assert all(torch.equal(x, seen[0]) for x in seen)
+
+
 @pytest.mark.parametrize("dim", [64, 128])
 @pytest.mark.parametrize("q_lens, kv_lens, heads, shared", [
     ([1], [20000], 4, 0), ([4], [20000], 4, 0), ([3, 1], [9000, 17], 1, 0),  # one walk of the cache in hundreds of parts
