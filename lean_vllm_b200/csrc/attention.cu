@@ -303,11 +303,17 @@ attention_rows(const __grid_constant__ AttnParams p) {
             if (row >= rows) return 0;
             return p.query + (int64_t)(q.q0 + token_of(row)) * p.q_token_stride + (int64_t)head_of(row) * p.q_head_stride;
         };
+        // Stage i's first token, and which tokens are there: those from the window's first on, or (the modified form, which
+        // calls with a window and a prefix take) all but those between the prefix and the window. One comparison instead of
+        // two brings 64 ragged requests from 162 to 157 us.
+        const int token0 = (tile0 + (MODS ? 0 : work.skip)) * kTileTokens + warp * kWarpTokens;
         auto stage_token = [&](int i) {
-            return (tile0 + i + (tile0 + i >= work.front ? work.skip : 0)) * kTileTokens + warp * kWarpTokens;
+            return token0 + (i + (MODS && tile0 + i >= work.front ? work.skip : 0)) * kTileTokens;
         };
-        const uint32_t gap = max(0, work.lo - q.prefix);  // tokens between the prefix and the window
-        auto readable = [&](int t) { return t < q.kv_len && (uint32_t)(t - q.prefix) >= gap; };
+        const uint32_t gap = max(0, work.lo - q.prefix), span = max(0, q.kv_len - work.lo);
+        auto readable = [&](int t) {
+            return MODS ? t < q.kv_len && (uint32_t)(t - q.prefix) >= gap : (uint32_t)(t - work.lo) < span;
+        };
         const int64_t lane_from = (int64_t)h * p.head_stride +
                                   (stage_in_block ? (lane / kChunks) * p.token_stride + (lane % kChunks) * 16 : 0);
 
@@ -317,7 +323,7 @@ attention_rows(const __grid_constant__ AttnParams p) {
             if (i >= n_tiles) return -1;
             const int t = stage_token(i) + (stage_in_block ? 0 : lane);
             // (Of a stage in one block some token has to be there, so that the block's id is one.)
-            if (stage_in_block ? t >= q.kv_len || (t + kWarpTokens <= work.lo && t >= q.prefix)
+            if (stage_in_block ? t >= q.kv_len || (t + kWarpTokens <= work.lo && (!MODS || t >= q.prefix))
                                : lane >= kWarpTokens || !readable(t))
                 return -1;
             const int64_t at = token_at(p, s, t);
@@ -824,13 +830,14 @@ int kvx_attention(const kvx_attention_args *args, int flags, void *stream) {
     // Without q_starts every sequence has one query token, whatever bound came with the call.
     const int64_t max_q_len = a.q_starts ? std::max(a.max_q_len, 1) : 1;
     const int64_t q_rows = max_q_len * p.group;  // of the longest sequence and one KV head
+    const bool row_mods = mods || (a.window > 0 && a.prefix_lens);
     auto rows_kernel = [&](int64_t rows) {
         const int n = rows <= 8 ? 8 : 16;
         if (a.head_dim == 128)
-            return a.dtype == KVX_BF16 ? launch_rows<__nv_bfloat16, 128>(p, n, mods, device, queue)
-                                       : launch_rows<__half, 128>(p, n, mods, device, queue);
-        return a.dtype == KVX_BF16 ? launch_rows<__nv_bfloat16, 64>(p, n, mods, device, queue)
-                                   : launch_rows<__half, 64>(p, n, mods, device, queue);
+            return a.dtype == KVX_BF16 ? launch_rows<__nv_bfloat16, 128>(p, n, row_mods, device, queue)
+                                       : launch_rows<__half, 128>(p, n, row_mods, device, queue);
+        return a.dtype == KVX_BF16 ? launch_rows<__nv_bfloat16, 64>(p, n, row_mods, device, queue)
+                                   : launch_rows<__half, 64>(p, n, row_mods, device, queue);
     };
 
     auto join = [&](int parts, bool mixed) {
