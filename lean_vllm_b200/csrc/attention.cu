@@ -31,8 +31,8 @@ using namespace kvx;
 // and loads them itself with cp.async into its own ring: no barrier until the group's end.
 //
 // Bound by HBM (graph-replayed times; calls take 0 to 3 us more): 64 ragged requests of up to 16k tokens (957 MB) take 156
-// us, 6.1 TB/s; one of 131k 94 us, 5.7 TB/s: the walks end after 70 to 75 us on most SMs and 80 to 87 on the others, and 7
-// are the join of 55 parts a head. 16 requests of 4 drafts over 8192 tokens (16 rows) take 95 us, 5.6 TB/s. One request of
+// us, 6.1 TB/s; one of 131k 92 us, 5.8 TB/s: the walks end after 70 to 75 us on most SMs and 80 to 87 on the others, and 7
+// are the join of 55 parts a head. 16 requests of 4 drafts over 8192 tokens (16 rows) take 96 us, 5.6 TB/s. One request of
 // 317 tokens takes 7.2 us, a chain of waits: the launch, lengths, table, keys (0.5 us each) and the join of 5 parts.
 //
 // A window and a prefix mask leave keys between them that no row sees: the walk skips their tiles and fills what remains of
